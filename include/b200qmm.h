@@ -236,9 +236,81 @@ int b2_route_topk_dev(b2_ctx* ctx, const float* logits_dev, size_t t, size_t n_e
 int b2_prepare_x_dev(b2_ctx* ctx, const float* x_dev, size_t n_in);
 int b2_matvec_prepared_dev(b2_ctx* ctx, b2_weight w, b2_weight up, const float* x_dev, float* y_dev, int mode, const float* gate_dev);
 
+/* ---- a cache of 8-bit keys and values, and attention over it (device-resident; no counterpart in the reference, whose caches are f32) ----
+ * The pool holds n_blocks blocks of B2_KV8_BLOCK tokens; a value is an integer of -127 .. 127 times a power of two, one for each block, KV head and kind
+ * (keys, values): scale = 2^e, e the smallest (at least -100) with the largest magnitude <= 127 * 2^e, integers rounded to nearest even (at 2^122 at most 63: the value stays finite). Rows that go into a
+ * partly filled block keep the scale of the rows ahead of them, unless theirs is larger: the rows ahead are then brought to it by the same rounding, so one
+ * append of several rows and several appends of one can differ in the last bit of an integer. A row (token, head, kind) with a value that is not finite
+ * counts as NaN in all of its values, and changes no other row. hd is 64 or 128 (others are declined). Bytes: (64 hd + 32) n_blocks nkv. */
+#define B2_KV8_BLOCK 32
+typedef uint64_t b2_kv8;
+int b2_kv8_create(b2_ctx* ctx, size_t nkv, size_t hd, size_t n_blocks, b2_kv8* out);
+/* Waits for the context's stream; work on other streams that uses the pool has to be over. */
+int b2_kv8_free(b2_ctx* ctx, b2_kv8 kv);
+size_t b2_kv8_bytes(b2_ctx* ctx, b2_kv8 kv);
+/* The sequences of a call; the arrays are on the device. Rows rows[s] .. rows[s + 1] - 1 of the call's arrays are sequence s's (rows == NULL: max_rows each,
+ * n_rows = n_seqs * max_rows), at positions start[s], start[s] + 1, ...; a sequence may have none. Its block b (positions 32 b ..) is block
+ * table[s * max_blocks + b] of the pool (table == NULL: s * max_blocks + b). max_rows is the most rows of a sequence as far as the host knows (more rows
+ * cost time, nothing else). What the arrays say is checked where it is used: a sequence outside n_rows or max_blocks * 32 positions is left out, a block
+ * that the pool does not have is not touched, and b2_check_status returns B2_ERR_ARG once the stream is synchronized; the call's results are not valid then. */
+typedef struct b2_kv8_seqs {
+    uint32_t n_seqs;
+    uint32_t n_rows;
+    uint32_t max_rows;
+    uint32_t max_blocks;
+    const int32_t* table;
+    const int32_t* start;
+    const int32_t* rows;
+} b2_kv8_seqs;
+/* Keys and values of the rows into the pool: k_dev and v_dev of `dtype` (B2_F32 / B2_BF16 / B2_F16), head h of row r at r * row_stride + h * head_stride
+ * (elements), hd values side by side. Rows of a block behind the new ones are undefined until they are written. No two sequences of a call may append to one block. */
+int b2_kv8_append_dev(b2_ctx* ctx, b2_kv8 kv, const b2_kv8_seqs* seqs, const void* k_dev, const void* v_dev, int dtype, size_t row_stride, size_t head_stride);
+/* The values that the rows stand for, f32 [n_rows][nkv][hd] each; rows that no sequence has stay as they were. */
+int b2_kv8_read_dev(b2_ctx* ctx, b2_kv8 kv, const b2_kv8_seqs* seqs, float* k_dev, float* v_dev);
+/* Row i of sequence s is a query of nh heads at position p = start[s] + i over the sequence's keys 0 .. start[s] + its rows - 1 (which are in the pool by
+ * then): key j is seen where j <= p or j < prefix[s], and, with a window, p - j < window. Query head h reads KV head h / (nh / nkv).
+ *   score = cap * tanh(scale * q.k / cap) + slopes[h] * (j - p)
+ * (cap 0: scale * q.k; slopes NULL: no bias; prefix NULL: 0 each; window 0: none). q_dev and out_dev of `dtype`, rows of nh * hd values, a row q_stride /
+ * out_stride elements behind the one ahead; out_dev may be q_dev. f32 results, and those of up to eight rows a KV head, have f32-like accuracy (22 bits of queries
+ * and probabilities); more f16 / bf16 rows are multiplied as f16 with f32 sums. A row that sees nothing gives zeros; rows that no sequence has stay as they were. */
+typedef struct b2_kv8_attention {
+    uint32_t nh;
+    float scale;
+    float cap;
+    uint32_t window;
+    const float* slopes;   /* device [nh] or NULL */
+    const int32_t* prefix; /* device [n_seqs] or NULL */
+} b2_kv8_attention;
+int b2_attend_kv8_dev(b2_ctx* ctx, b2_kv8 kv, const b2_kv8_seqs* seqs, const b2_kv8_attention* attention, const void* q_dev, size_t q_stride, void* out_dev,
+                      size_t out_stride, int dtype);
+
+/* ---- rules on logits, and the greedy choice (device-resident; the reference does this on the host, src/sampler.rs) ----
+ * For each of t rows of n logits, in this order, every operation rounded to f32:
+ *   1. a token that the row's history holds c > 0 times: l = l > 0 ? l / repeat : l * repeat, then l = l - (frequency * c + presence);
+ *   2. a token of the row's bias list: l = l + bias (of a token given twice, the last entry);
+ *   3. a token that the mask does not allow: -inf.
+ * out_dev (may be logits_dev, or NULL) receives the rows, rounded to `dtype`; pick_dev[r] (may be NULL) the first of the largest as they are stored, -1 where none is
+ * above -inf (NaN is never chosen). Row r's history is history[history_ptr[r]] .. history[history_ptr[r + 1] - 1], of n_history in all (history_ptr NULL: all
+ * of it for every row); the same for the biases. Ids outside 0 .. n - 1 are left out. Bit i % 32 of word i / 32 of a row's mask allows token i; a row's
+ * mask lies mask_stride words behind the one ahead (0: one mask for all rows). Lists and mask are on the device. A row whose part of a list lies outside it has
+ * none, and b2_check_status returns B2_ERR_ARG. */
+typedef struct b2_logit_rules {
+    float repeat, frequency, presence; /* 1, 0, 0: the history changes nothing */
+    uint32_t n_history, n_bias;
+    const int32_t* history;
+    const int32_t* history_ptr; /* [t + 1] or NULL */
+    const int32_t* bias_ids;
+    const float* bias;
+    const int32_t* bias_ptr; /* [t + 1] or NULL */
+    const uint32_t* mask;    /* or NULL */
+    size_t mask_stride;
+} b2_logit_rules;
+int b2_logits_dev(b2_ctx* ctx, const void* logits_dev, void* out_dev, int dtype, size_t t, size_t n, size_t logits_stride, size_t out_stride,
+                  const b2_logit_rules* rules, int32_t* pick_dev);
+
 /* After the caller has synchronized the stream: B2_OK, or B2_ERR_TIMEOUT when a device-side wait of
  * a product ran into its time limit (the kernel then returned early and its output is
- * not valid). The reference logs a failed launch and returns false (src/cuda.rs:625-628); this is
+ * not valid), or B2_ERR_ARG when a call's device arrays did not fit its host arguments (the 8-bit cache, rules on logits). The reference logs a failed launch and returns false (src/cuda.rs:625-628); this is
  * the same report for the device-resident calls, which do not synchronize themselves. */
 int b2_check_status(b2_ctx* ctx);
 /* For tests of a host program's handling of such failures (no counterpart in the reference): leaves, from the host, the mark that a

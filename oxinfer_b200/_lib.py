@@ -35,6 +35,27 @@ class View(C.Structure):
     _fields_ = [("buf", C.c_uint32), ("off", C.c_uint32)]
 
 
+class Kv8Seqs(C.Structure):
+    """``b2_kv8_seqs``."""
+
+    _fields_ = [("n_seqs", C.c_uint32), ("n_rows", C.c_uint32), ("max_rows", C.c_uint32), ("max_blocks", C.c_uint32), ("table", C.c_void_p),
+                ("start", C.c_void_p), ("rows", C.c_void_p)]
+
+
+class Kv8Attention(C.Structure):
+    """``b2_kv8_attention``."""
+
+    _fields_ = [("nh", C.c_uint32), ("scale", C.c_float), ("cap", C.c_float), ("window", C.c_uint32), ("slopes", C.c_void_p), ("prefix", C.c_void_p)]
+
+
+class LogitRules(C.Structure):
+    """``b2_logit_rules``."""
+
+    _fields_ = [("repeat", C.c_float), ("frequency", C.c_float), ("presence", C.c_float), ("n_history", C.c_uint32), ("n_bias", C.c_uint32),
+                ("history", C.c_void_p), ("history_ptr", C.c_void_p), ("bias_ids", C.c_void_p), ("bias", C.c_void_p), ("bias_ptr", C.c_void_p),
+                ("mask", C.c_void_p), ("mask_stride", C.c_size_t)]
+
+
 OP_NORM, OP_LINEAR, OP_QK_ROPE, OP_ATTEND, OP_GLU, OP_EXCHANGE = 1, 2, 3, 4, 5, 6
 PLAN_HANDLE_BYTES = 128
 COMM_ID_BYTES = 128
@@ -109,6 +130,15 @@ _SIGNATURES = {
     "b2_matvec_rows": (C.c_int, [C.c_void_p, C.c_void_p, C.c_size_t, C.c_size_t, C.POINTER(RowsJob), C.c_size_t]),
     "b2_matmul_dev": (C.c_int, [C.c_void_p, C.c_uint64, C.c_void_p, C.c_int, C.c_size_t, C.c_void_p, C.c_int]),
     "b2_matvec_dev": (C.c_int, [C.c_void_p, C.c_uint64, C.c_uint64, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p]),
+    "b2_kv8_create": (C.c_int, [C.c_void_p, C.c_size_t, C.c_size_t, C.c_size_t, C.POINTER(C.c_uint64)]),
+    "b2_kv8_free": (C.c_int, [C.c_void_p, C.c_uint64]),
+    "b2_kv8_bytes": (C.c_size_t, [C.c_void_p, C.c_uint64]),
+    "b2_kv8_append_dev": (C.c_int, [C.c_void_p, C.c_uint64, C.POINTER(Kv8Seqs), C.c_void_p, C.c_void_p, C.c_int, C.c_size_t, C.c_size_t]),
+    "b2_kv8_read_dev": (C.c_int, [C.c_void_p, C.c_uint64, C.POINTER(Kv8Seqs), C.c_void_p, C.c_void_p]),
+    "b2_attend_kv8_dev": (C.c_int, [C.c_void_p, C.c_uint64, C.POINTER(Kv8Seqs), C.POINTER(Kv8Attention), C.c_void_p, C.c_size_t, C.c_void_p, C.c_size_t,
+                                    C.c_int]),
+    "b2_logits_dev": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_size_t, C.c_size_t, C.c_size_t, C.c_size_t, C.POINTER(LogitRules),
+                                C.c_void_p]),
     "b2_check_status": (C.c_int, [C.c_void_p]),
     "b2_inject_timeout": (C.c_int, [C.c_void_p, C.c_uint64]),
     "b2_upload_moe": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_size_t, C.c_size_t, C.POINTER(C.c_uint64)]),

@@ -316,6 +316,31 @@ class Backend:
         t, n = logits.shape
         return self._check(self._L.b2_route_topk_dev(self._ctx, _ptr(logits), t, n, k, _ptr(ids), _ptr(w)))
 
+    # -- the 8-bit cache, rules on logits (torch tensors on the device) ---------------------------
+    def kv8(self, nkv: int, hd: int, n_blocks: int) -> "Kv8Cache | None":
+        """A pool of 8-bit cache blocks of 32 tokens (``b2_kv8_create``), or None where the shape is declined."""
+        from .kv8 import Kv8Cache
+
+        h = C.c_uint64()
+        if not self._check(self._L.b2_kv8_create(self._ctx, nkv, hd, n_blocks, C.byref(h))):
+            return None
+        return Kv8Cache(self, h.value, nkv, hd, n_blocks)
+
+    def logits_dev(self, logits, out=None, pick=None, rules=None) -> bool:
+        """``rules`` (``sampling.LogitRules``) on ``logits [t][n]``: the rows into ``out`` (may be ``logits``), the first largest token of each into ``pick``
+        (int32 [t]; -1 where nothing is left)."""
+        import torch
+
+        t, n = logits.shape
+        dev = torch.device("cuda", self.ordinal)
+        assert logits.device == dev and logits.stride(1) == 1
+        assert out is None or (out.shape == logits.shape and out.dtype == logits.dtype and out.device == dev and out.stride(1) == 1)
+        assert pick is None or (pick.dtype == torch.int32 and pick.numel() == t and pick.is_contiguous() and pick.device == dev)
+        r = rules.c(t, n, dev) if rules is not None else None
+        return self._check(self._L.b2_logits_dev(self._ctx, logits.data_ptr(), out.data_ptr() if out is not None else None, _dtype_code(logits), t, n,
+                                                 logits.stride(0), out.stride(0) if out is not None else 0, C.byref(r) if r is not None else None,
+                                                 pick.data_ptr() if pick is not None else None))
+
     # -- several GPUs (one process per GPU; collectives over NCCL, opened by the library itself) ----------------------
     @staticmethod
     def comm_unique_id() -> bytes:

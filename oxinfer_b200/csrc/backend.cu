@@ -4,6 +4,7 @@
 // all of its work or none of it, and reports "declined" so that the caller can run the batch on the
 // CPU (src/gpu.rs:158-160, src/model.rs:875-886).
 #include <chrono>
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
@@ -36,6 +37,12 @@ struct Moe {
     float act_limit = 0.0f;  // SiluClamp's limit
     void* gate_up = nullptr;  // [experts][2 inter][h / 256][144]
     void* down = nullptr;     // [experts][h][inter / 256][144]
+    size_t bytes = 0;
+};
+
+// A pool of 8-bit cache blocks (b2_kv8_create).
+struct Kv8Pool {
+    Kv8Cache dev{};
     size_t bytes = 0;
 };
 
@@ -74,6 +81,7 @@ class Backend {
     std::unordered_map<uint64_t, Weight> weights;
     std::unordered_map<uint64_t, Moe> moes;
     std::unordered_map<uint64_t, DecodePlanImpl*> decode_plans;
+    std::unordered_map<uint64_t, Kv8Pool> kv8_pools;
     Scratch moe_idx, moe_xg, moe_g, moe_a, moe_o;
     // tensor / expert parallel (b2_comm_init): this process's rank in a group of `world` processes, one GPU each
     NcclComm comm = nullptr;
@@ -90,6 +98,8 @@ class Backend {
     cudaEvent_t stage_full[2] = {};  // the halves of [y] in turn, for results that do not fit (parts_out)
     GemmStatus* gemm_status = nullptr;  // device
     uint32_t* wait_status = nullptr;    // page-locked: the products of a few tokens write it when a bounded wait gives up; 64 bytes on, a copy of *gemm_status
+    uint32_t* list_status() { return (uint32_t*)((uint8_t*)wait_status + STATUS_BYTES - 64); }  // what the 8-bit cache's kernels and the rules on logits report
+    static constexpr size_t STATUS_BYTES = 64 + (sizeof(GemmStatus) + 63) / 64 * 64 + 64;
     // cached tensor maps of the tensor-core GEMM (see matmul_dev)
     std::vector<GemmPlan*> plans;
     // cumulative times, like Backend::stats (src/cuda.rs:403-409)
@@ -1499,6 +1509,130 @@ class Backend {
         return stats_text.c_str();
     }
 
+    // ---- the 8-bit cache, attention over it, rules on logits --------------------------------------------------------
+    int check_list_status() {
+        volatile uint32_t* w = list_status();
+        const uint32_t s = *w;
+        if (!s) return B2_OK;
+        *w = 0;
+        if (s == KV8_BAD_SEQUENCE) return fail(B2_ERR_ARG, "[b200qmm: 8-bit cache: a sequence's rows or positions lie outside the call's]");
+        if (s == KV8_BAD_BLOCK) return fail(B2_ERR_ARG, "[b200qmm: 8-bit cache: a table names a block that the cache does not have]");
+        if (s == LOGITS_BAD_LIST) return fail(B2_ERR_ARG, "[b200qmm: logits: a row's part of a list lies outside the list]");
+        return fail(B2_ERR_TIMEOUT, "[b200qmm: 8-bit cache: a device wait gave up]");
+    }
+    int kv8_create(size_t nkv, size_t hd, size_t n_blocks, uint64_t* out) {
+        if (!out) return fail(B2_ERR_ARG, "[b200qmm: kv8_create: null argument]");
+        if (nkv == 0 || n_blocks == 0) return fail(B2_ERR_ARG, "[b200qmm: kv8_create: a cache has heads and blocks]");
+        if (nkv > 0xffffffffu || hd > 0xffffffffu || !kv8_supports((uint32_t)nkv, (uint32_t)hd) || n_blocks > 0x7fffffffu)
+            return fail(B2_DECLINED, "[b200qmm: kv8_create: %zu KV heads of %zu in %zu blocks are outside the kernels (head dimension 64 or 128, up to 4096 heads)]", nkv, hd, n_blocks);
+        Kv8Pool p;
+        p.dev.nkv = (uint32_t)nkv;
+        p.dev.hd = (uint32_t)hd;
+        p.dev.n_blocks = (uint32_t)n_blocks;
+        p.bytes = kv8_bytes(p.dev.nkv, p.dev.hd, p.dev.n_blocks);
+        cudaError_t e = cudaMalloc((void**)&p.dev.units, p.bytes);
+        if (e != cudaSuccess) {
+            cudaGetLastError();
+            return cuda_fail(e, "cudaMalloc(8-bit cache)");
+        }
+        e = cudaMemset(p.dev.units, 0, p.bytes);  // (scales of zero: blocks nobody has written yet hold zeros)
+        if (e == cudaSuccess) e = cudaStreamSynchronize(cudaStreamLegacy);
+        if (e != cudaSuccess) {
+            cudaFree(p.dev.units);
+            return cuda_fail(e, "cudaMemset(8-bit cache)");
+        }
+        *out = next_handle++;
+        kv8_pools[*out] = p;
+        return B2_OK;
+    }
+    Kv8Pool* find_kv8(uint64_t h) {
+        auto it = kv8_pools.find(h);
+        return it == kv8_pools.end() ? nullptr : &it->second;
+    }
+    int kv8_free(uint64_t h) {
+        Kv8Pool* p = find_kv8(h);
+        if (!p) return fail(B2_ERR_ARG, "[b200qmm: kv8_free: unknown cache]");
+        cudaStreamSynchronize(stream);
+        cudaFree(p->dev.units);
+        kv8_pools.erase(h);
+        return B2_OK;
+    }
+    static bool dtype_ok(int d) { return d == B2_F32 || d == B2_BF16 || d == B2_F16; }
+    int kv8_seqs(const Kv8Pool* p, const b2_kv8_seqs* s, const char* who, Kv8Seqs* out) {
+        if (!p) return fail(B2_ERR_ARG, "[b200qmm: %s: unknown cache]", who);
+        if (!s) return fail(B2_ERR_ARG, "[b200qmm: %s: null argument]", who);
+        *out = Kv8Seqs{s->n_seqs, s->n_rows, s->max_rows, s->max_blocks, s->table, s->start, s->rows};
+        if (s->n_seqs == 0 || s->n_rows == 0) return B2_OK;
+        if (!s->start) return fail(B2_ERR_ARG, "[b200qmm: %s: the sequences' first positions are missing]", who);
+        if (s->max_rows == 0 || s->max_rows > s->n_rows || (!s->rows && (uint64_t)s->n_seqs * s->max_rows != s->n_rows))
+            return fail(B2_ERR_ARG, "[b200qmm: %s: %u rows in %u sequences of up to %u]", who, s->n_rows, s->n_seqs, s->max_rows);
+        if (s->max_blocks == 0 || s->max_blocks >= 1u << 26 || s->n_rows > 0x7fffffffu)
+            return fail(B2_ERR_ARG, "[b200qmm: %s: a sequence has 1 to 2^26 - 1 blocks, and a call up to 2^31 - 1 rows]", who);
+        if (!s->table && (uint64_t)s->n_seqs * s->max_blocks > p->dev.n_blocks)
+            return fail(B2_ERR_ARG, "[b200qmm: %s: %u sequences of %u blocks without a table in a cache of %u]", who, s->n_seqs, s->max_blocks, p->dev.n_blocks);
+        return B2_OK;
+    }
+    int kv8_append(uint64_t h, const b2_kv8_seqs* seqs, const void* k, const void* v, int dtype, size_t rs, size_t hs) {
+        Kv8Pool* p = find_kv8(h);
+        Kv8Seqs s;
+        if (int rc = kv8_seqs(p, seqs, "kv8_append", &s)) return rc;
+        if (!dtype_ok(dtype)) return fail(B2_ERR_ARG, "[b200qmm: kv8_append: unknown element type %d]", dtype);
+        if (s.n_seqs == 0 || s.n_rows == 0) return B2_OK;
+        if (!k || !v) return fail(B2_ERR_ARG, "[b200qmm: kv8_append: null argument]");
+        cudaError_t e = launch_kv8_append(p->dev, s, Kv8Rows{k, v, dtype, rs, hs}, false, list_status(), stream);
+        launches++;
+        return e == cudaSuccess ? B2_OK : cuda_fail(e, "kv8_append");
+    }
+    int kv8_read(uint64_t h, const b2_kv8_seqs* seqs, float* k, float* v) {
+        Kv8Pool* p = find_kv8(h);
+        Kv8Seqs s;
+        if (int rc = kv8_seqs(p, seqs, "kv8_read", &s)) return rc;
+        if (s.n_seqs == 0 || s.n_rows == 0) return B2_OK;
+        if (!k || !v || (((uintptr_t)k | (uintptr_t)v) & 15)) return fail(B2_ERR_ARG, "[b200qmm: kv8_read: the results are missing or not aligned to 16 bytes]");
+        cudaError_t e = launch_kv8_read(p->dev, s, k, v, list_status(), stream);
+        launches++;
+        return e == cudaSuccess ? B2_OK : cuda_fail(e, "kv8_read");
+    }
+    int attend_kv8(uint64_t h, const b2_kv8_seqs* seqs, const b2_kv8_attention* a, const void* q, size_t q_stride, void* out, size_t out_stride, int dtype) {
+        Kv8Pool* p = find_kv8(h);
+        Kv8Seqs s;
+        if (int rc = kv8_seqs(p, seqs, "attend_kv8", &s)) return rc;
+        if (!a) return fail(B2_ERR_ARG, "[b200qmm: attend_kv8: null argument]");
+        if (!dtype_ok(dtype)) return fail(B2_ERR_ARG, "[b200qmm: attend_kv8: unknown element type %d]", dtype);
+        if (a->nh == 0 || a->nh % p->dev.nkv) return fail(B2_ERR_ARG, "[b200qmm: attend_kv8: %u query heads over %u KV heads]", a->nh, p->dev.nkv);
+        if (!std::isfinite(a->scale) || !std::isfinite(a->cap) || a->cap < 0.0f) return fail(B2_ERR_ARG, "[b200qmm: attend_kv8: the scale and the cap are finite, the cap not negative]");
+        if (s.n_seqs == 0 || s.n_rows == 0) return B2_OK;
+        if (!q || !out) return fail(B2_ERR_ARG, "[b200qmm: attend_kv8: null argument]");
+        if (s.n_rows > 1 && out_stride < (size_t)a->nh * p->dev.hd) return fail(B2_ERR_ARG, "[b200qmm: attend_kv8: rows of the result overlap]");
+        if ((uint64_t)s.n_rows * (a->nh / p->dev.nkv) > 0x7fffffffu) return fail(B2_DECLINED, "[b200qmm: attend_kv8: too many rows for one call]");
+        cudaError_t e = launch_attend_kv8(p->dev, s, Kv8Attn{a->nh, a->scale, a->cap, a->window, a->slopes, a->prefix}, q, q_stride, out, out_stride, dtype, list_status(), stream);
+        launches++;
+        return e == cudaSuccess ? B2_OK : cuda_fail(e, "attend_kv8");
+    }
+    int logit_rules(const b2_logit_rules* r, size_t n, const char* who, LogitRulesDev* out) {
+        *out = LogitRulesDev{1.0f, 0.0f, 0.0f, nullptr, nullptr, 0, nullptr, nullptr, nullptr, 0, nullptr, 0};
+        if (!r) return B2_OK;
+        if (!(r->repeat > 0.0f) || !std::isfinite(r->repeat) || !std::isfinite(r->frequency) || !std::isfinite(r->presence))
+            return fail(B2_ERR_ARG, "[b200qmm: %s: penalties are finite, the one for repetition above zero]", who);
+        if ((r->n_history && !r->history) || (r->n_bias && (!r->bias_ids || !r->bias)) || r->n_history > 0x7fffffffu || r->n_bias > 0x7fffffffu)
+            return fail(B2_ERR_ARG, "[b200qmm: %s: a list is missing, or longer than 2^31 - 1]", who);
+        if (r->mask && r->mask_stride && r->mask_stride < (n + 31) / 32) return fail(B2_ERR_ARG, "[b200qmm: %s: rows of the mask overlap]", who);
+        *out = LogitRulesDev{r->repeat, r->frequency, r->presence, r->history, r->history_ptr, r->n_history, r->bias_ids, r->bias, r->bias_ptr, r->n_bias, r->mask, r->mask_stride};
+        return B2_OK;
+    }
+    int logits(const void* x, void* out, int dtype, size_t t, size_t n, size_t xs, size_t os, const b2_logit_rules* rules, int32_t* pick) {
+        LogitRulesDev r;
+        if (int rc = logit_rules(rules, n, "logits", &r)) return rc;
+        if (!dtype_ok(dtype)) return fail(B2_ERR_ARG, "[b200qmm: logits: unknown element type %d]", dtype);
+        if (t == 0 || n == 0) return B2_OK;
+        if (!x || (!out && !pick)) return fail(B2_ERR_ARG, "[b200qmm: logits: null argument]");
+        if (n > 0x7fffff00u || t > 0x7ffffffu) return fail(B2_DECLINED, "[b200qmm: logits: %zu rows of %zu are too many for one call]", t, n);
+        if (t > 1 && ((out && os < n) || xs < n)) return fail(B2_ERR_ARG, "[b200qmm: logits: rows overlap]");
+        cudaError_t e = launch_logits(x, out, dtype, xs, os, (uint32_t)t, (uint32_t)n, r, pick, list_status(), stream);
+        launches++;
+        return e == cudaSuccess ? B2_OK : cuda_fail(e, "logits");
+    }
+
     // ---- Backend::decode_plan (src/gpu.rs:262-289) and DecodePlan::step (src/gpu_decode.rs:538-587) ----
     int decode_plan(const b2_graph* g, uint64_t* out, int tokens = 1, bool prefill = false) {
         if (!out) return fail(B2_ERR_ARG, "[b200qmm: decode_plan: null argument]");
@@ -1603,6 +1737,8 @@ class Backend {
             cudaFree(kv.second.down);
         }
         moes.clear();
+        for (auto& kv : kv8_pools) cudaFree(kv.second.dev.units);
+        kv8_pools.clear();
         comm_free();
         for (Scratch* sc : {&tp_stage, &tp_gather, &ep_idx, &ep_send, &ep_recv, &ep_out, &ep_back}) sc->release();
         moe_idx.release();
@@ -1682,7 +1818,7 @@ B2_EXPORT int b2_open(int ordinal, b2_ctx** out) {
         return B2_ERR_CUDA;
     }
     uint32_t* word = nullptr;
-    if (cudaHostAlloc((void**)&word, 64 + sizeof(b2::GemmStatus), cudaHostAllocMapped | cudaHostAllocPortable) != cudaSuccess) {
+    if (cudaHostAlloc((void**)&word, Backend::STATUS_BYTES, cudaHostAllocMapped | cudaHostAllocPortable) != cudaSuccess) {
         g_open_error = "[b200qmm: cudaHostAlloc failed]";
         cudaGetLastError();
         return B2_ERR_NOMEM;
@@ -1690,6 +1826,7 @@ B2_EXPORT int b2_open(int ordinal, b2_ctx** out) {
     *word = 0;
     b2_ctx* c = new b2_ctx();
     c->be.wait_status = word;
+    *c->be.list_status() = 0;
     c->be.device = ordinal;
     c->be.sm_count = prop.multiProcessorCount;
     *out = c;
@@ -1859,7 +1996,48 @@ B2_EXPORT int b2_matvec_prepared_dev(b2_ctx* ctx, b2_weight w, b2_weight up, con
 // stream: B2_OK, or B2_ERR_TIMEOUT where a bounded device wait gave up.
 B2_EXPORT int b2_check_status(b2_ctx* ctx) {
     LOCKED(ctx);
+    if (int rc = ctx->be.check_list_status()) return rc;
     return ctx->be.check_gemm_status();
+}
+
+B2_EXPORT int b2_kv8_create(b2_ctx* ctx, size_t nkv, size_t hd, size_t n_blocks, b2_kv8* out) {
+    LOCKED(ctx);
+    return ctx->be.kv8_create(nkv, hd, n_blocks, out);
+}
+
+B2_EXPORT int b2_kv8_free(b2_ctx* ctx, b2_kv8 kv) {
+    LOCKED(ctx);
+    return ctx->be.kv8_free(kv);
+}
+
+B2_EXPORT size_t b2_kv8_bytes(b2_ctx* ctx, b2_kv8 kv) {
+    if (!ctx) return 0;
+    std::lock_guard<std::mutex> lock(ctx->be.mu);
+    b2::Kv8Pool* p = ctx->be.find_kv8(kv);
+    return p ? p->bytes : 0;
+}
+
+B2_EXPORT int b2_kv8_append_dev(b2_ctx* ctx, b2_kv8 kv, const b2_kv8_seqs* seqs, const void* k_dev, const void* v_dev, int dtype, size_t row_stride,
+                                size_t head_stride) {
+    LOCKED(ctx);
+    return ctx->be.kv8_append(kv, seqs, k_dev, v_dev, dtype, row_stride, head_stride);
+}
+
+B2_EXPORT int b2_kv8_read_dev(b2_ctx* ctx, b2_kv8 kv, const b2_kv8_seqs* seqs, float* k_dev, float* v_dev) {
+    LOCKED(ctx);
+    return ctx->be.kv8_read(kv, seqs, k_dev, v_dev);
+}
+
+B2_EXPORT int b2_attend_kv8_dev(b2_ctx* ctx, b2_kv8 kv, const b2_kv8_seqs* seqs, const b2_kv8_attention* attention, const void* q_dev, size_t q_stride,
+                                void* out_dev, size_t out_stride, int dtype) {
+    LOCKED(ctx);
+    return ctx->be.attend_kv8(kv, seqs, attention, q_dev, q_stride, out_dev, out_stride, dtype);
+}
+
+B2_EXPORT int b2_logits_dev(b2_ctx* ctx, const void* logits_dev, void* out_dev, int dtype, size_t t, size_t n, size_t logits_stride, size_t out_stride,
+                            const b2_logit_rules* rules, int32_t* pick_dev) {
+    LOCKED(ctx);
+    return ctx->be.logits(logits_dev, out_dev, dtype, t, n, logits_stride, out_stride, rules, pick_dev);
 }
 
 B2_EXPORT int b2_inject_timeout(b2_ctx* ctx, b2_plan plan) {

@@ -289,6 +289,61 @@ cudaError_t launch_glu(const float* g, const float* u, float* out, uint32_t n, i
 cudaError_t launch_argmax(const float* logits, uint32_t n, float* pval, int* pidx, uint32_t* counter, int* token, int* out_tokens, uint32_t* sp,
                           cudaStream_t st, bool pdl = false);
 
+// ---- kv8.cu, attend_kv8.cu: a cache of 8-bit integers in blocks of 32 tokens, a scale for each block, head and kind, and attention over it ----
+constexpr uint32_t KV8_BLOCK = 32, KV8_HEADER = 32;  // tokens; bytes ahead of a unit's keys (kv8.cuh)
+struct Kv8Cache {
+    uint8_t* units;  // [n_blocks][nkv][unit]
+    uint32_t nkv, hd, n_blocks;
+};
+// The sequences of a call: rows rows[s] .. rows[s + 1] - 1 of its arrays (rows null: max_rows each) belong to sequence s, at positions start[s] ..;
+// block b of a sequence is the cache's table[s max_blocks + b] (table null: s max_blocks + b). All on the device.
+struct Kv8Seqs {
+    uint32_t n_seqs, n_rows, max_rows, max_blocks;
+    const int32_t* table;
+    const int32_t* start;
+    const int32_t* rows;
+};
+// What the kernels leave in the status word (and b2_check_status reports) where a call's device arrays do not fit its host arguments.
+constexpr uint32_t KV8_BAD_SEQUENCE = 11, KV8_BAD_BLOCK = 12, KV8_TIMEOUT = 13, LOGITS_BAD_LIST = 14;
+size_t kv8_bytes(uint32_t nkv, uint32_t hd, uint32_t n_blocks);
+bool kv8_supports(uint32_t nkv, uint32_t hd);
+// Rows of keys and values, a head hs elements behind the one ahead of it, a row rs behind the one ahead. keep_behind: rows of a block behind the new ones
+// stay what they are too (else they are undefined until they are written).
+struct Kv8Rows {
+    const void *k, *v;
+    int dtype;  // B2_F32 / B2_BF16 / B2_F16
+    size_t rs, hs;
+};
+cudaError_t launch_kv8_append(const Kv8Cache& c, const Kv8Seqs& s, const Kv8Rows& x, bool keep_behind, uint32_t* status, cudaStream_t st, bool pdl = false);
+// The values that the rows stand for, f32 [n_rows][nkv][hd] each.
+cudaError_t launch_kv8_read(const Kv8Cache& c, const Kv8Seqs& s, float* k, float* v, uint32_t* status, cudaStream_t st);
+struct Kv8Attn {
+    uint32_t nh;
+    float scale, cap;       // cap 0: scores as they are
+    uint32_t window;        // 0: none
+    const float* slopes;    // [nh] or null
+    const int32_t* prefix;  // [n_seqs] or null
+};
+// Row i of a sequence is a query at start + i, and sees the sequence's keys up to its own position and below the prefix, the last `window` of them.
+cudaError_t launch_attend_kv8(const Kv8Cache& c, const Kv8Seqs& s, const Kv8Attn& p, const void* q, size_t q_stride, void* out, size_t out_stride, int dtype,
+                              uint32_t* status, cudaStream_t st, bool pdl = false);
+
+// ---- logits.cu: penalties, biases and masks on rows of logits, and the largest that is left ----
+struct LogitRulesDev {
+    float repeat, frequency, presence;
+    const int32_t* history;      // ids; row r's: history_ptr[r] .. history_ptr[r + 1]
+    const int32_t* history_ptr;
+    uint32_t n_history;
+    const int32_t* bias_ids;
+    const float* bias;
+    const int32_t* bias_ptr;     // null: the whole list for every row
+    uint32_t n_bias;
+    const uint32_t* mask;        // bit i % 32 of word i / 32: token i is allowed
+    size_t mask_stride;          // words from a row to the next, 0: one mask for all
+};
+cudaError_t launch_logits(const void* x, void* out, int dtype, size_t x_stride, size_t out_stride, uint32_t t, uint32_t n, const LogitRulesDev& r, int32_t* pick,
+                          uint32_t* status, cudaStream_t st, bool pdl = false);
+
 // ---- prefill_ops.cu: the same ops over many token rows (row r of an activation `stride` floats behind row r - 1) -----------
 // Token row r is at position sp[0] + r; sp[1] is the position of row 0 of the RoPE table.
 cudaError_t launch_qk_rope_rows(const float* qkv, float* qo, size_t stride, uint32_t rows, void* kc, void* vc, int kv_f16, const float* qn,
