@@ -368,6 +368,13 @@ typedef struct b2_op {
     uint32_t gelu;       /* GLU */
 } b2_op;
 
+/* A plan's caches as blocks of 8-bit integers with a power of two as the scale of 32 tokens, head and kind (the format of b2_kv8_create, a quarter of the f32 caches'
+ * bytes): keys and values are rounded when they are appended, attention takes any number of query heads a KV head, head dimension 64 or 128. A step of
+ * several tokens scales a block by all of its rows at once, so its caches, and with them the results, can differ from those of one-token steps by that
+ * rounding (the bits of both are the same from run to run); what a step appended and the next one overwrites can leave its block's scale larger than need
+ * be. b2_plan_kv_write keeps the other rows of a block, brought to the block's scale; rows that are not finite come back as NaN. */
+#define B2_KV_I8 2
+
 typedef struct b2_graph {
     const uint64_t* bufs; /* floats in each activation buffer */
     uint32_t n_bufs;
@@ -385,7 +392,7 @@ typedef struct b2_graph {
     const uint32_t* rope_halves; /* Graph::rope_halves: a step's rope_cs holds, per entry, cos[half] then sin[half] */
     uint32_t n_rope;
     uint32_t max_len;     /* positions each KV cache holds */
-    uint32_t kv_f16;      /* 0: f32 caches (the reference's); 1: f16 caches */
+    uint32_t kv_f16;      /* 0: f32 caches (the reference's); 1: f16 caches; B2_KV_I8: 8-bit caches */
 } b2_graph;
 
 /* B2_OK and a plan, B2_DECLINED (> 0) for an op or shape outside the supported set, < 0 on error. */
@@ -434,6 +441,19 @@ int b2_plan_kv_read(b2_ctx* ctx, b2_plan plan, uint32_t kv, size_t pos0, size_t 
  * elapsed_ms (optional): device time of the n_tokens steps. Needs n_logits > 0. */
 int b2_plan_generate(b2_ctx* ctx, b2_plan plan, b2_weight embed, int32_t first_token, size_t pos0, size_t n_tokens,
                      const float* rope_cs_table, int32_t* out_tokens, float* elapsed_ms);
+/* The same with rules on the logits of every step (those of b2_logits_dev; all arrays on the host, read during the call): the history is `prompt` and every
+ * token chosen in this call (first_token counts where the prompt has it), the biases and the mask (one bit a token, (n_logits + 31) / 32 words, or NULL)
+ * hold for all steps. A mask without a token is refused; where nothing else is left (biases of -inf, NaN) token 0 is taken. rules == NULL: b2_plan_generate. */
+typedef struct b2_generate_rules {
+    float repeat, frequency, presence;
+    uint32_t n_prompt, n_bias;
+    const int32_t* prompt;
+    const int32_t* bias_ids;
+    const float* bias;
+    const uint32_t* mask;
+} b2_generate_rules;
+int b2_plan_generate_ruled(b2_ctx* ctx, b2_plan plan, b2_weight embed, int32_t first_token, size_t pos0, size_t n_tokens, const float* rope_cs_table,
+                           const b2_generate_rules* rules, int32_t* out_tokens, float* elapsed_ms);
 /* Kernel launches of one step of the plan (for launch accounting). */
 int b2_plan_launches(b2_ctx* ctx, b2_plan plan, uint64_t* per_step);
 

@@ -56,6 +56,14 @@ class LogitRules(C.Structure):
                 ("mask", C.c_void_p), ("mask_stride", C.c_size_t)]
 
 
+class GenerateRules(C.Structure):
+    """``b2_generate_rules``."""
+
+    _fields_ = [("repeat", C.c_float), ("frequency", C.c_float), ("presence", C.c_float), ("n_prompt", C.c_uint32), ("n_bias", C.c_uint32),
+                ("prompt", C.c_void_p), ("bias_ids", C.c_void_p), ("bias", C.c_void_p), ("mask", C.c_void_p)]
+
+
+KV_I8 = 2
 OP_NORM, OP_LINEAR, OP_QK_ROPE, OP_ATTEND, OP_GLU, OP_EXCHANGE = 1, 2, 3, 4, 5, 6
 PLAN_HANDLE_BYTES = 128
 COMM_ID_BYTES = 128
@@ -162,6 +170,8 @@ _SIGNATURES = {
     "b2_plan_kv_read": (C.c_int, [C.c_void_p, C.c_uint64, C.c_uint32, C.c_size_t, C.c_size_t, C.c_void_p, C.c_void_p]),
     "b2_plan_generate": (C.c_int, [C.c_void_p, C.c_uint64, C.c_uint64, C.c_int32, C.c_size_t, C.c_size_t, C.c_void_p, C.c_void_p,
                                    C.POINTER(C.c_float)]),
+    "b2_plan_generate_ruled": (C.c_int, [C.c_void_p, C.c_uint64, C.c_uint64, C.c_int32, C.c_size_t, C.c_size_t, C.c_void_p, C.POINTER(GenerateRules), C.c_void_p,
+                                         C.POINTER(C.c_float)]),
     "b2_plan_launches": (C.c_int, [C.c_void_p, C.c_uint64, C.POINTER(C.c_uint64)]),
     "b2_plan_export": (C.c_int, [C.c_void_p, C.c_uint64, C.c_void_p]),
     "b2_plan_attach_peers": (C.c_int, [C.c_void_p, C.c_uint64, C.c_uint32, C.c_uint32, C.c_void_p]),

@@ -25,9 +25,9 @@ __device__ __forceinline__ float block_sum(float v, float* red) {  // red: 32 fl
 // One head of the token's attention inputs: h < nh a query head, then nkv key heads, then nkv value heads. Every thread
 // of the CTA calls this (it uses the CTA barrier); thread i < hd owns dimension i. Optional per-head RMS norm, RoPE on
 // the first 2 * half_rot dimensions (unfused multiplies and adds, as the CPU's apply_rope), queries to `qo`, keys and
-// values to row `pos` of the caches [nkv][max_len][hd]. buf: 256 floats of shared memory.
+// values to row `row` of the caches [nkv][max_len][hd] (the position, or the token of the step where they are staged). buf: 256 floats of shared memory.
 template <typename T>
-__device__ __forceinline__ void rope_head(const uint32_t h, const uint32_t i, const uint32_t pos, const uint32_t table_pos0,
+__device__ __forceinline__ void rope_head(const uint32_t h, const uint32_t i, const uint32_t pos, const uint32_t table_pos0, const uint32_t row,
                                           const float* qkv, float* qo, T* kc, T* vc,
                                           const float* __restrict__ qn, const float* __restrict__ kn, const float* __restrict__ cs_table,
                                           const DecRope& p, float* buf, float* red) {
@@ -45,8 +45,8 @@ __device__ __forceinline__ void rope_head(const uint32_t h, const uint32_t i, co
         if (on && kind == 0) v *= qn[i];
         else if (on && kind == 1) v *= kn[i];
     }
-    const bool room = pos < p.max_len;  // a full cache: nothing is written (the host refuses the step before this)
-    const size_t at = ((size_t)hh * p.max_len + pos) * hd + i;
+    const bool room = row < p.max_len;  // a full cache: nothing is written (the host refuses the step before this)
+    const size_t at = ((size_t)hh * p.max_len + row) * hd + i;
     if (on && kind != 2) buf[i] = v;
     __syncthreads();
     if (on && room) {

@@ -1696,14 +1696,14 @@ class Backend {
         if (rc) err = e;
         return rc;
     }
-    int plan_generate(uint64_t h, uint64_t embed, int32_t first, size_t pos0, size_t n, const float* rope, int32_t* out, float* ms) {
+    int plan_generate(uint64_t h, uint64_t embed, int32_t first, size_t pos0, size_t n, const float* rope, const b2_generate_rules* rules, int32_t* out, float* ms) {
         DecodePlanImpl* p = find_plan(h);
         if (!p) return fail(B2_ERR_ARG, "[b200qmm: plan_generate: unknown plan]");
         Weight* w = find(embed);
         if (!w) return fail(B2_ERR_ARG, "[b200qmm: plan_generate: unknown embedding weight]");
         std::string e;
-        int rc = p->generate(stream, embed, w->dev, first, pos0, n, rope, out, ms, e);
-        launches += (p->launches_per_step() + 2) * n + 1;
+        int rc = p->generate(stream, embed, w->dev, first, pos0, n, rope, rules, out, ms, e);
+        launches += (p->launches_per_step() + (rules ? 3 : 2)) * n + 1;
         calls++;
         if (rc) err = e;
         return rc;
@@ -2151,7 +2151,13 @@ B2_EXPORT int b2_plan_kv_read(b2_ctx* ctx, b2_plan plan, uint32_t kv, size_t pos
 B2_EXPORT int b2_plan_generate(b2_ctx* ctx, b2_plan plan, b2_weight embed, int32_t first_token, size_t pos0, size_t n_tokens,
                                const float* rope_cs_table, int32_t* out_tokens, float* elapsed_ms) {
     LOCKED(ctx);
-    return ctx->be.plan_generate(plan, embed, first_token, pos0, n_tokens, rope_cs_table, out_tokens, elapsed_ms);
+    return ctx->be.plan_generate(plan, embed, first_token, pos0, n_tokens, rope_cs_table, nullptr, out_tokens, elapsed_ms);
+}
+
+B2_EXPORT int b2_plan_generate_ruled(b2_ctx* ctx, b2_plan plan, b2_weight embed, int32_t first_token, size_t pos0, size_t n_tokens, const float* rope_cs_table,
+                                     const b2_generate_rules* rules, int32_t* out_tokens, float* elapsed_ms) {
+    LOCKED(ctx);
+    return ctx->be.plan_generate(plan, embed, first_token, pos0, n_tokens, rope_cs_table, rules, out_tokens, elapsed_ms);
 }
 
 B2_EXPORT int b2_plan_launches(b2_ctx* ctx, b2_plan plan, uint64_t* per_step) {

@@ -231,6 +231,7 @@ struct DecRope {
     uint32_t nh, nkv, hd, half_rot, q_stride, k_off, v_off, interleaved, v_norm, v_from_k, max_len;
     uint32_t cs_stride, cs_off;  // floats per position in the RoPE table, and where this op's cos/sin start in a row
     float eps;
+    uint32_t staged = 0;  // keys and values go to row 0, 1, .. of [nkv][max_len][hd] by token of the step, not by position
 };
 struct DecAttn {
     uint32_t nh, nkv, hd, max_len, window;
@@ -341,6 +342,8 @@ struct LogitRulesDev {
     const uint32_t* mask;        // bit i % 32 of word i / 32: token i is allowed
     size_t mask_stride;          // words from a row to the next, 0: one mask for all
 };
+// After a choice: the token (0 where pick is -1), the output list, the history behind history_ptr[1], and the step words move on.
+cudaError_t launch_advance(const int32_t* pick, int* token, int* out_tokens, int32_t* history, int32_t* history_ptr, uint32_t* sp, cudaStream_t st, bool pdl = false);
 cudaError_t launch_logits(const void* x, void* out, int dtype, size_t x_stride, size_t out_stride, uint32_t t, uint32_t n, const LogitRulesDev& r, int32_t* pick,
                           uint32_t* status, cudaStream_t st, bool pdl = false);
 

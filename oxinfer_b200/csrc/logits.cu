@@ -220,7 +220,23 @@ cudaError_t logits_t(LgArgs& a, uint32_t t, cudaStream_t st, bool pdl) {
     return cudaLaunchKernelEx(&cfg, kern, a);
 }
 
+__global__ void advance_kernel(const int32_t* pick, int* token, int* out_tokens, int32_t* history, int32_t* history_ptr, uint32_t* sp) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int id = max(*pick, 0);
+    *token = id;
+    out_tokens[sp[2]] = id;
+    history[history_ptr[1]] = id;
+    history_ptr[1] += 1;
+    sp[2] += 1;
+    sp[0] += 1;
+}
+
 }  // namespace
+
+cudaError_t launch_advance(const int32_t* pick, int* token, int* out_tokens, int32_t* history, int32_t* history_ptr, uint32_t* sp, cudaStream_t st, bool pdl) {
+    return launch_k(advance_kernel, dim3(1), dim3(1), 0, st, pdl, pick, token, out_tokens, history, history_ptr, sp);
+}
 
 cudaError_t launch_logits(const void* x, void* out, int dtype, size_t x_stride, size_t out_stride, uint32_t t, uint32_t n, const LogitRulesDev& r, int32_t* pick,
                           uint32_t* status, cudaStream_t st, bool pdl) {

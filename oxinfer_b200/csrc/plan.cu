@@ -5,6 +5,7 @@
 // (src/cuda_decode.rs:1466-1658) is one cudaGraphLaunch here.
 #include "plan.h"
 
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <cstdlib>
@@ -116,6 +117,7 @@ DecodePlanImpl::~DecodePlanImpl() {
     for (cudaGraphExec_t e : multi_exec_)
         if (e) cudaGraphExecDestroy(e);
     if (gen_exec_) cudaGraphExecDestroy(gen_exec_);
+    if (gen_rules_exec_) cudaGraphExecDestroy(gen_rules_exec_);
     if (ev0_) cudaEventDestroy(ev0_);
     if (ev1_) cudaEventDestroy(ev1_);
     if (cap_stream_) cudaStreamDestroy(cap_stream_);
@@ -126,7 +128,7 @@ DecodePlanImpl::~DecodePlanImpl() {
     for (void* m : peer_maps_) cudaIpcCloseMemHandle(m);
     for (auto& kv : gemm_plans_)
         for (GemmPlan* gp : kv.second) gemm_tc_plan_destroy(gp);
-    void* frees[] = {kv16_, x16_, unscale_, tmp_a_, tmp_b_, gemm_status_, xflags_, bufs_, records_, consts_, att_scratch_.part, words_, rope_table_, argmax_val_, argmax_idx_, token_, out_tokens_, stage_};
+    void* frees[] = {kv8_rows_, gen_rules_.room, gen_rules_.words, kv16_, x16_, unscale_, tmp_a_, tmp_b_, gemm_status_, xflags_, bufs_, records_, consts_, att_scratch_.part, words_, rope_table_, argmax_val_, argmax_idx_, token_, out_tokens_, stage_};
     for (void* p : frees)
         if (p) cudaFree(p);
 }
@@ -134,7 +136,7 @@ DecodePlanImpl::~DecodePlanImpl() {
 bool DecodePlanImpl::uses_weight(uint64_t h) const {
     for (uint64_t w : weight_handles_)
         if (w == h) return true;
-    return h != 0 && h == gen_embed_;
+    return h != 0 && (h == gen_embed_ || h == gen_rules_.embed);
 }
 
 int DecodePlanImpl::create(const b2_graph* g, const std::function<const WeightDev*(uint64_t)>& resolve, int sm_count, bool fast, int tokens,
@@ -173,7 +175,9 @@ int DecodePlanImpl::create(const b2_graph* g, const std::function<const WeightDe
         p->loop_attend_ = e && strcmp(e, "loop") == 0;
     }
     p->max_len_ = g->max_len;
-    p->kv_f16_ = g->kv_f16 ? 1 : 0;
+    p->kv8_ = g->kv_f16 == B2_KV_I8;
+    p->kv_f16_ = g->kv_f16 && !p->kv8_ ? 1 : 0;
+    if (p->kv8_) p->fuse_rope_ = false;  // (the step's rows are quantized on their way into the cache)
 
     // ---- activation buffers: one allocation, each buffer 256-byte aligned --------------------------
     size_t total = 0;
@@ -212,6 +216,18 @@ int DecodePlanImpl::create(const b2_graph* g, const std::function<const WeightDe
         Kv k;
         k.nkv = g->kv_nkv[i];
         k.hd = g->kv_hd[i];
+        if (p->kv8_) {
+            if (!kv8_supports(k.nkv, k.hd) || g->max_len > 0x7fffff00u) {
+                err = fmt("[b200qmm: decode_plan: an 8-bit cache of %u KV heads of %u is outside the kernels (head dimension 64 or 128)]", k.nkv, k.hd);
+                return B2_DECLINED;
+            }
+            const size_t bytes = kv8_bytes(k.nkv, k.hd, (g->max_len + KV8_BLOCK - 1) / KV8_BLOCK);
+            PLAN_CUDA(cudaMalloc(&k.k, bytes), "cudaMalloc(8-bit cache)");
+            p->kv_.push_back(k);
+            PLAN_CUDA(cudaMemset(k.k, 0, bytes), "cudaMemset(8-bit cache)");
+            max_row = std::max(max_row, (size_t)k.nkv * k.hd);
+            continue;
+        }
         size_t bytes = (size_t)k.nkv * g->max_len * k.hd * esz;
         PLAN_CUDA(cudaMalloc(&k.k, bytes), "cudaMalloc(K cache)");
         p->kv_.push_back(k);  // pushed before V so that a failure below still frees K
@@ -219,6 +235,11 @@ int DecodePlanImpl::create(const b2_graph* g, const std::function<const WeightDe
         PLAN_CUDA(cudaMemset(p->kv_.back().k, 0, bytes), "cudaMemset(K cache)");
         PLAN_CUDA(cudaMemset(p->kv_.back().v, 0, bytes), "cudaMemset(V cache)");
         max_row = std::max(max_row, (size_t)k.nkv * k.hd);
+    }
+
+    if (p->kv8_) {
+        p->kv8_row_floats_ = T * std::max<size_t>(max_row, 64);
+        PLAN_CUDA(cudaMalloc((void**)&p->kv8_rows_, 2 * p->kv8_row_floats_ * sizeof(float)), "cudaMalloc(rows of a step)");
     }
 
     // ---- norm weights: one device block -----------------------------------------------------------
@@ -380,11 +401,15 @@ int DecodePlanImpl::create(const b2_graph* g, const std::function<const WeightDe
                     err = "[b200qmm: decode_plan: attend does not match its KV cache]";
                     return B2_ERR_ARG;
                 }
-                if (prefill && !attend_rows_supports(o.nh, o.nkv, o.hd)) {
+                if (p->kv8_ && (o.nh == 0 || o.nh % o.nkv)) {
+                    err = fmt("[b200qmm: decode_plan: %u query heads over %u KV heads]", o.nh, o.nkv);
+                    return B2_DECLINED;
+                }
+                if (!p->kv8_ && prefill && !attend_rows_supports(o.nh, o.nkv, o.hd)) {
                     err = "[b200qmm: decode_plan: prefill attention takes head dimensions 64 and 128]";
                     return B2_DECLINED;
                 }
-                if ((!prefill || p->loop_attend_) && !attend_supports(o.nh, o.nkv, o.hd)) {
+                if (!p->kv8_ && (!prefill || p->loop_attend_) && !attend_supports(o.nh, o.nkv, o.hd)) {
                     err = fmt("[b200qmm: decode_plan: attention with %u heads over %u KV heads of %u is outside the kernel (head dim 64 / 128, "
                               "1 / 2 / 4 / 8 heads per KV head)]", o.nh, o.nkv, o.hd);
                     return B2_DECLINED;
@@ -606,7 +631,7 @@ int DecodePlanImpl::create(const b2_graph* g, const std::function<const WeightDe
     // ---- scratch ------------------------------------------------------------------------------------
     size_t part_floats = 0, count_words = 0;
     for (const Op& o : p->ops_) {
-        if (o.kind != B2_OP_ATTEND || (prefill && !p->loop_attend_)) continue;
+        if (o.kind != B2_OP_ATTEND || p->kv8_ || (prefill && !p->loop_attend_)) continue;
         const uint32_t tokens = prefill ? 1 : (uint32_t)T;
         part_floats = std::max(part_floats, attend_part_floats(o.attn.nh, o.attn.nkv, o.attn.hd, o.attn.max_len, tokens));
         count_words = std::max(count_words, attend_count_words(o.attn.nh, o.attn.nkv, o.attn.max_len, tokens));
@@ -622,6 +647,7 @@ int DecodePlanImpl::create(const b2_graph* g, const std::function<const WeightDe
     p->sp_ = p->words_;
     p->status_ = p->words_ + 4;
     p->argmax_counter_ = p->words_ + 5;
+    p->kv8_at_ = p->words_ + 6;
     p->sp_multi_ = p->words_ + 8;
     p->att_scratch_.counts = p->words_ + 8 + 4 * T;
     size_t table = (size_t)std::max<uint32_t>(p->cs_stride_, 1) * g->max_len;
@@ -660,7 +686,7 @@ int DecodePlanImpl::create(const b2_graph* g, const std::function<const WeightDe
         PLAN_CUDA(cudaMalloc((void**)&p->tmp_a_, T * max_n * sizeof(float)), "cudaMalloc(products)");
         PLAN_CUDA(cudaMalloc((void**)&p->tmp_b_, T * max_n * sizeof(float)), "cudaMalloc(products)");
         size_t kv16 = 0;
-        for (const Kv& k : p->kv_) kv16 = std::max(kv16, attend_rows_scratch_bytes(k.nkv, g->max_len, k.hd, p->kv_f16_));
+        for (const Kv& k : p->kv_) kv16 = std::max(kv16, p->kv8_ ? 0 : attend_rows_scratch_bytes(k.nkv, g->max_len, k.hd, p->kv_f16_));
         if (kv16) PLAN_CUDA(cudaMalloc(&p->kv16_, kv16), "cudaMalloc(f16 cache rows)");
         PLAN_CUDA(cudaMalloc((void**)&p->gemm_status_, sizeof(GemmStatus)), "cudaMalloc(GEMM status)");
         PLAN_CUDA(cudaMemset(p->gemm_status_, 0, sizeof(GemmStatus)), "cudaMemset(GEMM status)");
@@ -712,6 +738,23 @@ GemvIn DecodePlanImpl::product_in(const Op& o, bool self) const {
     return in;
 }
 
+cudaError_t DecodePlanImpl::rope_kv8(const Op& o, const uint32_t* at, uint32_t nt, bool rows_kernel, cudaStream_t st, bool pdl) {
+    DecRope r = o.rope;
+    r.max_len = nt;
+    r.staged = 1;
+    float *k = kv8_rows_, *v = kv8_rows_ + kv8_row_floats_;
+    cudaError_t e = rows_kernel ? launch_qk_rope_rows(o.x, o.y, block_floats_, nt, k, v, 0, o.p0, o.p1, rope_table_, at, r, st)
+                                : launch_qk_rope(o.x, o.y, k, v, 0, o.p0, o.p1, rope_table_, at, r, st, pdl);
+    if (e != cudaSuccess) return e;
+    const Kv8Cache c{(uint8_t*)kv_[o.kv].k, r.nkv, r.hd, (max_len_ + KV8_BLOCK - 1) / KV8_BLOCK};
+    return launch_kv8_append(c, kv8_seqs(at, nt), Kv8Rows{k, v, B2_F32, r.hd, (size_t)nt * r.hd}, false, status_, st, pdl);
+}
+cudaError_t DecodePlanImpl::attend_kv8(const Op& o, const uint32_t* at, uint32_t nt, cudaStream_t st, bool pdl) {
+    const Kv8Cache c{(uint8_t*)kv_[o.kv].k, o.attn.nkv, o.attn.hd, (max_len_ + KV8_BLOCK - 1) / KV8_BLOCK};
+    return launch_attend_kv8(c, kv8_seqs(at, nt), Kv8Attn{o.attn.nh, o.attn.scale, 0.0f, o.attn.window, nullptr, nullptr}, o.x, block_floats_, o.y, block_floats_,
+                             B2_F32, status_, st, pdl);
+}
+
 // `chained`: every launch but the first (`first_chained`: the first too) carries the programmatic-dependent-launch
 // attribute, so each kernel starts (and fetches its first weights) while the one before it drains.
 int DecodePlanImpl::run_ops(cudaStream_t st, std::string& err, bool chained, bool first_chained) {
@@ -730,10 +773,17 @@ int DecodePlanImpl::run_ops(cudaStream_t st, std::string& err, bool chained, boo
                                   : launch_gemv_f8_float(o.w, o.pair ? &o.w2 : nullptr, o.x, o.y, o.mode, o.z, sm_count_, st, pdl);
                 break;
             case B2_OP_QK_ROPE:
+                if (kv8_) {
+                    e = rope_kv8(o, sp_, 1, false, st, pdl);
+                    launches_++;
+                    break;
+                }
                 e = launch_qk_rope(o.x, o.y, kv_[o.kv].k, kv_[o.kv].v, kv_f16_, o.p0, o.p1, rope_table_, sp_, o.rope, st, pdl);
                 break;
             case B2_OP_ATTEND:
-                if (o.fr.qkv) {
+                if (kv8_) {
+                    e = attend_kv8(o, sp_, 1, st, pdl);
+                } else if (o.fr.qkv) {
                     FusedRope fr = o.fr;
                     fr.cs_table = rope_table_;
                     e = launch_attend(o.x, kv_[o.kv].k, kv_[o.kv].v, kv_f16_, o.y, sp_, o.attn, status_, att_scratch_, st, pdl, &fr);
@@ -797,12 +847,22 @@ int DecodePlanImpl::run_ops_multi(cudaStream_t st, int nt, std::string& err, boo
                     e = launch_gemv_f8_float(o.w, o.pair ? &o.w2 : nullptr, A(o.x, tk), A(o.y, tk), o.mode, A(o.z, tk), sm_count_, st, pdl());
                 break;
             case B2_OP_QK_ROPE:  // all tokens in one launch (the one-token arithmetic per head)
+                if (kv8_) {
+                    e = rope_kv8(o, sp_multi_, (uint32_t)nt, true, st, chained);
+                    first = false;
+                    count += 2;
+                    break;
+                }
                 e = launch_qk_rope_rows(o.x, o.y, block_floats_, (uint32_t)nt, kv_[o.kv].k, kv_[o.kv].v, kv_f16_, o.p0, o.p1, rope_table_, sp_multi_, o.rope,
                                         st);
                 first = false;
                 count++;
                 break;
             case B2_OP_ATTEND: {
+                if (kv8_) {
+                    e = attend_kv8(o, sp_multi_, (uint32_t)nt, st, pdl());
+                    break;
+                }
                 // One launch attends for all tokens, and rotates and appends where the one-token plan's does. Otherwise it is an
                 // ordinary launch: all tokens' rows of the caches come from the launch just ahead of it.
                 const AttnTokens at{nt, block_floats_};
@@ -834,7 +894,11 @@ int DecodePlanImpl::capture(cudaStream_t st, bool with_head, cudaGraphExec_t* ou
     cudaError_t e = cudaSuccess;
     if (with_head) e = launch_dequantize(gen_embed_dev_, 0, 1, input_, st, token_);
     if (e == cudaSuccess) rc = nt > 1 ? run_ops_multi(st, nt, err, pdl_) : run_ops(st, err, pdl_, with_head);
-    if (e == cudaSuccess && rc == B2_OK && with_head)
+    if (e == cudaSuccess && rc == B2_OK && with_head && out == &gen_rules_exec_) {
+        int32_t* const w = gen_rules_.words;
+        e = launch_logits(logits_, nullptr, B2_F32, n_logits_, n_logits_, 1, n_logits_, gen_rules_.dev, w + 4, status_, st, pdl_);
+        if (e == cudaSuccess) e = launch_advance(w + 4, token_, out_tokens_, const_cast<int32_t*>(gen_rules_.dev.history), w, sp_, st, pdl_);
+    } else if (e == cudaSuccess && rc == B2_OK && with_head)
         e = launch_argmax(logits_, n_logits_, argmax_val_, argmax_idx_, argmax_counter_, token_, out_tokens_, sp_, st, pdl_);
     cudaGraph_t graph = nullptr;
     cudaError_t e2 = cudaStreamEndCapture(st, &graph);
@@ -1056,12 +1120,19 @@ int DecodePlanImpl::run_prefill(cudaStream_t st, size_t pos, size_t t, std::stri
                 break;
             }
             case B2_OP_QK_ROPE:
-                e = launch_qk_rope_rows(o.x, o.y, ld, rows, kv_[o.kv].k, kv_[o.kv].v, kv_f16_, o.p0, o.p1, rope_table_, sp_, o.rope, st);
+                if (kv8_) {
+                    e = rope_kv8(o, sp_, rows, true, st, false);
+                    count++;
+                } else
+                    e = launch_qk_rope_rows(o.x, o.y, ld, rows, kv_[o.kv].k, kv_[o.kv].v, kv_f16_, o.p0, o.p1, rope_table_, sp_, o.rope, st);
                 count++;
                 if (overlaps_f(o.y, (size_t)o.rope.nh * o.rope.hd, x16_src, x16_k)) x16_src = nullptr;
                 break;
             case B2_OP_ATTEND:
-                if (loop_attend_) {
+                if (kv8_) {
+                    e = attend_kv8(o, sp_, rows, st, false);
+                    count++;
+                } else if (loop_attend_) {
                     for (size_t tk = 0; tk < t && e == cudaSuccess; tk++, count++)
                         e = launch_attend(o.x + tk * ld, kv_[o.kv].k, kv_[o.kv].v, kv_f16_, o.y + tk * ld, sp_multi_ + 4 * tk, o.attn, status_, att_scratch_, st);
                 } else {
@@ -1152,6 +1223,17 @@ int DecodePlanImpl::kv_write(cudaStream_t st, uint32_t kv, size_t pos0, size_t n
     }
     const Kv& c = kv_[kv];
     const size_t row = (size_t)c.nkv * c.hd, chunk = stage_floats_ / row;
+    for (size_t at = 0, m = 0; kv8_ && at < n; at += m) {  // (runs that end where blocks do: a block's rows go in together)
+        m = std::min(chunk / KV8_BLOCK * KV8_BLOCK - (pos0 + at) % KV8_BLOCK, n - at);
+        const uint32_t first = (uint32_t)(pos0 + at);
+        PLAN_CUDA(cudaMemcpyAsync(stage_, k + at * row, m * row * 4, cudaMemcpyHostToDevice, st), "cudaMemcpy(K rows)");
+        PLAN_CUDA(cudaMemcpyAsync(stage_ + stage_floats_, v + at * row, m * row * 4, cudaMemcpyHostToDevice, st), "cudaMemcpy(V rows)");
+        PLAN_CUDA(cudaMemcpyAsync(kv8_at_, &first, 4, cudaMemcpyHostToDevice, st), "cudaMemcpy(position)");
+        const Kv8Cache cache{(uint8_t*)c.k, c.nkv, c.hd, (max_len_ + KV8_BLOCK - 1) / KV8_BLOCK};
+        PLAN_CUDA(launch_kv8_append(cache, kv8_seqs(kv8_at_, (uint32_t)m), Kv8Rows{stage_, stage_ + stage_floats_, B2_F32, row, c.hd}, true, status_, st), "kv8 rows");
+        PLAN_CUDA(cudaStreamSynchronize(st), "kv_write");
+    }
+    if (kv8_) return B2_OK;
     for (size_t at = 0; at < n; at += chunk) {
         size_t m = std::min(chunk, n - at);
         PLAN_CUDA(cudaMemcpyAsync(stage_, k + at * row, m * row * 4, cudaMemcpyHostToDevice, st), "cudaMemcpy(K rows)");
@@ -1171,6 +1253,17 @@ int DecodePlanImpl::kv_read(cudaStream_t st, uint32_t kv, size_t pos0, size_t n,
     }
     const Kv& c = kv_[kv];
     const size_t row = (size_t)c.nkv * c.hd, chunk = stage_floats_ / row;
+    for (size_t at = 0; kv8_ && at < n; at += chunk) {
+        const size_t m = std::min(chunk, n - at);
+        const uint32_t first = (uint32_t)(pos0 + at);
+        PLAN_CUDA(cudaMemcpyAsync(kv8_at_, &first, 4, cudaMemcpyHostToDevice, st), "cudaMemcpy(position)");
+        const Kv8Cache cache{(uint8_t*)c.k, c.nkv, c.hd, (max_len_ + KV8_BLOCK - 1) / KV8_BLOCK};
+        PLAN_CUDA(launch_kv8_read(cache, kv8_seqs(kv8_at_, (uint32_t)m), stage_, stage_ + stage_floats_, status_, st), "kv8 rows");
+        PLAN_CUDA(cudaMemcpyAsync(k + at * row, stage_, m * row * 4, cudaMemcpyDeviceToHost, st), "cudaMemcpy(K rows)");
+        PLAN_CUDA(cudaMemcpyAsync(v + at * row, stage_ + stage_floats_, m * row * 4, cudaMemcpyDeviceToHost, st), "cudaMemcpy(V rows)");
+        PLAN_CUDA(cudaStreamSynchronize(st), "kv_read");
+    }
+    if (kv8_) return B2_OK;
     for (size_t at = 0; at < n; at += chunk) {
         size_t m = std::min(chunk, n - at);
         PLAN_CUDA(launch_kv_rows(stage_, c.k, kv_f16_, false, c.nkv, c.hd, max_len_, (uint32_t)(pos0 + at), (uint32_t)m, st), "kv_rows");
@@ -1183,8 +1276,67 @@ int DecodePlanImpl::kv_read(cudaStream_t st, uint32_t kv, size_t pos0, size_t n,
     return B2_OK;
 }
 
+// The rules on the device. Their graph is captured anew where what it holds by value has changed: penalties, addresses, room.
+int DecodePlanImpl::put_rules(cudaStream_t st, const b2_generate_rules& r, size_t n_tokens, std::string& err) {
+    const bool penal = r.repeat != 1.0f || r.frequency != 0.0f || r.presence != 0.0f;
+    const size_t words = ((size_t)n_logits_ + 31) / 32, n_prompt = penal ? r.n_prompt : 0;  // (without penalties nobody reads the history)
+    if (!(r.repeat > 0.0f) || !std::isfinite(r.repeat) || !std::isfinite(r.frequency) || !std::isfinite(r.presence) || (r.n_prompt && !r.prompt) ||
+        (r.n_bias && (!r.bias_ids || !r.bias)) || r.n_prompt > 1u << 30 || r.n_bias > 1u << 30) {
+        err = "[b200qmm: plan generate: penalties are finite, the one for repetition above zero, and lists are not missing]";
+        return B2_ERR_ARG;
+    }
+    if (r.mask) {
+        bool some = false;
+        for (size_t i = 0; i < words && !some; i++) some = (i + 1 < words || n_logits_ % 32 == 0 ? r.mask[i] : r.mask[i] & ((1u << n_logits_ % 32) - 1)) != 0;
+        if (!some) {
+            err = "[b200qmm: plan generate: the mask allows no token]";
+            return B2_ERR_ARG;
+        }
+    }
+    GenRules& d = gen_rules_;
+    const size_t n_history = n_prompt + n_tokens, n_bias = r.n_bias;
+    if (!d.words) PLAN_CUDA(cudaMalloc((void**)&d.words, 8 * 4), "cudaMalloc(rules)");
+    if (!d.room || n_history > d.dev.n_history || n_bias > d.dev.n_bias) {
+        const size_t h = align_up(std::max(n_history, (size_t)d.dev.n_history), 1024), b = align_up(std::max(n_bias, (size_t)d.dev.n_bias), 64);
+        if (gen_rules_exec_) cudaGraphExecDestroy(gen_rules_exec_);
+        gen_rules_exec_ = nullptr;
+        if (d.room) cudaFree(d.room);
+        d.room = nullptr;
+        PLAN_CUDA(cudaMalloc(&d.room, (h + 2 * b + words) * 4), "cudaMalloc(rules)");
+        int32_t* const at = (int32_t*)d.room;
+        d.dev.history = at;
+        d.dev.n_history = (uint32_t)h;
+        d.dev.bias_ids = at + h;
+        d.dev.bias = (const float*)(at + h + b);
+        d.dev.n_bias = (uint32_t)b;
+        d.dev.mask = (const uint32_t*)(at + h + 2 * b);
+        d.dev.history_ptr = d.words;
+        d.dev.bias_ptr = d.words + 2;
+    }
+    LogitRulesDev now = d.dev;
+    now.repeat = r.repeat;
+    now.frequency = r.frequency;
+    now.presence = r.presence;
+    now.mask = r.mask ? (const uint32_t*)((int32_t*)d.room + d.dev.n_history + 2 * (size_t)d.dev.n_bias) : nullptr;
+    if (gen_rules_exec_ && (now.repeat != d.dev.repeat || now.frequency != d.dev.frequency || now.presence != d.dev.presence || now.mask != d.dev.mask)) {
+        cudaGraphExecDestroy(gen_rules_exec_);
+        gen_rules_exec_ = nullptr;
+    }
+    d.dev = now;
+    d.parts[1] = (int32_t)n_prompt;
+    d.parts[3] = (int32_t)n_bias;
+    if (n_prompt) PLAN_CUDA(cudaMemcpyAsync((void*)now.history, r.prompt, n_prompt * 4, cudaMemcpyHostToDevice, st), "cudaMemcpy(history)");
+    if (n_bias) {
+        PLAN_CUDA(cudaMemcpyAsync((void*)now.bias_ids, r.bias_ids, n_bias * 4, cudaMemcpyHostToDevice, st), "cudaMemcpy(biases)");
+        PLAN_CUDA(cudaMemcpyAsync((void*)now.bias, r.bias, n_bias * 4, cudaMemcpyHostToDevice, st), "cudaMemcpy(biases)");
+    }
+    if (r.mask) PLAN_CUDA(cudaMemcpyAsync((void*)now.mask, r.mask, words * 4, cudaMemcpyHostToDevice, st), "cudaMemcpy(mask)");
+    PLAN_CUDA(cudaStreamSynchronize(st), "rules");  // (the caller's arrays are only read during the call)
+    return B2_OK;
+}
+
 int DecodePlanImpl::generate(cudaStream_t st, uint64_t embed_handle, const WeightDev& embed, int32_t first_token, size_t pos0, size_t n_tokens,
-                             const float* rope_cs_table, int32_t* out_tokens, float* elapsed_ms, std::string& err) {
+                             const float* rope_cs_table, const b2_generate_rules* rules, int32_t* out_tokens, float* elapsed_ms, std::string& err) {
     if (!n_logits_ || !logits_) {
         err = "[b200qmm: plan generate: the graph has no logits]";
         return B2_ERR_ARG;
@@ -1202,7 +1354,33 @@ int DecodePlanImpl::generate(cudaStream_t st, uint64_t embed_handle, const Weigh
         err = "[b200qmm: plan generate: the embedding matrix does not match the graph's input, or the token is outside it]";
         return B2_ERR_ARG;
     }
-    if (!gen_exec_ || gen_embed_ != embed_handle || gen_embed_dev_.p0 != embed.p0) {
+    if (rules) {
+        if (int rc = put_rules(st, *rules, n_tokens, err)) return rc;
+        if (!gen_rules_exec_ || gen_rules_.embed != embed_handle || gen_rules_.embed_p0 != embed.p0) {
+            if (gen_rules_exec_) cudaGraphExecDestroy(gen_rules_exec_);
+            gen_rules_exec_ = nullptr;
+            // the kernels that the step graph does not have, once outside a capture (their words are set anew below)
+            gen_embed_dev_ = embed;
+            int32_t* const w = gen_rules_.words;
+            PLAN_CUDA(cudaMemsetAsync(w, 0, 8 * 4, cap_stream_), "cudaMemset(rules)");
+            PLAN_CUDA(launch_set_step(sp_, 0, 0, 0, token_, first_token, cap_stream_), "set_step");
+            PLAN_CUDA(launch_dequantize(embed, 0, 1, input_, cap_stream_, token_), "embedding lookup");
+            LogitRulesDev none = gen_rules_.dev;
+            none.n_history = none.n_bias = 0;
+            none.mask = nullptr;
+            PLAN_CUDA(launch_logits(logits_, nullptr, B2_F32, n_logits_, n_logits_, 1, n_logits_, none, w + 4, status_, cap_stream_), "logits");
+            PLAN_CUDA(launch_advance(w + 4, token_, out_tokens_, w + 5, w, sp_, cap_stream_), "advance");
+            PLAN_CUDA(cudaStreamSynchronize(cap_stream_), "generate warm-up");
+            int rc = capture(cap_stream_, true, &gen_rules_exec_, err);
+            if (gen_exec_) {  // (its embedding may be another)
+                cudaGraphExecDestroy(gen_exec_);
+                gen_exec_ = nullptr;
+            }
+            if (rc) return rc;
+            gen_rules_.embed = gen_embed_ = embed_handle;
+            gen_rules_.embed_p0 = embed.p0;
+        }
+    } else if (!gen_exec_ || gen_embed_ != embed_handle || gen_embed_dev_.p0 != embed.p0) {
         if (gen_exec_) cudaGraphExecDestroy(gen_exec_);
         gen_exec_ = nullptr;
         gen_embed_ = embed_handle;
@@ -1215,11 +1393,12 @@ int DecodePlanImpl::generate(cudaStream_t st, uint64_t embed_handle, const Weigh
         int rc = capture(cap_stream_, true, &gen_exec_, err);
         if (rc) return rc;
     }
+    if (rules) PLAN_CUDA(cudaMemcpyAsync(gen_rules_.words, gen_rules_.parts, sizeof gen_rules_.parts, cudaMemcpyHostToDevice, st), "cudaMemcpy(rules)");
     PLAN_CUDA(launch_set_step(sp_, (uint32_t)pos0, (uint32_t)pos0, 0, token_, first_token, st), "set_step");
     if (cs_stride_)
         PLAN_CUDA(cudaMemcpyAsync(rope_table_, rope_cs_table, n_tokens * cs_stride_ * sizeof(float), cudaMemcpyHostToDevice, st), "cudaMemcpy(rope)");
     PLAN_CUDA(cudaEventRecord(ev0_, st), "cudaEventRecord");
-    for (size_t i = 0; i < n_tokens; i++) PLAN_CUDA(cudaGraphLaunch(gen_exec_, st), "cudaGraphLaunch");
+    for (size_t i = 0; i < n_tokens; i++) PLAN_CUDA(cudaGraphLaunch(rules ? gen_rules_exec_ : gen_exec_, st), "cudaGraphLaunch");
     PLAN_CUDA(cudaEventRecord(ev1_, st), "cudaEventRecord");
     PLAN_CUDA(cudaMemcpyAsync(out_tokens, out_tokens_, n_tokens * sizeof(int), cudaMemcpyDeviceToHost, st), "cudaMemcpy(tokens)");
     PLAN_CUDA(cudaStreamSynchronize(st), "generate");

@@ -35,8 +35,9 @@ class DecodePlanImpl {
     float last_step_ms() const { return last_ms_; }  // device time of the last prefill step's kernels (without the copies)
     int kv_write(cudaStream_t st, uint32_t kv, size_t pos0, size_t n, const float* k, const float* v, std::string& err);
     int kv_read(cudaStream_t st, uint32_t kv, size_t pos0, size_t n, float* k, float* v, std::string& err);
+    // rules: null for the plain greedy choice.
     int generate(cudaStream_t st, uint64_t embed_handle, const WeightDev& embed, int32_t first_token, size_t pos0, size_t n_tokens,
-                 const float* rope_cs_table, int32_t* out_tokens, float* elapsed_ms, std::string& err);
+                 const float* rope_cs_table, const b2_generate_rules* rules, int32_t* out_tokens, float* elapsed_ms, std::string& err);
     int export_handle(void* out128, std::string& err);
     int attach_peers(uint32_t rank, uint32_t world, const void* handles, std::string& err);
     uint64_t launches_per_step() const { return prefill_ ? prefill_launches_ : launches_; }
@@ -81,6 +82,11 @@ class DecodePlanImpl {
     int run_ops_multi(cudaStream_t st, int nt, std::string& err, bool chained);
     int run_prefill(cudaStream_t st, size_t pos, size_t t, std::string& err);
     int step_prefill(cudaStream_t st, size_t pos, size_t t, const float* x, const float* rope_cs, float* hidden, std::string& err);
+    // Rotated queries where the op wants them and the step's rows into an 8-bit cache; attention over it. at: the first token's position on the device.
+    cudaError_t rope_kv8(const Op& o, const uint32_t* at, uint32_t nt, bool rows_kernel, cudaStream_t st, bool pdl);
+    cudaError_t attend_kv8(const Op& o, const uint32_t* at, uint32_t nt, cudaStream_t st, bool pdl);
+    Kv8Seqs kv8_seqs(const uint32_t* at, uint32_t nt) const { return Kv8Seqs{1, nt, nt, (max_len_ + KV8_BLOCK - 1) / KV8_BLOCK, nullptr, (const int32_t*)at, nullptr}; }
+    int put_rules(cudaStream_t st, const b2_generate_rules& r, size_t n_tokens, std::string& err);
     int capture(cudaStream_t st, bool with_head, cudaGraphExec_t* out, std::string& err, int nt = 1);
     int check_status(std::string& err);
 
@@ -130,6 +136,10 @@ class DecodePlanImpl {
     std::vector<Kv> kv_;
     uint32_t max_len_ = 0;
     int kv_f16_ = 0;
+    bool kv8_ = false;            // 8-bit caches: Kv::k holds the units of kv8.cuh, v is null
+    float* kv8_rows_ = nullptr;   // [2][largest nkv hd][tokens]: a step's rotated keys and its values on their way into one
+    size_t kv8_row_floats_ = 0;   // of one of the two
+    uint32_t* kv8_at_ = nullptr;  // a word of words_: kv_write's and kv_read's first position
     AttScratch att_scratch_;      // (the counts are words)
     uint32_t* words_ = nullptr;   // sp[4] | status | argmax counter | - | - | sp[4] of each token of a step | attention counts
     uint32_t* sp_ = nullptr;
@@ -148,6 +158,16 @@ class DecodePlanImpl {
     cudaStream_t cap_stream_ = nullptr;
     cudaGraphExec_t step_exec_ = nullptr;
     cudaGraphExec_t gen_exec_ = nullptr;
+    cudaGraphExec_t gen_rules_exec_ = nullptr;  // the same with rules on the logits
+    struct GenRules {  // device copies; list lengths are what there is room for, the rows' parts are in the words
+        LogitRulesDev dev{};
+        void* room = nullptr;        // history | bias ids | biases | mask
+        size_t room_bytes = 0;
+        int32_t* words = nullptr;    // history's part (2), the biases' (2), the choice (1)
+        int32_t parts[4] = {};       // what they begin with
+        uint64_t embed = 0;
+        const uint8_t* embed_p0 = nullptr;
+    } gen_rules_;
     uint64_t gen_embed_ = 0;
     WeightDev gen_embed_dev_{};
     cudaEvent_t ev0_ = nullptr, ev1_ = nullptr;

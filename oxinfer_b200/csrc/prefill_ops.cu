@@ -29,7 +29,7 @@ __global__ void __launch_bounds__(256) qk_rope_rows_kernel(const float* __restri
     __shared__ float red[32];
     pdl_launch_dependents();
     const size_t off = (size_t)blockIdx.y * stride;
-    rope_head<T>(blockIdx.x, threadIdx.x, sp[0] + blockIdx.y, sp[1], qkv + off, qo + off, kc, vc, qn, kn, cs_table, p, buf, red);
+    rope_head<T>(blockIdx.x, threadIdx.x, sp[0] + blockIdx.y, sp[1], p.staged ? blockIdx.y : sp[0] + blockIdx.y, qkv + off, qo + off, kc, vc, qn, kn, cs_table, p, buf, red);
 }
 
 // RoPE and cache append without per-head norms: a warp per head of a token, lane l owning dimensions 4 l .. 4 l + 3 (and
@@ -56,11 +56,11 @@ __global__ void __launch_bounds__(256) qk_rope_fast_kernel(const float* __restri
     const uint32_t tok = unit / heads, h = unit - tok * heads;
     const uint32_t kind = h < p.nh ? 0 : (h < p.nh + p.nkv ? 1 : 2);
     const uint32_t hh = kind == 0 ? h : (kind == 1 ? h - p.nh : h - p.nh - p.nkv);
-    const uint32_t pos = sp[0] + tok, hd = p.hd, hr = p.half_rot;
-    if (pos >= p.max_len) return;
+    const uint32_t pos = sp[0] + tok, row = p.staged ? tok : pos, hd = p.hd, hr = p.half_rot;
+    if (row >= p.max_len) return;
     const float* src = qkv + (size_t)tok * stride + (kind == 0 ? hh * p.q_stride : (kind == 1 || p.v_from_k) ? p.k_off + hh * hd : p.v_off + hh * hd);
     const float* cs = cs_table + (size_t)(pos - sp[1]) * p.cs_stride + p.cs_off;
-    const size_t at = ((size_t)hh * p.max_len + pos) * hd;
+    const size_t at = ((size_t)hh * p.max_len + row) * hd;
     for (uint32_t d0 = 4 * lane; d0 < hd; d0 += 128) {
         float4 v = *(const float4*)(src + d0);
         if (kind != 2 && d0 < 2 * hr) {

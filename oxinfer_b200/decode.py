@@ -180,20 +180,28 @@ class DecodePlan:
         self._be._check(self._be._L.b2_plan_kv_read(self._be._ctx, self.handle, kv, pos0, n, k.ctypes.data, v.ctypes.data))
         return k, v
 
-    def generate(self, embed, first_token: int, pos0: int, n_tokens: int, rope_cs_table: np.ndarray):
-        """Greedy tokens without the host in the loop: returns (tokens int32 [n_tokens], device milliseconds)."""
+    def generate(self, embed, first_token: int, pos0: int, n_tokens: int, rope_cs_table: np.ndarray, rules=None):
+        """Greedy tokens without the host in the loop: returns (tokens int32 [n_tokens], device milliseconds). ``rules``: ``sampling.GenerateRules`` for the
+        logits of every step."""
         cs = np.ascontiguousarray(rope_cs_table, dtype=np.float32)
         assert cs.size == n_tokens * self.cs_stride
         out = np.empty(n_tokens, dtype=np.int32)
         ms = C.c_float()
-        self._be._check(self._be._L.b2_plan_generate(self._be._ctx, self.handle, embed.handle, first_token, pos0, n_tokens, cs.ctypes.data,
-                                                     out.ctypes.data, C.byref(ms)))
+        if rules is None:
+            self._be._check(self._be._L.b2_plan_generate(self._be._ctx, self.handle, embed.handle, first_token, pos0, n_tokens, cs.ctypes.data,
+                                                         out.ctypes.data, C.byref(ms)))
+        else:
+            r, keep = rules.c(self.graph.logits[1] if self.graph.logits else 0)
+            self._be._check(self._be._L.b2_plan_generate_ruled(self._be._ctx, self.handle, embed.handle, first_token, pos0, n_tokens, cs.ctypes.data,
+                                                               C.byref(r), out.ctypes.data, C.byref(ms)))
         return out, ms.value
 
 
-def decode_plan(be, g: Graph, max_len: int, kv_f16: bool = False, tokens: int = 1, prefill: bool = False) -> DecodePlan | None:
+def decode_plan(be, g: Graph, max_len: int, kv_f16: bool = False, tokens: int = 1, prefill: bool = False, kv_i8: bool = False) -> DecodePlan | None:
     """``Backend::decode_plan`` (``src/gpu.rs:262-289``): a plan, or ``None`` when the graph is declined. ``tokens`` > 1:
-    ``Backend::decode_plan_multi`` (``src/gpu.rs:273-276``), steps of up to that many tokens."""
+    ``Backend::decode_plan_multi`` (``src/gpu.rs:273-276``), steps of up to that many tokens. ``kv_f16`` / ``kv_i8``: caches of f16, or of 8-bit integers with
+    a scale for 32 tokens (``B2_KV_I8``), instead of f32."""
+    assert not (kv_f16 and kv_i8)
     bufs = (C.c_uint64 * len(g.bufs))(*g.bufs)
     ops = (_lib.Op * len(g.ops))(*g.ops)
     nkv = (C.c_uint32 * max(1, len(g.kv)))(*[k[0] for k in g.kv])
@@ -202,7 +210,7 @@ def decode_plan(be, g: Graph, max_len: int, kv_f16: bool = False, tokens: int = 
     lv, ln = g.logits if g.logits else (View(0), 0)
     desc = _lib.GraphDesc(bufs=bufs, n_bufs=len(g.bufs), ops=ops, n_ops=len(g.ops), input=g.input.c(), n_input=g.n_input, hidden=g.hidden.c(),
                           n_hidden=g.n_hidden, logits=lv.c(), n_logits=ln, kv_nkv=nkv, kv_hd=hd, n_kv=len(g.kv), rope_halves=halves,
-                          n_rope=len(g.rope_halves), max_len=max_len, kv_f16=int(kv_f16))
+                          n_rope=len(g.rope_halves), max_len=max_len, kv_f16=_lib.KV_I8 if kv_i8 else int(kv_f16))
     h = C.c_uint64()
     if prefill:
         rc = be._L.b2_decode_plan_prefill(be._ctx, C.byref(desc), tokens, C.byref(h))
@@ -215,15 +223,15 @@ def decode_plan(be, g: Graph, max_len: int, kv_f16: bool = False, tokens: int = 
     return DecodePlan(be, h.value, g, max_len)
 
 
-def decode_plan_multi(be, g: Graph, max_len: int, tokens: int, kv_f16: bool = False) -> DecodePlan | None:
+def decode_plan_multi(be, g: Graph, max_len: int, tokens: int, kv_f16: bool = False, kv_i8: bool = False) -> DecodePlan | None:
     """``Backend::decode_plan_multi`` (``src/gpu.rs:273-276``); also what ``decode_plan_multi_fast`` gives (the exact plan)."""
-    return decode_plan(be, g, max_len, kv_f16=kv_f16, tokens=tokens)
+    return decode_plan(be, g, max_len, kv_f16=kv_f16, tokens=tokens, kv_i8=kv_i8)
 
 
-def decode_plan_prefill(be, g: Graph, max_len: int, tokens: int, kv_f16: bool = False) -> DecodePlan | None:
+def decode_plan_prefill(be, g: Graph, max_len: int, tokens: int, kv_f16: bool = False, kv_i8: bool = False) -> DecodePlan | None:
     """``Backend::decode_plan_prefill`` (``src/gpu.rs:283-289``): steps of up to ``tokens`` tokens on batched kernels; the graph
     has no head. Steps go through ``DecodePlan.step_multi``."""
-    return decode_plan(be, g, max_len, kv_f16=kv_f16, tokens=tokens, prefill=True)
+    return decode_plan(be, g, max_len, kv_f16=kv_f16, tokens=tokens, prefill=True, kv_i8=kv_i8)
 
 
 # ---- RoPE tables (src/kernels.rs:2277-2306) ---------------------------------------------------------

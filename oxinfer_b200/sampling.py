@@ -5,7 +5,32 @@ from __future__ import annotations
 
 from dataclasses import dataclass
 
+import numpy as np
+
 from . import _lib
+
+
+@dataclass
+class GenerateRules:
+    """Rules for every step of ``DecodePlan.generate`` (``b2_generate_rules``), host arrays: the history is ``prompt`` and what the call has chosen so far."""
+    repeat: float = 1.0
+    frequency: float = 0.0
+    presence: float = 0.0
+    prompt: np.ndarray | None = None     # int32
+    bias_ids: np.ndarray | None = None   # int32
+    bias: np.ndarray | None = None       # float32
+    mask: np.ndarray | None = None       # uint32 words, bit i % 32 of word i / 32: token i is allowed
+
+    def c(self, n: int):
+        """The struct, and the arrays that it points into."""
+        prompt, ids = (None if x is None else np.ascontiguousarray(x, dtype=np.int32) for x in (self.prompt, self.bias_ids))
+        bias = None if self.bias is None else np.ascontiguousarray(self.bias, dtype=np.float32)
+        mask = None if self.mask is None else np.ascontiguousarray(self.mask).view(np.uint32)
+        assert (ids is None) == (bias is None) and (ids is None or ids.size == bias.size)
+        assert mask is None or mask.size == (n + 31) // 32
+        ptr = lambda x: x.ctypes.data if x is not None and x.size else None
+        size = lambda x: x.size if x is not None else 0
+        return _lib.GenerateRules(self.repeat, self.frequency, self.presence, size(prompt), size(ids), ptr(prompt), ptr(ids), ptr(bias), ptr(mask)), (prompt, ids, bias, mask)
 
 
 @dataclass
