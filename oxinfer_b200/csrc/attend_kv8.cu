@@ -28,17 +28,17 @@ namespace {
 constexpr int AK_WARPS = 4, AK_THREADS = AK_WARPS * 32;
 constexpr float P_BITS = 14.0f;  // probabilities are held 2^14 times as large: what is below 2^-28 of a row's largest loses bits, not before
 
-template <int HD>
+template <int HD, int TERMS>
 struct AkShared {
     static constexpr uint32_t UNIT = unit_bytes(HD);
-    static constexpr int STAGES = HD == 128 ? 3 : 6;
+    static constexpr int CTAS = TERMS == 2 ? 3 : 2;                // of an SM (registers)
+    static constexpr int STAGES = (TERMS == 2 ? 2 : 3) * (HD == 128 ? 1 : 2);
     static constexpr uint32_t RING = STAGES * UNIT;
-    static constexpr uint32_t SUM = AK_WARPS * RING;               // [16][HD] the CTA's sums
-    static constexpr uint32_t ML = SUM + 16 * HD * 4;              // [16] largest, [16] denominators of the CTA, then of the warps [warp][16][2]
+    static constexpr uint32_t ML = AK_WARPS * RING;                // [16] largest, [16] denominators of the CTA, then of the warps [warp][16][2]
     static constexpr uint32_t BARS = ML + (2 + 2 * AK_WARPS) * 16 * 4;
     static constexpr uint32_t BYTES = BARS + AK_WARPS * STAGES * 8;
     static_assert(RING >= 16 * HD * 4, "a warp's sums take its ring's place");
-    static_assert(BYTES + 1024 <= 228 * 1024 / 2, "two CTAs an SM");
+    static_assert(CTAS * (BYTES + 1024) <= 228 * 1024);
 };
 
 struct AkArgs {
@@ -86,7 +86,7 @@ __device__ __forceinline__ uint32_t pack_rest(float a, float b, uint32_t hi) {
 __device__ __forceinline__ float capped(float x, float cap2, float cap_in) {
     const float z = 0.5f * 0.69314718f * (x * cap_in), z2 = z * z;
     const float series = z * fmaf(z2, fmaf(z2, fmaf(z2, fmaf(z2, 62.0f / 2835.0f, -17.0f / 315.0f), 2.0f / 15.0f), -1.0f / 3.0f), 1.0f);
-    const float far = 1.0f - 2.0f * __frcp_rn(1.0f + ex2(x * cap_in));
+    const float far = 1.0f - __fdividef(2.0f, 1.0f + ex2(x * cap_in));
     return cap2 * (fabsf(z) < 0.3f ? series : far);
 }
 template <typename T>
@@ -140,8 +140,8 @@ __device__ __forceinline__ float weight_of(float m, float most) { return ex2(m -
 
 // A CTA's grid index: (unit of work, CTA of the cluster); a unit: (sequence, tile of rows from the last on, KV head).
 template <int HD, int TERMS, typename T>
-__global__ void __launch_bounds__(AK_THREADS, 2) attend_kv8_kernel(const AkArgs a) {
-    using L = AkShared<HD>;
+__global__ void __launch_bounds__(AK_THREADS, TERMS == 2 ? 3 : 2) attend_kv8_kernel(const AkArgs a) {
+    using L = AkShared<HD, TERMS>;
     constexpr int R = TERMS == 2 ? 8 : 16, RG = TERMS == 2 ? 1 : 2;  // rows of a tile; a lane's rows
     constexpr int KS = HD / 16, NT = HD / 8, QD = HD / 4, S = L::STAGES;
     extern __shared__ __align__(128) uint8_t smem[];
@@ -151,7 +151,7 @@ __global__ void __launch_bounds__(AK_THREADS, 2) attend_kv8_kernel(const AkArgs 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     uint8_t* const ring = smem + warp * L::RING;
     uint64_t* const bars = (uint64_t*)(smem + L::BARS) + warp * S;
-    float* const sum_s = (float*)(smem + L::SUM);
+    float* const sum_s = (float*)smem;  // the CTA's sums, where the first warp's were
     float* const m_s = (float*)(smem + L::ML);
     float* const l_s = m_s + 16;
     float* const wm = l_s + 16;                 // [warp][16]
@@ -457,7 +457,7 @@ __global__ void __launch_bounds__(AK_THREADS, 2) attend_kv8_kernel(const AkArgs 
 
 template <int HD, int TERMS, typename T>
 cudaError_t attend_t(AkArgs& a, uint32_t units_per_tile, cudaStream_t st, bool pdl) {
-    using L = AkShared<HD>;
+    using L = AkShared<HD, TERMS>;
     constexpr uint32_t R = TERMS == 2 ? 8 : 16;
     auto kern = attend_kv8_kernel<HD, TERMS, T>;
     const size_t rows = (size_t)a.sq.max_rows * a.G;
@@ -471,6 +471,7 @@ cudaError_t attend_t(AkArgs& a, uint32_t units_per_tile, cudaStream_t st, bool p
     uint32_t C = 1;
     const size_t blocks = a.window && !a.prefix ? std::min<size_t>(a.sq.max_blocks, ((size_t)a.window + a.sq.max_rows) / KV8_BLOCK + 2) : a.sq.max_blocks;
     while (C < 16 && units * C * 2 <= (C == 8 ? 224 : 288) && blocks >= 2 * C * 2 * AK_WARPS) C *= 2;
+    if (getenv("AK_C")) C = atoi(getenv("AK_C"));
     if (cudaError_t e = ensure_dynamic_smem((const void*)kern, L::BYTES, 0); e != cudaSuccess) return e;
     if (cudaError_t e = cudaFuncSetAttribute((const void*)kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1); e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
