@@ -471,7 +471,6 @@ cudaError_t attend_t(AkArgs& a, uint32_t units_per_tile, cudaStream_t st, bool p
     uint32_t C = 1;
     const size_t blocks = a.window && !a.prefix ? std::min<size_t>(a.sq.max_blocks, ((size_t)a.window + a.sq.max_rows) / KV8_BLOCK + 2) : a.sq.max_blocks;
     while (C < 16 && units * C * 2 <= (C == 8 ? 224 : 288) && blocks >= 2 * C * 2 * AK_WARPS) C *= 2;
-    if (getenv("AK_C")) C = atoi(getenv("AK_C"));
     if (cudaError_t e = ensure_dynamic_smem((const void*)kern, L::BYTES, 0); e != cudaSuccess) return e;
     if (cudaError_t e = cudaFuncSetAttribute((const void*)kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1); e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
@@ -507,6 +506,10 @@ cudaError_t launch_attend_kv8(const Kv8Cache& c, const Kv8Seqs& s, const Kv8Attn
                               uint32_t* status, cudaStream_t st, bool pdl) {
     if (!kv8_supports(c.nkv, c.hd) || p.nh == 0 || p.nh % c.nkv) return cudaErrorInvalidValue;
     if (s.n_seqs == 0 || s.n_rows == 0 || s.max_rows == 0) return cudaSuccess;
+    // Many rows go to the form on tcgen05, from 64 of a KV head and sequence on. mma.sync / tcgen05, us, 4 heads a KV head, 8 KV heads of 128, one sequence behind
+    // 4096 keys, eight behind 1024, 32 behind 512: 64 rows 18.1 / 19.7, 22.1 / 18.3, 35.5 / 31.2; 128 rows 26.3 / 21.4, 28.2 / 21.9, 62.8 / 36.1; 512 rows 76 / 30, 84 / 31.
+    if ((dtype != B2_F32 || p.halves) && (size_t)s.max_rows * (p.nh / c.nkv) >= 64)
+        return launch_attend_kv8_rows(c, s, p, q, q_stride, out, out_stride, dtype, status, st, pdl);
     AkArgs a{};
     a.c = c;
     a.sq = s;

@@ -751,7 +751,7 @@ cudaError_t DecodePlanImpl::rope_kv8(const Op& o, const uint32_t* at, uint32_t n
 }
 cudaError_t DecodePlanImpl::attend_kv8(const Op& o, const uint32_t* at, uint32_t nt, cudaStream_t st, bool pdl) {
     const Kv8Cache c{(uint8_t*)kv_[o.kv].k, o.attn.nkv, o.attn.hd, (max_len_ + KV8_BLOCK - 1) / KV8_BLOCK};
-    return launch_attend_kv8(c, kv8_seqs(at, nt), Kv8Attn{o.attn.nh, o.attn.scale, 0.0f, o.attn.window, nullptr, nullptr}, o.x, block_floats_, o.y, block_floats_,
+    return launch_attend_kv8(c, kv8_seqs(at, nt), Kv8Attn{o.attn.nh, o.attn.scale, 0.0f, o.attn.window, nullptr, nullptr, prefill_ ? 1 : 0}, o.x, block_floats_, o.y, block_floats_,
                              B2_F32, status_, st, pdl);
 }
 

@@ -77,10 +77,10 @@ class Setting:
                     sc = sc + slopes[h].double() * (j[None] - p[:, None])
                 sc = torch.where(see, sc, -math.inf)
                 w = torch.softmax(sc, -1)
-                y[self.first[s]:self.first[s + 1], h] = torch.where(see[:, :, None] & (w[:, :, None] == w[:, :, None]), w[:, :, None] * v[None, :, h // G], 0.0 * w[:, :, None].nan_to_num(0.0)).sum(1) \
-                    if n * t * self.hd < 4e6 and torch.isnan(v).any() else w @ v[:, h // G]
-                if torch.isnan(sc[see]).any():
-                    y[self.first[s]:self.first[s + 1], h][torch.isnan(torch.where(see, sc, 0.0)).any(1)] = math.nan
+                o = w @ v[:, h // G].nan_to_num(0.0)
+                lost = (torch.isnan(sc) | torch.isnan(v[:, h // G]).any(1)[None]) & see  # (what is not seen is nobody's)
+                o[lost.any(1)] = math.nan
+                y[self.first[s]:self.first[s + 1], h] = o
                 vmax = v[:, h // G].nan_to_num(0.0).abs().amax()
                 bias = slopes[h].abs().double() * n if slopes is not None else 0.0
                 d = vmax * (2.0 ** -18.5 * a + 2.0 ** -19 + cap * 2.0 ** -20 + bias * 2.0 ** -21 + (0.0 if few else 2.0 ** -11))

@@ -85,6 +85,10 @@ def test_steps_append_and_attend(backend, kind, nh, nkv, hd, interleaved, window
         for a, b in zip(plan.kv_read(0, 0, pos + t), kv):
             assert np.array_equal(a, b), (n, pos)
         want, tol = attend64(q, *kv, pos, window)
+        if kind == "prefill" and t * (nh // nkv) >= 64:
+            # many rows of a prefill step are multiplied as f16: each query value is off by 2^-11 of itself, so a score by 2^-11 of the magnitudes in it and a
+            # probability by twice that (and its own rounding, 2^-11), where the bound above has 2^-18.5 of them: 2^8.5 as much, and 2^-10 of the largest value
+            tol = tol * 2.0 ** 8.5 + 2.0 ** -10 * np.abs(kv[1]).max()
         assert (np.abs(got - want) <= tol).all(), (n, pos, np.abs(got - want).max())
         pos += t
     plan.close()
