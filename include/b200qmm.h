@@ -280,7 +280,10 @@ typedef struct b2_kv8_attention {
     uint32_t window;
     const float* slopes;   /* device [nh] or NULL */
     const int32_t* prefix; /* device [n_seqs] or NULL */
+    void* work;            /* device memory of b2_attend_kv8_work_bytes, 16-byte aligned, or NULL: with it the keys of few rows are shared out over all of the GPU.
+                              A call writes it before it reads it; calls that may run at the same time need memory of their own. */
 } b2_kv8_attention;
+size_t b2_attend_kv8_work_bytes(b2_ctx* ctx, b2_kv8 kv);
 int b2_attend_kv8_dev(b2_ctx* ctx, b2_kv8 kv, const b2_kv8_seqs* seqs, const b2_kv8_attention* attention, const void* q_dev, size_t q_stride, void* out_dev,
                       size_t out_stride, int dtype);
 

@@ -45,7 +45,8 @@ class Kv8Seqs(C.Structure):
 class Kv8Attention(C.Structure):
     """``b2_kv8_attention``."""
 
-    _fields_ = [("nh", C.c_uint32), ("scale", C.c_float), ("cap", C.c_float), ("window", C.c_uint32), ("slopes", C.c_void_p), ("prefix", C.c_void_p)]
+    _fields_ = [("nh", C.c_uint32), ("scale", C.c_float), ("cap", C.c_float), ("window", C.c_uint32), ("slopes", C.c_void_p), ("prefix", C.c_void_p),
+                ("work", C.c_void_p)]
 
 
 class LogitRules(C.Structure):
@@ -143,6 +144,7 @@ _SIGNATURES = {
     "b2_kv8_bytes": (C.c_size_t, [C.c_void_p, C.c_uint64]),
     "b2_kv8_append_dev": (C.c_int, [C.c_void_p, C.c_uint64, C.POINTER(Kv8Seqs), C.c_void_p, C.c_void_p, C.c_int, C.c_size_t, C.c_size_t]),
     "b2_kv8_read_dev": (C.c_int, [C.c_void_p, C.c_uint64, C.POINTER(Kv8Seqs), C.c_void_p, C.c_void_p]),
+    "b2_attend_kv8_work_bytes": (C.c_size_t, [C.c_void_p, C.c_uint64]),
     "b2_attend_kv8_dev": (C.c_int, [C.c_void_p, C.c_uint64, C.POINTER(Kv8Seqs), C.POINTER(Kv8Attention), C.c_void_p, C.c_size_t, C.c_void_p, C.c_size_t,
                                     C.c_int]),
     "b2_logits_dev": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_size_t, C.c_size_t, C.c_size_t, C.c_size_t, C.POINTER(LogitRules),

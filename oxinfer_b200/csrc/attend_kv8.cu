@@ -26,6 +26,9 @@ using namespace kv8;
 namespace {
 
 constexpr int AK_WARPS = 4, AK_THREADS = AK_WARPS * 32;
+constexpr uint32_t DEALT_CTAS = 3 * 148, DEALT_LEAST = 4;  // three an SM; blocks of a warp
+template <int HD>
+constexpr size_t DEALT_FLOAT4 = 8 * HD / 4 + 8;  // of a place: the sums of eight rows, their largest scores and denominators
 constexpr float P_BITS = 14.0f;  // probabilities are held 2^14 times as large: what is below 2^-28 of a row's largest loses bits, not before
 
 template <int HD, int TERMS>
@@ -52,6 +55,7 @@ struct AkArgs {
     const float* slopes;
     const int32_t* prefix;
     int aligned;
+    float4* work;  // dealt-out launches: sums of units of work that several CTAs share
     uint32_t* status;
 };
 
@@ -59,6 +63,12 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// The same from zero (no registers to clear first).
+__device__ __forceinline__ void mma16816_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
 }
 // Bytes q + 128 as f16: 1024 + byte by its bits, then minus 1152 (exact).
 __device__ __forceinline__ uint32_t two_halves(uint32_t w, uint32_t sel) {
@@ -82,12 +92,20 @@ __device__ __forceinline__ uint32_t pack_rest(float a, float b, uint32_t hi) {
     const float2 f = __half22float2(*(const __half2*)&hi);
     return pack(a - f.x, b - f.y);
 }
-// cap tanh(x / cap), x and the result in powers of two. Near zero by tanh's Taylor series (1 - 2 / (e^2z + 1) would lose bits there).
+// cap tanh(x / cap), x and the result in powers of two: up to |z| = 1 by an odd polynomial fitted at Chebyshev nodes of z^2 (off by 1.5e-7), beyond by an exponential.
 __device__ __forceinline__ float capped(float x, float cap2, float cap_in) {
     const float z = 0.5f * 0.69314718f * (x * cap_in), z2 = z * z;
-    const float series = z * fmaf(z2, fmaf(z2, fmaf(z2, fmaf(z2, 62.0f / 2835.0f, -17.0f / 315.0f), 2.0f / 15.0f), -1.0f / 3.0f), 1.0f);
-    const float far = 1.0f - __fdividef(2.0f, 1.0f + ex2(x * cap_in));
-    return cap2 * (fabsf(z) < 0.3f ? series : far);
+    float y = fmaf(z2, 1.04555360e-3f, -6.21706992e-3f);
+    y = fmaf(z2, y, 2.03055199e-2f);
+    y = fmaf(z2, y, -5.34651764e-2f);
+    y = fmaf(z2, y, 1.33253977e-1f);
+    y = fmaf(z2, y, -3.33328575e-1f);
+    y = z * fmaf(z2, y, 9.9999994e-1f);
+    if (!(fabsf(z) <= 1.0f)) {
+        const float far = 1.0f - __fdividef(2.0f, 1.0f + ex2(x * cap_in));
+        y = far;
+    }
+    return cap2 * y;
 }
 template <typename T>
 __device__ __forceinline__ void store4(T* p, float4 v, bool aligned) {
@@ -138,16 +156,83 @@ __device__ __forceinline__ void cluster_sync() {
 }
 __device__ __forceinline__ float weight_of(float m, float most) { return ex2(m - (most == -INFINITY ? 0.0f : most)); }
 
-// A CTA's grid index: (unit of work, CTA of the cluster); a unit: (sequence, tile of rows from the last on, KV head).
-template <int HD, int TERMS, typename T>
+// Dealt-out launches. The blocks of all units (tile of rows, KV head) of all sequences lie one behind another, and CTA i of n takes i W / n .. (i + 1) W / n
+// of them; a unit that several CTAs share leaves their sums in memory, two places a CTA (the unit it begins in the middle of, the one it ends in), and
+// a kernel behind this one adds them in order. Tiles of a sequence count the same blocks, those that any of its rows sees.
+struct Dealt {
+    uint32_t lo, blocks, tiles;  // a sequence's first block, blocks of a unit, tiles
+};
+template <int R>
+__device__ __forceinline__ Dealt dealt_of(const AkArgs& a, uint32_t s) {
+    Seq q;
+    if (s >= a.sq.n_seqs || !sequence(a.sq, s, &q, a.status) || q.count == 0) return Dealt{0, 0, 0};
+    const uint32_t lo = a.window && q.start + 1 > a.window ? (q.start + 1 - a.window) / KV8_BLOCK : 0;
+    return Dealt{lo, (q.start + q.count + KV8_BLOCK - 1) / KV8_BLOCK - lo, (q.count * a.G + R - 1) / R};
+}
+__device__ __forceinline__ unsigned long long dealt_weight(const AkArgs& a, const Dealt& d) { return (unsigned long long)d.tiles * a.c.nkv * d.blocks; }
+// The weights of all sequences ahead of s, and of all: every thread of the CTA calls this. red: two words a warp.
+template <int R>
+__device__ __forceinline__ void dealt_sums(const AkArgs& a, uint32_t s, unsigned long long* ahead, unsigned long long* all, unsigned long long* red) {
+    unsigned long long before = 0, sum = 0;
+    for (uint32_t x = threadIdx.x; x < a.sq.n_seqs; x += blockDim.x) {
+        const unsigned long long w = dealt_weight(a, dealt_of<R>(a, x));
+        sum += w;
+        if (x < s) before += w;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        before += __shfl_xor_sync(0xffffffffu, before, o);
+        sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    }
+    if ((threadIdx.x & 31) == 0) {
+        red[2 * (threadIdx.x >> 5)] = before;
+        red[2 * (threadIdx.x >> 5) + 1] = sum;
+    }
+    __syncthreads();
+    *ahead = *all = 0;
+    for (uint32_t i = 0; i < blockDim.x / 32; i++) {
+        *ahead += red[2 * i];
+        *all += red[2 * i + 1];
+    }
+    __syncthreads();
+}
+// The sequence that block `at` of all belongs to, and the weights ahead of it (one warp).
+template <int R>
+__device__ __forceinline__ uint32_t dealt_find(const AkArgs& a, unsigned long long at, unsigned long long* ahead) {
+    unsigned long long before = 0;
+    for (uint32_t s0 = 0; s0 < a.sq.n_seqs; s0 += 32) {
+        const unsigned long long w = dealt_weight(a, dealt_of<R>(a, s0 + (threadIdx.x & 31)));
+        unsigned long long upto = w;
+#pragma unroll
+        for (int o = 1; o < 32; o *= 2) {
+            const unsigned long long x = __shfl_up_sync(0xffffffffu, upto, o);
+            if ((int)(threadIdx.x & 31) >= o) upto += x;
+        }
+        const uint32_t hit = __ballot_sync(0xffffffffu, before + upto > at);
+        if (hit) {
+            const int i = __ffs(hit) - 1;
+            *ahead = before + __shfl_sync(0xffffffffu, upto - w, i);
+            return s0 + i;
+        }
+        before += __shfl_sync(0xffffffffu, upto, 31);
+    }
+    *ahead = before;
+    return a.sq.n_seqs;
+}
+// CTAs that get work: a warp has some blocks, at least
+__device__ __forceinline__ uint32_t dealt_ctas(unsigned long long all, uint32_t ctas) { return (uint32_t)min((unsigned long long)ctas, max(all / (DEALT_LEAST * AK_WARPS), 1ull)); }
+
+// A CTA's grid index: (unit of work, CTA of the cluster); a unit: (sequence, tile of rows from the last on, KV head). SPECIAL: a cap or a bias. DEALT: see above.
+template <int HD, int TERMS, typename T, bool SPECIAL, bool DEALT>
 __global__ void __launch_bounds__(AK_THREADS, TERMS == 2 ? 3 : 2) attend_kv8_kernel(const AkArgs a) {
     using L = AkShared<HD, TERMS>;
     constexpr int R = TERMS == 2 ? 8 : 16, RG = TERMS == 2 ? 1 : 2;  // rows of a tile; a lane's rows
     constexpr int KS = HD / 16, NT = HD / 8, QD = HD / 4, S = L::STAGES;
     extern __shared__ __align__(128) uint8_t smem[];
     pdl_launch_dependents();
-    const uint32_t C = cluster_size(), cta = cluster_rank();
-    const uint32_t work = blockIdx.x / C, head = work % a.c.nkv, rest = work / a.c.nkv, first_tile = a.tiles - 1 - rest % a.tiles, s = rest / a.tiles;
+    const uint32_t C = DEALT ? 1 : cluster_size(), cta = DEALT ? 0 : cluster_rank();
+    const uint32_t work = blockIdx.x / C, rest = work / a.c.nkv, first_tile = a.tiles - 1 - rest % a.tiles;
+    uint32_t head = work % a.c.nkv, s = rest / a.tiles;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     uint8_t* const ring = smem + warp * L::RING;
     uint64_t* const bars = (uint64_t*)(smem + L::BARS) + warp * S;
@@ -163,21 +248,58 @@ __global__ void __launch_bounds__(AK_THREADS, TERMS == 2 ? 3 : 2) attend_kv8_ker
     __syncwarp();
     pdl_wait();
     Seq seq;
-    if (!sequence(a.sq, s, &seq, a.status)) return;  // (the same in every CTA of the cluster)
-    const uint32_t rows = seq.count * a.G, len = seq.start + seq.count;
-    const uint32_t prefix = a.prefix ? (uint32_t)min(max(a.prefix[s], 0), (int)len) : 0;
+    uint32_t rows = 0, len = 0, prefix = 0;
+    auto take = [&](uint32_t x) {  // sequence x
+        if (!sequence(a.sq, x, &seq, a.status)) return false;
+        rows = seq.count * a.G;
+        len = seq.start + seq.count;
+        prefix = a.prefix ? (uint32_t)min(max(a.prefix[x], 0), (int)len) : 0;
+        return true;
+    };
+    unsigned long long at = 0, upto = 0, ahead = 0;  // DEALT: the blocks of this CTA, and the weights ahead of the sequence
+    Dealt d{};
+    if constexpr (DEALT) {
+        unsigned long long* const red = (unsigned long long*)wm;
+        unsigned long long all;
+        dealt_sums<R>(a, 0, &ahead, &all, red);
+        const uint32_t n = dealt_ctas(all, gridDim.x);
+        if (blockIdx.x >= n || all == 0) return;
+        at = all * blockIdx.x / n;
+        upto = all * (blockIdx.x + 1) / n;
+        s = dealt_find<R>(a, at, &ahead);
+        d = dealt_of<R>(a, s);
+        take(s);
+    } else {
+        if (!take(s)) return;  // (the same in every CTA of the cluster)
+    }
     const uint32_t NW = C * AK_WARPS, gw = cta * AK_WARPS + warp;
-    uint32_t slot = 0, phase = 0;
+    uint32_t slot = 0, phase = 0, tile = first_tile;
     bool ok = true;
 
-    for (uint32_t tile = first_tile; (size_t)tile * R < rows; tile += a.tiles) {
+    while (true) {
+        uint32_t off = 0, part_end = 0;  // DEALT: the blocks of the unit that this CTA takes
+        if constexpr (DEALT) {
+            if (at >= upto) break;
+            while (at >= ahead + dealt_weight(a, d)) {  // on to the next sequence that has rows
+                ahead += dealt_weight(a, d);
+                d = dealt_of<R>(a, ++s);
+                if (d.blocks) take(s);
+            }
+            const uint32_t unit = (uint32_t)((at - ahead) / d.blocks);
+            off = (uint32_t)((at - ahead) % d.blocks);
+            part_end = (uint32_t)min((unsigned long long)d.blocks, off + (upto - at));
+            tile = unit / a.c.nkv;
+            head = unit % a.c.nkv;
+        } else {
+            if ((size_t)tile * R >= rows) break;
+        }
         const uint32_t row0 = tile * R;
         const uint32_t p_first = seq.start + row0 / a.G, p_last = seq.start + min(row0 + R - 1, rows - 1) / a.G;
         const uint32_t k_end = max(p_last + 1, prefix);                                                // keys below are seen by some row
         const uint32_t k_lo = a.window && p_first + 1 > a.window ? p_first + 1 - a.window : 0;         // keys from here on
         const uint32_t in_lo = a.window && p_last + 1 > a.window ? p_last + 1 - a.window : 0;          // keys from here to in_end are seen by every row
         const uint32_t in_end = max(p_first + 1, prefix);
-        const uint32_t b_beg = k_lo / KV8_BLOCK, b_end = (k_end + KV8_BLOCK - 1) / KV8_BLOCK;
+        const uint32_t b_beg = DEALT ? d.lo + off : k_lo / KV8_BLOCK, b_end = DEALT ? d.lo + part_end : (k_end + KV8_BLOCK - 1) / KV8_BLOCK;
 
         // copies run ahead: block b_beg + gw + i NW is the warp's i-th
         const uint32_t n_mine = ok && b_end - b_beg > gw ? (b_end - b_beg - gw + NW - 1) / NW : 0;
@@ -207,7 +329,7 @@ __global__ void __launch_bounds__(AK_THREADS, TERMS == 2 ? 3 : 2) attend_kv8_ker
         for (int i = 0; i < RG; i++) {
             const uint32_t r = row0 + g + 8 * i, rc = min(r, rows - 1), tok = rc / a.G, h = head * a.G + rc % a.G;
             pos[i] = seq.start + tok;
-            slope[i] = a.slopes ? a.slopes[h] * 1.44269504f : 0.0f;
+            slope[i] = SPECIAL && a.slopes ? a.slopes[h] * 1.44269504f : 0.0f;
             const T* const src = (const T*)a.q + (size_t)(seq.r0 + tok) * a.q_stride + (size_t)h * HD + t * QD;
             float v[QD];
             float top = 0.0f;
@@ -265,12 +387,17 @@ __global__ void __launch_bounds__(AK_THREADS, TERMS == 2 ? 3 : 2) attend_kv8_ker
             float sc[RG][8];  // [row][key 2 t + e of tile j]: 2 j + e
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                float d0[4] = {0.f, 0.f, 0.f, 0.f}, d1[4] = {0.f, 0.f, 0.f, 0.f};
+                float d0[4], d1[4];
 #pragma unroll
                 for (int hf = 0; hf < KS / 4; hf++) {
                     const uint4 w = *(const uint4*)(unit + KV8_HEADER + j * (8 * HD) + hf * 512 + lane * 16);
-                    mma16816(d0, qa[4 * hf], low_half(w.x), high_half(w.x));
-                    mma16816(d1, qa[4 * hf + 1], low_half(w.y), high_half(w.y));
+                    if (hf == 0) {
+                        mma16816_first(d0, qa[0], low_half(w.x), high_half(w.x));
+                        mma16816_first(d1, qa[1], low_half(w.y), high_half(w.y));
+                    } else {
+                        mma16816(d0, qa[4 * hf], low_half(w.x), high_half(w.x));
+                        mma16816(d1, qa[4 * hf + 1], low_half(w.y), high_half(w.y));
+                    }
                     mma16816(d0, qa[4 * hf + 2], low_half(w.z), high_half(w.z));
                     mma16816(d1, qa[4 * hf + 3], low_half(w.w), high_half(w.w));
                 }
@@ -296,8 +423,8 @@ __global__ void __launch_bounds__(AK_THREADS, TERMS == 2 ? 3 : 2) attend_kv8_ker
                 for (int x = 0; x < 8; x++) {
                     const uint32_t key = key0 + 16 * (x >> 2) + 4 * t + (x & 3);
                     float y = sc[i][x] * f;
-                    if (a.cap2 > 0.0f) y = capped(y, a.cap2, a.cap_in);
-                    if (a.slopes) y = fmaf(slope[i], (float)(int)(key - pos[i]), y);
+                    if (SPECIAL && a.cap2 > 0.0f) y = capped(y, a.cap2, a.cap_in);
+                    if (SPECIAL) y = fmaf(slope[i], (float)(int)(key - pos[i]), y);
                     if (!whole) {
                         const bool see = key < len && (key <= pos[i] || key < prefix) && (a.window == 0 || (int)(pos[i] - key) < (int)a.window);
                         if ((bad >> (key - key0)) & 1) y = NAN;
@@ -347,9 +474,9 @@ __global__ void __launch_bounds__(AK_THREADS, TERMS == 2 ? 3 : 2) attend_kv8_ker
 #pragma unroll
             for (int n = 0; n < NT; n += 2) {
                 const uint4 w = *(const uint4*)(unit + KV8_HEADER + KV8_BLOCK * HD + n / 2 * 512 + lane * 16);
-                float d0[4] = {0.f, 0.f, 0.f, 0.f}, d1[4] = {0.f, 0.f, 0.f, 0.f};
-                mma16816(d0, pa[0], low_half(w.x), high_half(w.x));
-                mma16816(d1, pa[0], low_half(w.z), high_half(w.z));
+                float d0[4], d1[4];
+                mma16816_first(d0, pa[0], low_half(w.x), high_half(w.x));
+                mma16816_first(d1, pa[0], low_half(w.z), high_half(w.z));
                 mma16816(d0, pa[1], low_half(w.y), high_half(w.y));
                 mma16816(d1, pa[1], low_half(w.w), high_half(w.w));
 #pragma unroll
@@ -420,7 +547,11 @@ __global__ void __launch_bounds__(AK_THREADS, TERMS == 2 ? 3 : 2) attend_kv8_ker
                 v.x = fmaf(k, x.x, v.x), v.y = fmaf(k, x.y, v.y), v.z = fmaf(k, x.z, v.z), v.w = fmaf(k, x.w, v.w);
                 den = fmaf(k, wl[w * 16 + r], den);
             }
-            if (C == 1) {
+            if (DEALT && (off > 0 || part_end < d.blocks)) {
+                float4* const to = a.work + (size_t)(2 * blockIdx.x + (off > 0 ? 0 : 1)) * DEALT_FLOAT4<HD>;
+                to[item] = v;
+                if (item % (HD / 4) == 0) to[R * HD / 4 + r] = make_float4(M, den, 0.0f, 0.0f);
+            } else if (C == 1) {
                 finish(item, v, den);
             } else {
                 ((float4*)sum_s)[item] = v;
@@ -452,14 +583,82 @@ __global__ void __launch_bounds__(AK_THREADS, TERMS == 2 ? 3 : 2) attend_kv8_ker
         // the rings are free again: their copies are asynchronous writes behind these reads and writes
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncthreads();
+        if constexpr (DEALT) at += part_end - off;
+        else tile += a.tiles;
     }
 }
 
-template <int HD, int TERMS, typename T>
-cudaError_t attend_t(AkArgs& a, uint32_t units_per_tile, cudaStream_t st, bool pdl) {
+// Adds the sums of the units that several CTAs shared, `ctas` of them ahead of it. A thread has four outputs. Grid: (sequence, tile, KV head) and, ROW (few units,
+// shared by many CTAs), row of the tile: eight groups of threads take a place in turn then, and their sums are added in order.
+template <int HD, bool ROW, typename T>
+__global__ void __launch_bounds__(2 * HD) attend_kv8_join(const AkArgs a, uint32_t ctas) {
+    constexpr int R = 8, ITEMS = R * HD / 4, F4 = HD / 4, GROUPS = ROW ? 8 : 1;
+    __shared__ unsigned long long red[2 * 2 * HD / 32];
+    __shared__ float4 part[GROUPS][F4];
+    __shared__ float part_l[GROUPS], top[2 * HD / 32];
+    pdl_launch_dependents();
+    pdl_wait();
+    const uint32_t tid = threadIdx.x, f = tid % F4, grp = ROW ? tid / F4 : 0, r = ROW ? blockIdx.x % R : tid / F4, unit = ROW ? blockIdx.x / R : blockIdx.x;
+    const uint32_t head = unit % a.c.nkv, rest = unit / a.c.nkv, s = rest / a.tiles;
+    unsigned long long ahead, all;
+    dealt_sums<R>(a, s, &ahead, &all, red);
+    const Dealt d = dealt_of<R>(a, s);
+    Seq seq;
+    if (d.blocks == 0 || !sequence(a.sq, s, &seq, a.status)) return;
+    const uint32_t n = dealt_ctas(all, ctas), rows = seq.count * a.G;
+    for (uint32_t tile = rest % a.tiles; tile < d.tiles; tile += a.tiles) {
+        const uint32_t row = tile * R + r;
+        const unsigned long long from = ahead + ((unsigned long long)tile * a.c.nkv + head) * d.blocks, last = from + d.blocks - 1;
+        const uint32_t i0 = (uint32_t)(((from + 1) * n - 1) / all), i1 = (uint32_t)(((last + 1) * n - 1) / all);  // CTA i has all i / n .. all (i + 1) / n, rounded down
+        if (i0 == i1 || (ROW && row >= rows)) continue;
+        auto place = [&](uint32_t i) { return a.work + (size_t)(2 * i + (all * i / n > from ? 0 : 1)) * DEALT_FLOAT4<HD>; };
+        float M = -INFINITY;
+        if (ROW) {
+            for (uint32_t i = i0 + tid; i <= i1; i += 2 * HD) M = fmaxf(M, __ldcg(place(i) + ITEMS + r).x);
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+            if ((tid & 31) == 0) top[tid >> 5] = M;
+            __syncthreads();
+            for (int w = 0; w < 2 * HD / 32; w++) M = fmaxf(M, top[w]);
+        } else {
+            for (uint32_t i = i0; i <= i1; i++) M = fmaxf(M, __ldcg(place(i) + ITEMS + r).x);
+        }
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        float den = 0.0f;
+#pragma unroll 4
+        for (uint32_t i = i0 + grp; i <= i1; i += GROUPS) {
+            const float4 x = __ldcg(place(i) + r * F4 + f), ml = __ldcg(place(i) + ITEMS + r);
+            const float k = weight_of(ml.x, M);
+            v.x = fmaf(k, x.x, v.x), v.y = fmaf(k, x.y, v.y), v.z = fmaf(k, x.z, v.z), v.w = fmaf(k, x.w, v.w);
+            den = fmaf(k, ml.y, den);
+        }
+        if (ROW) {
+            part[grp][f] = v;
+            if (f == 0) part_l[grp] = den;
+            __syncthreads();
+        }
+        if (grp == 0 && row < rows) {
+            if (ROW) {
+#pragma unroll
+                for (int k = 1; k < GROUPS; k++) {
+                    const float4 x = part[k][f];
+                    v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
+                    den += part_l[k];
+                }
+            }
+            const float inv = den > 0.0f || den != den ? 1.0f / den : 0.0f;
+            T* const to = (T*)a.out + (size_t)(seq.r0 + row / a.G) * a.out_stride + (size_t)(head * a.G + row % a.G) * HD + f * 4;
+            store4<T>(to, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv), a.aligned);
+        }
+        if (ROW) __syncthreads();
+    }
+}
+
+template <int HD, int TERMS, bool SPECIAL, typename T>
+cudaError_t attend_p(AkArgs& a, uint32_t units_per_tile, cudaStream_t st, bool pdl) {
     using L = AkShared<HD, TERMS>;
     constexpr uint32_t R = TERMS == 2 ? 8 : 16;
-    auto kern = attend_kv8_kernel<HD, TERMS, T>;
+    auto kern = attend_kv8_kernel<HD, TERMS, T, SPECIAL, false>;
     const size_t rows = (size_t)a.sq.max_rows * a.G;
     size_t tiles = (rows + R - 1) / R;
     const size_t most = 0x7fffffffu / ((size_t)units_per_tile * 16);
@@ -471,6 +670,20 @@ cudaError_t attend_t(AkArgs& a, uint32_t units_per_tile, cudaStream_t st, bool p
     uint32_t C = 1;
     const size_t blocks = a.window && !a.prefix ? std::min<size_t>(a.sq.max_blocks, ((size_t)a.window + a.sq.max_rows) / KV8_BLOCK + 2) : a.sq.max_blocks;
     while (C < 16 && units * C * 2 <= (C == 8 ? 224 : 288) && blocks >= 2 * C * 2 * AK_WARPS) C *= 2;
+    if constexpr (TERMS == 2) {
+        // Dealt out where that saves a warp six blocks, one behind the other, of what it has otherwise (a launch more, and finding out what is whose, take as long; lengths
+        // that differ are put at a quarter off the longest). us, cluster / dealt: one token of 32 heads of 8 KV heads over 8192, 32768 and 131071 keys 15.3 / 18.6,
+        // 35.7 / 27.0, 121 / 56; 16 sequences of up to 2000 and 8000 keys 19 / 25, 57 / 40; 64 of up to 4096 75.6 / 70; 256 of up to 2000 127 / 145.
+        const double mine = std::max(1.0, (double)units * C / DEALT_CTAS) * blocks / (C * AK_WARPS), dealt_out = 0.75 * units * blocks / (DEALT_CTAS * AK_WARPS) + 6;
+        const char* e1 = getenv("AK_DEALT");
+        if (a.work && (e1 ? atoi(e1) : (units <= 2 * DEALT_CTAS && mine >= dealt_out))) {
+            auto dealt = attend_kv8_kernel<HD, TERMS, T, SPECIAL, true>;
+            if (cudaError_t e = ensure_dynamic_smem((const void*)dealt, L::BYTES, 0); e != cudaSuccess) return e;
+            if (cudaError_t e = launch_k(dealt, dim3(DEALT_CTAS), dim3(AK_THREADS), L::BYTES, st, pdl, a); e != cudaSuccess) return e;
+            if (units <= 64) return launch_k(attend_kv8_join<HD, true, T>, dim3((unsigned)units * 8), dim3(2 * HD), 0, st, true, a, DEALT_CTAS);
+            return launch_k(attend_kv8_join<HD, false, T>, dim3((unsigned)units), dim3(2 * HD), 0, st, true, a, DEALT_CTAS);
+        }
+    }
     if (cudaError_t e = ensure_dynamic_smem((const void*)kern, L::BYTES, 0); e != cudaSuccess) return e;
     if (cudaError_t e = cudaFuncSetAttribute((const void*)kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1); e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
@@ -489,6 +702,10 @@ cudaError_t attend_t(AkArgs& a, uint32_t units_per_tile, cudaStream_t st, bool p
     cfg.numAttrs = pdl ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, kern, a);
 }
+template <int HD, int TERMS, typename T>
+cudaError_t attend_t(AkArgs& a, uint32_t units_per_tile, cudaStream_t st, bool pdl) {
+    return a.cap2 > 0.0f || a.slopes ? attend_p<HD, TERMS, true, T>(a, units_per_tile, st, pdl) : attend_p<HD, TERMS, false, T>(a, units_per_tile, st, pdl);
+}
 template <int HD>
 cudaError_t attend_hd(AkArgs& a, int dtype, uint32_t units_per_tile, cudaStream_t st, bool pdl) {
     const bool few = (size_t)a.sq.max_rows * a.G <= 8;
@@ -501,6 +718,8 @@ cudaError_t attend_hd(AkArgs& a, int dtype, uint32_t units_per_tile, cudaStream_
 }
 
 }  // namespace
+
+size_t attend_kv8_work_bytes(uint32_t hd) { return (size_t)DEALT_CTAS * 2 * (hd == 64 ? DEALT_FLOAT4<64> : DEALT_FLOAT4<128>) * 16; }
 
 cudaError_t launch_attend_kv8(const Kv8Cache& c, const Kv8Seqs& s, const Kv8Attn& p, const void* q, size_t q_stride, void* out, size_t out_stride, int dtype,
                               uint32_t* status, cudaStream_t st, bool pdl) {
@@ -525,6 +744,7 @@ cudaError_t launch_attend_kv8(const Kv8Cache& c, const Kv8Seqs& s, const Kv8Attn
     a.slopes = p.slopes;
     a.prefix = p.prefix;
     a.status = status;
+    a.work = (float4*)p.work;
     const size_t esz = dtype == B2_F32 ? 4 : 2, unit = 4 * esz;
     a.aligned = (((uintptr_t)q | (uintptr_t)out | q_stride * esz | out_stride * esz) & (unit - 1)) == 0;
     const size_t per_tile = (size_t)s.n_seqs * c.nkv;

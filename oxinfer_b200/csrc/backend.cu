@@ -1603,9 +1603,10 @@ class Backend {
         if (!std::isfinite(a->scale) || !std::isfinite(a->cap) || a->cap < 0.0f) return fail(B2_ERR_ARG, "[b200qmm: attend_kv8: the scale and the cap are finite, the cap not negative]");
         if (s.n_seqs == 0 || s.n_rows == 0) return B2_OK;
         if (!q || !out) return fail(B2_ERR_ARG, "[b200qmm: attend_kv8: null argument]");
+        if ((uintptr_t)a->work & 15) return fail(B2_ERR_ARG, "[b200qmm: attend_kv8: the work memory is not aligned to 16 bytes]");
         if (s.n_rows > 1 && out_stride < (size_t)a->nh * p->dev.hd) return fail(B2_ERR_ARG, "[b200qmm: attend_kv8: rows of the result overlap]");
         if ((uint64_t)s.n_rows * (a->nh / p->dev.nkv) > 0x7fffffffu) return fail(B2_DECLINED, "[b200qmm: attend_kv8: too many rows for one call]");
-        cudaError_t e = launch_attend_kv8(p->dev, s, Kv8Attn{a->nh, a->scale, a->cap, a->window, a->slopes, a->prefix}, q, q_stride, out, out_stride, dtype, list_status(), stream);
+        cudaError_t e = launch_attend_kv8(p->dev, s, Kv8Attn{a->nh, a->scale, a->cap, a->window, a->slopes, a->prefix, 0, a->work}, q, q_stride, out, out_stride, dtype, list_status(), stream);
         launches++;
         return e == cudaSuccess ? B2_OK : cuda_fail(e, "attend_kv8");
     }
@@ -2026,6 +2027,13 @@ B2_EXPORT int b2_kv8_append_dev(b2_ctx* ctx, b2_kv8 kv, const b2_kv8_seqs* seqs,
 B2_EXPORT int b2_kv8_read_dev(b2_ctx* ctx, b2_kv8 kv, const b2_kv8_seqs* seqs, float* k_dev, float* v_dev) {
     LOCKED(ctx);
     return ctx->be.kv8_read(kv, seqs, k_dev, v_dev);
+}
+
+B2_EXPORT size_t b2_attend_kv8_work_bytes(b2_ctx* ctx, b2_kv8 kv) {
+    if (!ctx) return 0;
+    std::lock_guard<std::mutex> lock(ctx->be.mu);
+    b2::Kv8Pool* p = ctx->be.find_kv8(kv);
+    return p ? b2::attend_kv8_work_bytes(p->dev.hd) : 0;
 }
 
 B2_EXPORT int b2_attend_kv8_dev(b2_ctx* ctx, b2_kv8 kv, const b2_kv8_seqs* seqs, const b2_kv8_attention* attention, const void* q_dev, size_t q_stride,

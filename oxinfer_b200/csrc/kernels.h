@@ -325,7 +325,9 @@ struct Kv8Attn {
     const float* slopes;    // [nh] or null
     const int32_t* prefix;  // [n_seqs] or null
     int halves = 0;         // f32 rows may be multiplied as f16
+    void* work = nullptr;   // attend_kv8_work_bytes of memory that one launch at a time uses, or null: work is then shared out within clusters only
 };
+size_t attend_kv8_work_bytes(uint32_t hd);
 // Row i of a sequence is a query at start + i, and sees the sequence's keys up to its own position and below the prefix, the last `window` of them.
 // attend_kv8_rows.cu: f16 operands, 256 rows a CTA.
 cudaError_t launch_attend_kv8_rows(const Kv8Cache& c, const Kv8Seqs& s, const Kv8Attn& p, const void* q, size_t q_stride, void* out, size_t out_stride, int dtype,

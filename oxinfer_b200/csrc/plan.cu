@@ -128,7 +128,7 @@ DecodePlanImpl::~DecodePlanImpl() {
     for (void* m : peer_maps_) cudaIpcCloseMemHandle(m);
     for (auto& kv : gemm_plans_)
         for (GemmPlan* gp : kv.second) gemm_tc_plan_destroy(gp);
-    void* frees[] = {kv8_rows_, gen_rules_.room, gen_rules_.words, kv16_, x16_, unscale_, tmp_a_, tmp_b_, gemm_status_, xflags_, bufs_, records_, consts_, att_scratch_.part, words_, rope_table_, argmax_val_, argmax_idx_, token_, out_tokens_, stage_};
+    void* frees[] = {kv8_work_, kv8_rows_, gen_rules_.room, gen_rules_.words, kv16_, x16_, unscale_, tmp_a_, tmp_b_, gemm_status_, xflags_, bufs_, records_, consts_, att_scratch_.part, words_, rope_table_, argmax_val_, argmax_idx_, token_, out_tokens_, stage_};
     for (void* p : frees)
         if (p) cudaFree(p);
 }
@@ -240,6 +240,7 @@ int DecodePlanImpl::create(const b2_graph* g, const std::function<const WeightDe
     if (p->kv8_) {
         p->kv8_row_floats_ = T * std::max<size_t>(max_row, 64);
         PLAN_CUDA(cudaMalloc((void**)&p->kv8_rows_, 2 * p->kv8_row_floats_ * sizeof(float)), "cudaMalloc(rows of a step)");
+        PLAN_CUDA(cudaMalloc(&p->kv8_work_, attend_kv8_work_bytes(128)), "cudaMalloc(attention sums)");
     }
 
     // ---- norm weights: one device block -----------------------------------------------------------
@@ -751,7 +752,7 @@ cudaError_t DecodePlanImpl::rope_kv8(const Op& o, const uint32_t* at, uint32_t n
 }
 cudaError_t DecodePlanImpl::attend_kv8(const Op& o, const uint32_t* at, uint32_t nt, cudaStream_t st, bool pdl) {
     const Kv8Cache c{(uint8_t*)kv_[o.kv].k, o.attn.nkv, o.attn.hd, (max_len_ + KV8_BLOCK - 1) / KV8_BLOCK};
-    return launch_attend_kv8(c, kv8_seqs(at, nt), Kv8Attn{o.attn.nh, o.attn.scale, 0.0f, o.attn.window, nullptr, nullptr, prefill_ ? 1 : 0}, o.x, block_floats_, o.y, block_floats_,
+    return launch_attend_kv8(c, kv8_seqs(at, nt), Kv8Attn{o.attn.nh, o.attn.scale, 0.0f, o.attn.window, nullptr, nullptr, prefill_ ? 1 : 0, kv8_work_}, o.x, block_floats_, o.y, block_floats_,
                              B2_F32, status_, st, pdl);
 }
 

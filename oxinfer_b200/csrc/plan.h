@@ -139,6 +139,7 @@ class DecodePlanImpl {
     bool kv8_ = false;            // 8-bit caches: Kv::k holds the units of kv8.cuh, v is null
     float* kv8_rows_ = nullptr;   // [2][largest nkv hd][tokens]: a step's rotated keys and its values on their way into one
     size_t kv8_row_floats_ = 0;   // of one of the two
+    void* kv8_work_ = nullptr;    // of the attention over them
     uint32_t* kv8_at_ = nullptr;  // a word of words_: kv_write's and kv_read's first position
     AttScratch att_scratch_;      // (the counts are words)
     uint32_t* words_ = nullptr;   // sp[4] | status | argmax counter | - | - | sp[4] of each token of a step | attention counts

@@ -47,6 +47,7 @@ class Kv8Cache:
 
         self.backend, self.handle, self.nkv, self.hd, self.n_blocks = backend, handle, nkv, hd, n_blocks
         self.device = torch.device("cuda", backend.ordinal)
+        self._work_bytes = _lib.lib().b2_attend_kv8_work_bytes(backend._ctx, handle)
 
     def bytes(self) -> int:
         return _lib.lib().b2_kv8_bytes(self.backend._ctx, self.handle)
@@ -97,6 +98,9 @@ class Kv8Cache:
             assert x.stride(2) == 1 and x.stride(1) == self.hd
         assert slopes is None or (slopes.dtype == torch.float32 and slopes.numel() == nh and slopes.is_contiguous() and slopes.device == self.device)
         assert prefix is None or (prefix.dtype == torch.int32 and prefix.numel() == s.n_seqs and prefix.is_contiguous() and prefix.device == self.device)
-        a = _lib.Kv8Attention(nh, scale, cap, window or 0, slopes.data_ptr() if slopes is not None else None, prefix.data_ptr() if prefix is not None else None)
+        # (memory of the call's own, from torch's allocator: calls on other streams and captured ones have theirs)
+        work = torch.empty(self._work_bytes, dtype=torch.uint8, device=self.device) if q.dtype == torch.float32 or s.max_rows * (nh // self.nkv) <= 8 else None
+        a = _lib.Kv8Attention(nh, scale, cap, window or 0, slopes.data_ptr() if slopes is not None else None, prefix.data_ptr() if prefix is not None else None,
+                              work.data_ptr() if work is not None else None)
         return self.backend._check(self.backend._L.b2_attend_kv8_dev(self.backend._ctx, self.handle, C.byref(s), C.byref(a), q.data_ptr(), q.stride(0),
                                                                      out.data_ptr(), out.stride(0), _dtype_code(q)))

@@ -268,7 +268,7 @@ def test_refusals(backend):
     with pytest.raises(ob.BackendError):
         s.cache.attend(s.seqs, s.q[:, :3], out[:, :3], scale=1.0)  # three heads over two
     L, cs = ob.lib(), s.seqs.c(s.q.device)
-    a = ob._lib.Kv8Attention(4, 1.0, 0.0, 0, None, None)
+    a = ob._lib.Kv8Attention(4, 1.0, 0.0, 0, None, None, None)
     args = lambda **k: [backend._ctx, s.cache.handle, C.byref(cs), C.byref(a), s.q.data_ptr(), 256, out.data_ptr(), 256, 0]
     for i, bad in ((1, 1 << 40), (2, None), (3, None), (4, None), (6, None), (8, 7)):
         x = args()
