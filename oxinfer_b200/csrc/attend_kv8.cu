@@ -135,9 +135,9 @@ __device__ __forceinline__ float4 peer_f4(const void* p, uint32_t cta) {
     asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(peer(p, cta)) : "memory");
     return v;
 }
-__device__ __forceinline__ float peer_f(const void* p, uint32_t cta) {
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(peer(p, cta)) : "memory");
+__device__ __forceinline__ float2 peer_f2(const void* p, uint32_t cta) {
+    float2 v;
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(peer(p, cta)) : "memory");
     return v;
 }
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -237,9 +237,8 @@ __global__ void __launch_bounds__(AK_THREADS, TERMS == 2 ? 3 : 2) attend_kv8_ker
     uint8_t* const ring = smem + warp * L::RING;
     uint64_t* const bars = (uint64_t*)(smem + L::BARS) + warp * S;
     float* const sum_s = (float*)smem;  // the CTA's sums, where the first warp's were
-    float* const m_s = (float*)(smem + L::ML);
-    float* const l_s = m_s + 16;
-    float* const wm = l_s + 16;                 // [warp][16]
+    float2* const ml_s = (float2*)(smem + L::ML);  // the CTA's largest scores and denominators
+    float* const wm = (float*)(ml_s + 16);         // [warp][16]
     float* const wl = wm + AK_WARPS * 16;
     if (lane == 0) {
         for (int i = 0; i < S; i++) bar_init(&bars[i], 1);
@@ -555,24 +554,41 @@ __global__ void __launch_bounds__(AK_THREADS, TERMS == 2 ? 3 : 2) attend_kv8_ker
                 finish(item, v, den);
             } else {
                 ((float4*)sum_s)[item] = v;
-                if (item % (HD / 4) == 0) {
-                    m_s[r] = M;
-                    l_s[r] = den;
-                }
+                if (item % (HD / 4) == 0) ml_s[r] = make_float2(M, den);
             }
         }
         if (C > 1) {
             cluster_sync();
             for (int item = (int)cta * AK_THREADS + tid; item < ITEMS; item += (int)C * AK_THREADS) {
                 const int r = item / (HD / 4);
+                // (eight CTAs' words in flight at once)
                 float M = -INFINITY, den = 0.0f;
-                for (uint32_t k = 0; k < C; k++) M = fmaxf(M, peer_f(m_s + r, k));
                 float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-                for (uint32_t k = 0; k < C; k++) {
-                    const float w = weight_of(peer_f(m_s + r, k), M);
-                    const float4 x = peer_f4((const float4*)sum_s + item, k);
-                    v.x = fmaf(w, x.x, v.x), v.y = fmaf(w, x.y, v.y), v.z = fmaf(w, x.z, v.z), v.w = fmaf(w, x.w, v.w);
-                    den = fmaf(w, peer_f(l_s + r, k), den);
+                for (uint32_t k0 = 0; k0 < C; k0 += 8) {
+                    float2 ml[8];
+                    float4 x[8];
+#pragma unroll
+                    for (uint32_t k = 0; k < 8; k++) {
+                        ml[k] = make_float2(-INFINITY, 0.0f);
+                        x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+                        if (k0 + k < C) {
+                            ml[k] = peer_f2(ml_s + r, k0 + k);
+                            x[k] = peer_f4((const float4*)sum_s + item, k0 + k);
+                        }
+                    }
+                    float m = M;
+#pragma unroll
+                    for (int k = 0; k < 8; k++) m = fmaxf(m, ml[k].x);
+                    const float keep = weight_of(M, m);
+                    v = make_float4(v.x * keep, v.y * keep, v.z * keep, v.w * keep);
+                    den *= keep;
+                    M = m;
+#pragma unroll
+                    for (int k = 0; k < 8; k++) {
+                        const float w = weight_of(ml[k].x, M);
+                        v.x = fmaf(w, x[k].x, v.x), v.y = fmaf(w, x[k].y, v.y), v.z = fmaf(w, x[k].z, v.z), v.w = fmaf(w, x[k].w, v.w);
+                        den = fmaf(w, ml[k].y, den);
+                    }
                 }
                 finish(item, v, den);
             }
