@@ -6,6 +6,7 @@
 // A row with a value that is not finite is marked, and counts as NaN: it does not enter the scale, and the block's other rows are as they would be without it.
 #include "kv8.cuh"
 
+#include <algorithm>
 #include <cfloat>
 
 #include "pdl.cuh"
@@ -16,6 +17,7 @@ using namespace kv8;
 
 namespace {
 
+constexpr size_t KV_WAVE = 8;  // CTAs an SM of a launch over many blocks
 constexpr int KV_THREADS = 256;  // eight threads a token: thread i has dimensions 4 i .. 4 i + 3 and every 32nd behind them
 
 // e of the largest magnitude: mantissas up to 127 / 64 fit 127 * 2^(exponent - 6).
@@ -27,126 +29,218 @@ __device__ __forceinline__ int scale_exponent(float amax) {
 // `most`: 127, but 63 at the largest scale, 2^122, where 64 would no longer be a finite value.
 __device__ __forceinline__ uint32_t to_byte(float q, float most) { return (uint32_t)((int)fminf(fmaxf(rintf(q), -most), most) + 128); }
 
+// Sixteen bytes of a unit's keys or values, from byte `at` on: those of tokens that stay, times `shrink`, rounded.
+template <int HD>
+__device__ __forceinline__ uint4 requantized(uint4 w, uint32_t at, uint32_t kind, uint32_t staying, float shrink, float most) {
+    uint32_t x[4] = {w.x, w.y, w.z, w.w};
+    const uint32_t lane = (at & 511) >> 4, n = lane >> 2, j = at / (8 * HD);
+    const uint32_t token = 16 * (j >> 1) + 4 * (n >> 1) + 2 * (j & 1) + (n & 1);  // of all sixteen keys
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        uint32_t y = 0;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const uint32_t q = (x[i] >> (8 * e)) & 0xffu, tok = kind ? 16 * (i & 1) + 4 * (lane & 3) + e : token;
+            y |= ((staying >> tok) & 1 ? to_byte((float)((int)q - 128) * shrink, most) : q) << (8 * e);
+        }
+        x[i] = y;
+    }
+    return make_uint4(x[0], x[1], x[2], x[3]);
+}
+// The rows lo .. hi - 1 of a block that are written, and those that stay.
+__device__ __forceinline__ uint32_t rows_between(int lo, int hi) { return (uint32_t)((((1ull << hi) - 1) >> lo) << lo); }
+__device__ __forceinline__ uint32_t rows_staying(int lo, int hi, int keep_behind) { return ~rows_between(lo, hi) & (keep_behind ? 0xffffffffu : rows_between(0, lo)); }
+
+// Grid: (sequence, block of the rows', KV head, keys or values), a CTA each: the block's image in shared memory, then out of it 16 bytes a thread.
 template <int HD, typename T>
-__global__ void __launch_bounds__(KV_THREADS) append_kernel(Kv8Cache c, Kv8Seqs sq, Kv8Rows x, uint32_t tiles, int keep_behind, int aligned, uint32_t* status) {
-    constexpr int C = HD / 32, UNIT = (int)unit_bytes(HD);
-    __shared__ __align__(16) uint8_t image[2 * KV8_BLOCK * HD];
-    __shared__ float warp_max[2][KV_THREADS / 32];
-    __shared__ uint32_t warp_bad[2][KV_THREADS / 32];
+__global__ void __launch_bounds__(KV_THREADS, 4) append_kernel(Kv8Cache c, Kv8Seqs sq, Kv8Rows x, uint32_t tiles, int keep_behind, int aligned, uint32_t* status) {
+    constexpr int C = HD / 32, UNIT = (int)unit_bytes(HD), WARPS = KV_THREADS / 32, WORDS = (int)KV8_BLOCK * HD / 16;
+    __shared__ __align__(16) uint8_t image[KV8_BLOCK * HD];
+    __shared__ float warp_max[WARPS];
+    __shared__ uint32_t warp_bad[WARPS];
     pdl_launch_dependents();
     const int tid = threadIdx.x, r = tid >> 3, i4 = (tid & 7) * 4, warp = tid >> 5, lane = tid & 31;
-    const uint32_t head = blockIdx.x % c.nkv, rest = blockIdx.x / c.nkv, tile = rest % tiles, s = rest / tiles;
+    const uint32_t kind = blockIdx.x & 1, head = (blockIdx.x >> 1) % c.nkv, rest = (blockIdx.x >> 1) / c.nkv, tile = rest % tiles, s = rest / tiles;
     pdl_wait();
     Seq seq;
     if (!sequence(sq, s, &seq, status) || seq.count == 0) return;
     const uint32_t end = seq.start + seq.count, b_end = (end - 1) / KV8_BLOCK + 1;
-    for (uint32_t b = seq.start / KV8_BLOCK + tile; b < b_end; b += tiles) {
-        const int id = block_of(c, sq, s, b, status);
-        if (id < 0) continue;
-        uint8_t* const unit = c.units + ((size_t)id * c.nkv + head) * UNIT;
+    uint32_t b = seq.start / KV8_BLOCK + tile;
+    if (b >= b_end) return;
+    const T* const from = (const T*)(kind ? x.v : x.k) + (size_t)head * x.hs + i4;
+    auto rows_of = [&](uint32_t b, int* lo, int* hi) {
         const int base = (int)(b * KV8_BLOCK);  // (positions are below 2^31)
-        const int lo = max((int)seq.start - base, 0), hi = min((int)end - base, (int)KV8_BLOCK);
-        const bool kept = lo > 0 || (keep_behind && hi < (int)KV8_BLOCK), is_new = r >= lo && r < hi, stays = !is_new && (r < lo || keep_behind);
-        Header old = *(const Header*)unit;
-        float v[2][C][4];
-        float top[2] = {0.0f, 0.0f};
-        bool fine[2] = {true, true};
+        *lo = max((int)seq.start - base, 0);
+        *hi = min((int)end - base, (int)KV8_BLOCK);
+    };
+    float v[C][4];
+    int id;
+    auto fetch = [&](uint32_t b) {  // a block's rows and its place
+        int lo, hi;
+        rows_of(b, &lo, &hi);
+        const bool is_new = r >= lo && r < hi;
+        const T* const row = from + (size_t)(is_new ? seq.r0 + b * KV8_BLOCK + (uint32_t)r - seq.start : 0u) * x.rs;
 #pragma unroll
-        for (int kind = 0; kind < 2; kind++) {
-            const T* const row = (const T*)(kind ? x.v : x.k) + (size_t)(is_new ? seq.r0 + (uint32_t)(base + r) - seq.start : 0u) * x.rs + (size_t)head * x.hs;
+        for (int j = 0; j < C; j++) {
+            if (is_new) {
+                load4(v[j], row + 32 * j, aligned);
+            } else {
 #pragma unroll
-            for (int j = 0; j < C; j++) {
-                if (is_new) {
-                    load4(v[kind][j], row + i4 + 32 * j, aligned);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 4; e++) v[kind][j][e] = 0.0f;
-                }
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const float a = fabsf(v[kind][j][e]);
-                    fine[kind] = fine[kind] && a <= FLT_MAX;
-                    top[kind] = fmaxf(top[kind], a);
-                }
+                for (int e = 0; e < 4; e++) v[j][e] = 0.0f;
             }
         }
+        id = block_of(c, sq, s, b, status);
+    };
+    fetch(b);
+    for (; b < b_end; b += tiles) {
+        int lo, hi;
+        rows_of(b, &lo, &hi);
+        const bool is_new = r >= lo && r < hi;
+        const uint32_t staying = rows_staying(lo, hi, keep_behind);
+        if (id < 0) {
+            if (b + tiles < b_end) fetch(b + tiles);
+            continue;
+        }
+        uint8_t* const unit = c.units + ((size_t)id * c.nkv + head) * UNIT;
+        uint2* const header = (uint2*)unit + kind;  // the kind's scale and tokens that are not finite
+        uint8_t* const bytes = unit + KV8_HEADER + kind * (KV8_BLOCK * HD);
+        uint2 old = make_uint2(0, 0);
+        if (staying) old = *header;
+        uint32_t top = 0;  // of the magnitudes, by their bits (infinities and NaN above all others)
 #pragma unroll
-        for (int kind = 0; kind < 2; kind++) {
-            const uint32_t odd = __ballot_sync(0xffffffffu, !fine[kind]);  // a byte for each of the warp's four rows
+        for (int j = 0; j < C; j++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) top = max(top, __float_as_uint(v[j][e]) & 0x7fffffffu);
+        bool fine = top < 0x7f800000u;
+        {
+            const uint32_t odd = __ballot_sync(0xffffffffu, !fine);  // a byte for each of the warp's four rows
             uint32_t bad = 0;
 #pragma unroll
             for (int w = 0; w < 4; w++) bad |= ((odd >> (8 * w)) & 0xffu) ? 1u << w : 0u;
-            fine[kind] = !((bad >> (lane >> 3)) & 1u);
-            float m = fine[kind] ? top[kind] : 0.0f;
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+            fine = !((bad >> (lane >> 3)) & 1u);
+            const uint32_t m = __reduce_max_sync(0xffffffffu, fine ? top : 0u);
             if (lane == 0) {
-                warp_max[kind][warp] = m;
-                warp_bad[kind][warp] = bad << (4 * warp);
+                warp_max[warp] = __uint_as_float(m);
+                warp_bad[warp] = bad << (4 * warp);
             }
         }
         __syncthreads();  // (the old header has been read by everyone, too)
-        const uint32_t staying = ~(uint32_t)((((1ull << hi) - 1) >> lo) << lo) & (keep_behind ? 0xffffffffu : (uint32_t)((1ull << lo) - 1));
-        float scale[2], shrink[2];
-        uint32_t bad_bits[2];
-        bool grows = false;
+        float m = 0.0f;
+        uint32_t bad = old.y & staying;
 #pragma unroll
-        for (int kind = 0; kind < 2; kind++) {
-            float m = 0.0f;
-            uint32_t bad = kept ? (kind ? old.v_bad : old.k_bad) & staying : 0u;
-#pragma unroll
-            for (int w = 0; w < KV_THREADS / 32; w++) {
-                m = fmaxf(m, warp_max[kind][w]);
-                bad |= warp_bad[kind][w];
-            }
-            bad_bits[kind] = bad;
-            const float was = kept ? (kind ? old.v_scale : old.k_scale) : 0.0f;
-            scale[kind] = fmaxf(pow2(scale_exponent(m)), was);
-            shrink[kind] = was / scale[kind];  // (a power of two, 0 where nothing was written yet)
-            grows = grows || (kept && was < scale[kind]);
+        for (int w = 0; w < WARPS; w++) {
+            m = fmaxf(m, warp_max[w]);
+            bad |= warp_bad[w];
         }
-        // Whole blocks and those whose rows change leave as one image, 16 bytes a thread; a few rows (a decoding step) byte by byte, in place.
-        const bool whole = grows || hi - lo >= 8;
-        if (whole && kept) {
-            for (int o = tid; o < (int)(2 * KV8_BLOCK * HD / 16); o += KV_THREADS) ((uint4*)image)[o] = ((const uint4*)(unit + KV8_HEADER))[o];
+        const float was = __uint_as_float(old.x), scale = fmaxf(pow2(scale_exponent(m)), was);
+        const float inv = 1.0f / scale, most = inv == 0x1p-122f ? 63.0f : 127.0f;  // (powers of two)
+        if (hi - lo < (int)KV8_BLOCK) {  // what the image has of other rows
+            const float shrink = was * inv;
+            for (int o = tid; o < WORDS; o += KV_THREADS) {
+                uint4 w = make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
+                if (staying) {
+                    w = ((const uint4*)bytes)[o];
+                    if (was < scale) w = requantized<HD>(w, 16 * o, kind, staying, shrink, most);
+                }
+                ((uint4*)image)[o] = w;
+            }
             __syncthreads();
         }
-        if (whole || is_new) {
-            uint8_t* const to = whole ? image : unit + KV8_HEADER;
+        uint32_t w[C];
 #pragma unroll
-            for (int kind = 0; kind < 2; kind++) {
-                const float inv = 1.0f / scale[kind], most = inv == 0x1p-122f ? 63.0f : 127.0f;
+        for (int j = 0; j < C; j++) {
+            if (!fine) {
+                w[j] = 0x80808080u;
+            } else if (most == 127.0f) {  // a sum with 1.5 * 2^23 is rounded to a whole number, to even, and its last byte is the byte
+                uint32_t q[4];
 #pragma unroll
-                for (int j = 0; j < C; j++) {
-                    const uint32_t d = i4 + 32 * j;
-                    uint32_t q[4];
-                    if (is_new) {
+                for (int e = 0; e < 4; e++) q[e] = __float_as_uint(fmaf(v[j][e], inv, 12582912.0f + 128.0f));
+                w[j] = __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
+            } else {
+                w[j] = 0;
 #pragma unroll
-                        for (int e = 0; e < 4; e++) q[e] = fine[kind] ? to_byte(v[kind][j][e] * inv, most) : 128u;
-                    } else if (stays && kept) {
-#pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            const uint32_t at = kind ? KV8_BLOCK * HD + value_at(r, d + e) : key_at<HD>(r, d) + e;
-                            q[e] = to_byte((float)((int)image[at] - 128) * shrink[kind], most);
-                        }
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 4; e++) q[e] = 128u;
-                    }
-                    if (kind == 0) {
-                        *(uint32_t*)(to + key_at<HD>(r, d)) = q[0] | q[1] << 8 | q[2] << 16 | q[3] << 24;
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 4; e++) to[KV8_BLOCK * HD + value_at(r, d + e)] = (uint8_t)q[e];
-                    }
-                }
+                for (int e = 0; e < 4; e++) w[j] |= to_byte(v[j][e] * inv, most) << (8 * e);
             }
         }
-        if (tid == 0) *(Header*)unit = Header{scale[0], bad_bits[0], scale[1], bad_bits[1], {0, 0, 0, 0}};
+        if (b + tiles < b_end) fetch(b + tiles);  // (under this block's way out)
+        const uint32_t b0 = (lane >> 3) & 1, b1 = lane >> 4, quad = (rows_between(lo, hi) >> (4 * warp)) & 0xfu;  // the warp's four tokens
+        const uint32_t keep = ~(((quad & 1) | (quad & 2) << 7 | (quad & 4) << 14 | (quad & 8) << 21) * 0xffu);
+#pragma unroll
+        for (int j = 0; j < C; j++) {
+            if (kind == 0) {
+                if (is_new) *(uint32_t*)(image + key_at<HD>(r, i4 + 32 * j)) = w[j];
+            } else if (quad) {  // four dimensions of a token to four tokens of a dimension, over the lanes of the four tokens
+                const uint32_t p = __shfl_xor_sync(0xffffffffu, w[j], 8), z = __byte_perm(w[j], p, b0 ? 0x3715 : 0x6240);
+                const uint32_t p2 = __shfl_xor_sync(0xffffffffu, z, 16), y = __byte_perm(z, p2, b1 ? 0x3276 : 0x5410);
+                uint32_t* const to = (uint32_t*)(image + value_at(4 * warp, i4 + 32 * j + 2 * b1 + b0));
+                *to = keep ? (*to & keep) | (y & ~keep) : y;
+            }
+        }
+        if (tid == 0) *header = make_uint2(__float_as_uint(scale), bad);
         __syncthreads();
-        if (whole)
-            for (int o = tid; o < (int)(2 * KV8_BLOCK * HD / 16); o += KV_THREADS) ((uint4*)(unit + KV8_HEADER))[o] = ((const uint4*)image)[o];
+        for (int o = tid; o < WORDS; o += KV_THREADS) ((uint4*)bytes)[o] = ((const uint4*)image)[o];
         __syncthreads();
+    }
+}
+
+// A few rows a sequence (a decoding step): a warp for each (sequence, block, KV head, keys or values), bytes written where they lie. The rows are read twice, for
+// the scale and for the bytes.
+template <int HD, typename T>
+__global__ void __launch_bounds__(128) append_few_kernel(Kv8Cache c, Kv8Seqs sq, Kv8Rows x, uint32_t tiles, uint32_t units, int keep_behind, int aligned, uint32_t* status) {
+    constexpr int UNIT = (int)unit_bytes(HD), WORDS = (int)KV8_BLOCK * HD / 16, LANES = HD / 4;  // lanes of a row, four dimensions each
+    pdl_launch_dependents();
+    const int lane = threadIdx.x & 31;
+    const uint32_t at = blockIdx.x * 4 + (threadIdx.x >> 5), kind = at & 1, head = (at >> 1) % c.nkv, rest = (at >> 1) / c.nkv, tile = rest % tiles, s = rest / tiles;
+    pdl_wait();
+    Seq seq;
+    if (at >= units || !sequence(sq, s, &seq, status) || seq.count == 0) return;
+    const uint32_t end = seq.start + seq.count, b_end = (end - 1) / KV8_BLOCK + 1;
+    const T* const from = (const T*)(kind ? x.v : x.k) + (size_t)head * x.hs + 4 * (lane % LANES);
+    for (uint32_t b = seq.start / KV8_BLOCK + tile; b < b_end; b += tiles) {
+        const int base = (int)(b * KV8_BLOCK), lo = max((int)seq.start - base, 0), hi = min((int)end - base, (int)KV8_BLOCK);
+        const uint32_t staying = rows_staying(lo, hi, keep_behind);
+        auto load = [&](float (&v)[4], int r) { load4(v, from + (size_t)(seq.r0 + (uint32_t)(base + r) - seq.start) * x.rs, aligned); };
+        float first[4];
+        load(first, lo);
+        const int id = block_of(c, sq, s, b, status);
+        if (id < 0) continue;
+        uint8_t* const unit = c.units + ((size_t)id * c.nkv + head) * UNIT;
+        uint2* const header = (uint2*)unit + kind;
+        uint8_t* const bytes = unit + KV8_HEADER + kind * (KV8_BLOCK * HD);
+        uint2 old = make_uint2(0, 0);
+        if (staying) old = *header;
+        uint32_t top = 0, bad = old.y & staying;
+        for (int r = lo; r < hi; r++) {
+            float v[4] = {first[0], first[1], first[2], first[3]};
+            if (r > lo) load(v, r);
+            const float m = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
+            const bool fine = fabsf(v[0]) <= FLT_MAX && fabsf(v[1]) <= FLT_MAX && fabsf(v[2]) <= FLT_MAX && fabsf(v[3]) <= FLT_MAX;
+            if (__all_sync(0xffffffffu, fine)) top = max(top, __reduce_max_sync(0xffffffffu, __float_as_uint(m)));
+            else bad |= 1u << r;
+        }
+        const float was = __uint_as_float(old.x), scale = fmaxf(pow2(scale_exponent(__uint_as_float(top))), was);
+        const float inv = 1.0f / scale, most = inv == 0x1p-122f ? 63.0f : 127.0f;
+        if (staying && was < scale) {
+            const float shrink = was * inv;
+#pragma unroll 4
+            for (int o = lane; o < WORDS; o += 32) ((uint4*)bytes)[o] = requantized<HD>(((const uint4*)bytes)[o], 16 * o, kind, staying, shrink, most);
+            __syncwarp();
+        }
+        for (int r = lo; r < hi; r++) {
+            float v[4] = {first[0], first[1], first[2], first[3]};
+            if (r > lo) load(v, r);
+            uint32_t q[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) q[e] = (bad >> r) & 1 ? 128u : to_byte(v[e] * inv, most);
+            if (lane >= LANES) continue;
+            if (kind == 0) {
+                *(uint32_t*)(bytes + key_at<HD>(r, 4 * lane)) = q[0] | q[1] << 8 | q[2] << 16 | q[3] << 24;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; e++) bytes[value_at(r, 4 * lane + e)] = (uint8_t)q[e];
+            }
+        }
+        if (lane == 0) *header = make_uint2(__float_as_uint(scale), bad);
     }
 }
 
@@ -194,12 +288,19 @@ uint32_t tiles_of(const Kv8Seqs& s) { return (uint32_t)(((size_t)s.max_rows + 2 
 template <int HD, typename T>
 cudaError_t append_t(const Kv8Cache& c, const Kv8Seqs& s, const Kv8Rows& x, bool keep_behind, uint32_t* status, cudaStream_t st, bool pdl) {
     uint32_t tiles = tiles_of(s);
-    const size_t most = 0x7fffffffu / ((size_t)c.nkv * s.n_seqs);
+    const size_t most = 0x7fffffffu / ((size_t)c.nkv * s.n_seqs * 2);
     if (most == 0) return cudaErrorInvalidValue;
     if (tiles > most) tiles = (uint32_t)most;
     const size_t unit = 4 * sizeof(T);
     const int aligned = (((uintptr_t)x.k | (uintptr_t)x.v | x.rs * sizeof(T) | x.hs * sizeof(T)) & (unit - 1)) == 0;
-    return launch_k(append_kernel<HD, T>, dim3(tiles * c.nkv * s.n_seqs), dim3(KV_THREADS), 0, st, pdl, c, s, x, tiles, keep_behind ? 1 : 0, aligned, status);
+    // Up to eight rows a sequence. 64 sequences, 8 KV heads of 128, us, a warp / a CTA a block: one row 2.9 / 8.1, four 6.2 / 10.4, eight 9.0 / 10.9, sixteen 13.0 / 11.3.
+    if (s.max_rows <= 8) {
+        const uint32_t units = 2 * tiles * c.nkv * s.n_seqs;
+        return launch_k(append_few_kernel<HD, T>, dim3((units + 3) / 4), dim3(128), 0, st, pdl, c, s, x, tiles, units, keep_behind ? 1 : 0, aligned, status);
+    }
+    // some eight CTAs an SM, two waves, which fetch a block's rows while they write the one ahead
+    tiles = std::min<uint32_t>(tiles, std::max<uint32_t>(1, (uint32_t)(KV_WAVE * 148 / (2 * (size_t)c.nkv * s.n_seqs))));
+    return launch_k(append_kernel<HD, T>, dim3(2 * tiles * c.nkv * s.n_seqs), dim3(KV_THREADS), 0, st, pdl, c, s, x, tiles, keep_behind ? 1 : 0, aligned, status);
 }
 template <int HD>
 cudaError_t append_hd(const Kv8Cache& c, const Kv8Seqs& s, const Kv8Rows& x, bool keep_behind, uint32_t* status, cudaStream_t st, bool pdl) {
