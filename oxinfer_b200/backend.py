@@ -329,17 +329,14 @@ class Backend:
     def logits_dev(self, logits, out=None, pick=None, rules=None) -> bool:
         """``rules`` (``sampling.LogitRules``) on ``logits [t][n]``: the rows into ``out`` (may be ``logits``), the first largest token of each into ``pick``
         (int32 [t]; -1 where nothing is left)."""
-        import torch
-
         t, n = logits.shape
-        dev = torch.device("cuda", self.ordinal)
-        assert logits.device == dev and logits.stride(1) == 1
+        dev, (xs, one) = logits.device, logits.stride()
+        assert dev.index == self.ordinal and one == 1
         assert out is None or (out.shape == logits.shape and out.dtype == logits.dtype and out.device == dev and out.stride(1) == 1)
-        assert pick is None or (pick.dtype == torch.int32 and pick.numel() == t and pick.is_contiguous() and pick.device == dev)
+        assert pick is None or (pick.element_size() == 4 and not pick.is_floating_point() and pick.numel() == t and pick.is_contiguous() and pick.device == dev)
         r = rules.c(t, n, dev) if rules is not None else None
-        return self._check(self._L.b2_logits_dev(self._ctx, logits.data_ptr(), out.data_ptr() if out is not None else None, _dtype_code(logits), t, n,
-                                                 logits.stride(0), out.stride(0) if out is not None else 0, C.byref(r) if r is not None else None,
-                                                 pick.data_ptr() if pick is not None else None))
+        return self._check(self._L.b2_logits_dev(self._ctx, logits.data_ptr(), None if out is None else out.data_ptr(), _dtype_code(logits), t, n, xs,
+                                                 0 if out is None else out.stride(0), None if r is None else C.byref(r), None if pick is None else pick.data_ptr()))
 
     # -- several GPUs (one process per GPU; collectives over NCCL, opened by the library itself) ----------------------
     @staticmethod

@@ -691,8 +691,7 @@ cudaError_t attend_p(AkArgs& a, uint32_t units_per_tile, cudaStream_t st, bool p
         // that differ are put at a quarter off the longest). us, cluster / dealt: one token of 32 heads of 8 KV heads over 8192, 32768 and 131071 keys 15.3 / 18.6,
         // 35.7 / 27.0, 121 / 56; 16 sequences of up to 2000 and 8000 keys 19 / 25, 57 / 40; 64 of up to 4096 75.6 / 70; 256 of up to 2000 127 / 145.
         const double mine = std::max(1.0, (double)units * C / DEALT_CTAS) * blocks / (C * AK_WARPS), dealt_out = 0.75 * units * blocks / (DEALT_CTAS * AK_WARPS) + 6;
-        const char* e1 = getenv("AK_DEALT");
-        if (a.work && (e1 ? atoi(e1) : (units <= 2 * DEALT_CTAS && mine >= dealt_out))) {
+        if (a.work && units <= 2 * DEALT_CTAS && mine >= dealt_out) {
             auto dealt = attend_kv8_kernel<HD, TERMS, T, SPECIAL, true>;
             if (cudaError_t e = ensure_dynamic_smem((const void*)dealt, L::BYTES, 0); e != cudaSuccess) return e;
             if (cudaError_t e = launch_k(dealt, dim3(DEALT_CTAS), dim3(AK_THREADS), L::BYTES, st, pdl, a); e != cudaSuccess) return e;

@@ -536,8 +536,14 @@ __global__ void __launch_bounds__(KT_THREADS, 1) attend_kv8_rows_kernel(const __
                     }
                     if (a.slopes) {
                         const float at = slope * (float)((int)(j0 + 32 * h) - (int)qp), g = f[h];
+                        const float2 g2 = make_float2(g, g), s2 = make_float2(slope, slope), at2 = make_float2(at, at);
 #pragma unroll
-                        for (int e = 0; e < 32; e++) v[h][e] = __float_as_uint(fmaf(__uint_as_float(v[h][e]), g, fmaf(slope, (float)kt_tok(e), at)));
+                        for (int e = 0; e < 32; e += 2) {
+                            const float2 bias = kt_fma2(s2, make_float2((float)kt_tok(e), (float)kt_tok(e + 1)), at2);
+                            const float2 y = kt_fma2(make_float2(__uint_as_float(v[h][e]), __uint_as_float(v[h][e + 1])), g2, bias);
+                            v[h][e] = __float_as_uint(y.x);
+                            v[h][e + 1] = __float_as_uint(y.y);
+                        }
                         f[h] = 1.0f;
                     }
                 }

@@ -10,14 +10,15 @@ from dataclasses import dataclass
 from . import _lib
 
 BLOCK = 32  # tokens of a block
+DEALT_FROM = 768  # positions of a sequence: below, its keys are never shared out over all of the GPU
 
 
-@dataclass
+@dataclass(frozen=True)
 class Kv8Seqs:
     """The sequences of a call. ``start``: int32 [n], the position of each one's first row. ``rows``: int32 [n + 1], sequence ``s`` has rows
     ``rows[s] .. rows[s + 1] - 1`` of the call's tensors, or None: ``max_rows`` each. ``table``: int32 [n, max_blocks], the pool's number of
-    each one's blocks, or None: sequence ``s`` has blocks ``s * max_blocks ..``. All int32 tensors on the device. ``n_rows``: rows in all (None: ``n *
-    max_rows``); ``max_rows``: the most rows of a sequence."""
+    each one's blocks, or None: sequence ``s`` has blocks ``s * max_blocks ..``. All int32 tensors on the device; what they hold may change from call to call.
+    ``n_rows``: rows in all (None: ``n * max_rows``); ``max_rows``: the most rows of a sequence."""
     start: object
     max_blocks: int
     max_rows: int = 1
@@ -25,18 +26,25 @@ class Kv8Seqs:
     n_rows: int | None = None
     table: object = None
 
-    def c(self, device) -> _lib.Kv8Seqs:
+    def __post_init__(self):
         import torch
 
-        n = self.start.numel()
-        assert self.rows is None or self.rows.numel() == n + 1
+        n, device = self.start.numel(), self.start.device
+        assert self.rows is None or (self.rows.numel() == n + 1 and self.n_rows is not None)
         assert self.table is None or tuple(self.table.shape) == (n, self.max_blocks)
         for x in (self.start, self.rows, self.table):
             assert x is None or (x.dtype == torch.int32 and x.device == device and x.is_contiguous())
         ptr = lambda x: x.data_ptr() if x is not None else None
-        assert self.rows is None or self.n_rows is not None
-        return _lib.Kv8Seqs(n, n * self.max_rows if self.n_rows is None else self.n_rows, self.max_rows, self.max_blocks, ptr(self.table), ptr(self.start),
-                            ptr(self.rows))
+        if self.n_rows is None:
+            object.__setattr__(self, "n_rows", n * self.max_rows)
+        object.__setattr__(self, "device", device)
+        object.__setattr__(self, "n_seqs", n)
+        # (the tensors are held by this object, so their addresses stay)
+        object.__setattr__(self, "_c", _lib.Kv8Seqs(n, self.n_rows, self.max_rows, self.max_blocks, ptr(self.table), ptr(self.start), ptr(self.rows)))
+        object.__setattr__(self, "_ref", C.byref(self._c))
+
+    def c(self, device=None) -> _lib.Kv8Seqs:
+        return self._c
 
 
 class Kv8Cache:
@@ -45,6 +53,8 @@ class Kv8Cache:
     def __init__(self, backend, handle: int, nkv: int, hd: int, n_blocks: int):
         import torch
 
+        self._torch, self._f32 = torch, torch.float32
+        self._codes = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
         self.backend, self.handle, self.nkv, self.hd, self.n_blocks = backend, handle, nkv, hd, n_blocks
         self.device = torch.device("cuda", backend.ordinal)
         self._work_bytes = _lib.lib().b2_attend_kv8_work_bytes(backend._ctx, handle)
@@ -65,42 +75,34 @@ class Kv8Cache:
 
     def append(self, seqs: Kv8Seqs, k, v) -> bool:
         """Keys and values ``[n_rows][nkv][hd]`` (f32, bf16 or f16; any strides of rows and heads, the same for both)."""
-        from .backend import _dtype_code
-
-        s = seqs.c(self.device)
-        for x in (k, v):
-            assert tuple(x.shape) == (s.n_rows, self.nkv, self.hd) and x.device == self.device and x.stride(2) == 1
-        assert k.dtype == v.dtype and (s.n_rows == 0 or k.stride() == v.stride())
-        return self.backend._check(self.backend._L.b2_kv8_append_dev(self.backend._ctx, self.handle, C.byref(s), k.data_ptr(), v.data_ptr(), _dtype_code(k),
-                                                                     k.stride(0), k.stride(1)))
+        shape, stride = (seqs.n_rows, self.nkv, self.hd), k.stride()
+        assert k.shape == shape and v.shape == shape and k.dtype == v.dtype and k.device == self.device == v.device == seqs.device
+        assert v.stride() == stride and stride[2] == 1
+        be = self.backend
+        return be._check(be._L.b2_kv8_append_dev(be._ctx, self.handle, seqs._ref, k.data_ptr(), v.data_ptr(), self._codes[k.dtype], stride[0], stride[1]))
 
     def read(self, seqs: Kv8Seqs, k, v) -> bool:
         """The values that the rows stand for into f32 ``[n_rows][nkv][hd]``."""
-        import torch
-
-        s = seqs.c(self.device)
-        for x in (k, v):
-            assert tuple(x.shape) == (s.n_rows, self.nkv, self.hd) and x.device == self.device and x.dtype == torch.float32 and x.is_contiguous()
-        return self.backend._check(self.backend._L.b2_kv8_read_dev(self.backend._ctx, self.handle, C.byref(s), k.data_ptr(), v.data_ptr()))
+        shape = (seqs.n_rows, self.nkv, self.hd)
+        assert k.shape == shape and v.shape == shape and k.dtype == v.dtype == self._f32 and k.is_contiguous() and v.is_contiguous()
+        assert k.device == self.device == v.device == seqs.device
+        be = self.backend
+        return be._check(be._L.b2_kv8_read_dev(be._ctx, self.handle, seqs._ref, k.data_ptr(), v.data_ptr()))
 
     def attend(self, seqs: Kv8Seqs, q, out, scale: float, cap: float = 0.0, window: int | None = None, slopes=None, prefix=None) -> bool:
         """Row ``i`` of a sequence attends from position ``start + i``; ``q`` and ``out`` are ``[n_rows][nh][hd]`` of one type (rows of any
         stride). Scores are ``cap * tanh(scale * q.k / cap)`` (``cap`` 0: ``scale * q.k``) ``+ slopes[h] * (key - position)``; a key is seen up to the row's own
         position or below ``prefix`` (int32 [n]), and with a ``window`` only if it is less than that far behind."""
-        import torch
-
-        from .backend import _dtype_code
-
-        s = seqs.c(self.device)
-        nh = q.shape[1]
-        for x in (q, out):
-            assert tuple(x.shape) == (s.n_rows, nh, self.hd) and x.device == self.device and x.dtype == q.dtype
-            assert x.stride(2) == 1 and x.stride(1) == self.hd
-        assert slopes is None or (slopes.dtype == torch.float32 and slopes.numel() == nh and slopes.is_contiguous() and slopes.device == self.device)
-        assert prefix is None or (prefix.dtype == torch.int32 and prefix.numel() == s.n_seqs and prefix.is_contiguous() and prefix.device == self.device)
+        n, nh, hd = q.shape
+        dtype, qs, os = q.dtype, q.stride(), out.stride()
+        assert out.shape == q.shape and n == seqs.n_rows and hd == self.hd and out.dtype == dtype and q.device == self.device == out.device == seqs.device
+        assert qs[2] == os[2] == 1 and qs[1] == os[1] == hd
+        assert slopes is None or (slopes.dtype == self._f32 and slopes.numel() == nh and slopes.is_contiguous() and slopes.device == self.device)
+        assert prefix is None or (prefix.dtype == self._torch.int32 and prefix.numel() == seqs.n_seqs and prefix.is_contiguous() and prefix.device == self.device)
         # (memory of the call's own, from torch's allocator: calls on other streams and captured ones have theirs)
-        work = torch.empty(self._work_bytes, dtype=torch.uint8, device=self.device) if q.dtype == torch.float32 or s.max_rows * (nh // self.nkv) <= 8 else None
-        a = _lib.Kv8Attention(nh, scale, cap, window or 0, slopes.data_ptr() if slopes is not None else None, prefix.data_ptr() if prefix is not None else None,
-                              work.data_ptr() if work is not None else None)
-        return self.backend._check(self.backend._L.b2_attend_kv8_dev(self.backend._ctx, self.handle, C.byref(s), C.byref(a), q.data_ptr(), q.stride(0),
-                                                                     out.data_ptr(), out.stride(0), _dtype_code(q)))
+        few = dtype == self._f32 or seqs.max_rows * nh <= 8 * self.nkv
+        work = self._torch.empty(self._work_bytes, dtype=self._torch.uint8, device=self.device) if few and seqs.max_blocks * BLOCK >= DEALT_FROM else None
+        a = _lib.Kv8Attention(nh, scale, cap, window or 0, None if slopes is None else slopes.data_ptr(), None if prefix is None else prefix.data_ptr(),
+                              None if work is None else work.data_ptr())
+        be = self.backend
+        return be._check(be._L.b2_attend_kv8_dev(be._ctx, self.handle, seqs._ref, C.byref(a), q.data_ptr(), qs[0], out.data_ptr(), os[0], self._codes[dtype]))

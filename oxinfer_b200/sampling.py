@@ -51,16 +51,24 @@ class LogitRules:
     def c(self, t: int, n: int, device) -> _lib.LogitRules:
         import torch
 
-        for x in (self.history, self.history_ptr, self.bias_ids, self.bias_ptr, self.mask):
-            assert x is None or (x.dtype == torch.int32 and x.device == device and x.is_contiguous())
-        for x in (self.history_ptr, self.bias_ptr):
-            assert x is None or x.numel() == t + 1
-        assert (self.bias_ids is None) == (self.bias is None)
-        assert self.bias is None or (self.bias.dtype == torch.float32 and self.bias.device == device and self.bias.numel() == self.bias_ids.numel() and self.bias.is_contiguous())
-        words = (n + 31) // 32
-        assert self.mask is None or (self.mask.shape[-1] >= words and self.mask.numel() in (self.mask.shape[-1], t * self.mask.shape[-1]))
-        ptr = lambda x: x.data_ptr() if x is not None and x.numel() else None
-        size = lambda x: x.numel() if x is not None else 0
-        stride = 0 if self.mask is None or (self.mask.numel() == self.mask.shape[-1] and t != 1) else self.mask.shape[-1]
-        return _lib.LogitRules(self.repeat, self.frequency, self.presence, size(self.history), size(self.bias_ids), ptr(self.history), ptr(self.history_ptr),
-                               ptr(self.bias_ids), ptr(self.bias), ptr(self.bias_ptr), ptr(self.mask), stride)
+        r = _lib.LogitRules(self.repeat, self.frequency, self.presence)
+        int32 = torch.int32
+        ok = lambda x, dtype: x.dtype == dtype and x.device == device and x.is_contiguous()
+        h, b, m = self.history, self.bias_ids, self.mask
+        if h is not None:
+            assert ok(h, int32)
+            r.n_history, r.history = h.numel(), h.data_ptr()
+            if self.history_ptr is not None:
+                assert ok(self.history_ptr, int32) and self.history_ptr.numel() == t + 1
+                r.history_ptr = self.history_ptr.data_ptr()
+        if b is not None:
+            assert ok(b, int32) and ok(self.bias, torch.float32) and self.bias.numel() == b.numel()
+            r.n_bias, r.bias_ids, r.bias = b.numel(), b.data_ptr(), self.bias.data_ptr()
+            if self.bias_ptr is not None:
+                assert ok(self.bias_ptr, int32) and self.bias_ptr.numel() == t + 1
+                r.bias_ptr = self.bias_ptr.data_ptr()
+        if m is not None:
+            width = m.shape[-1]
+            assert ok(m, int32) and width >= (n + 31) // 32 and m.numel() in (width, t * width)
+            r.mask, r.mask_stride = m.data_ptr(), width if m.numel() == t * width else 0
+        return r
