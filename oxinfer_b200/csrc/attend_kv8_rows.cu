@@ -14,9 +14,11 @@
 //
 // What bounds it: a tile's exponentials, 1024 cycles of the exponential unit for each of the two row tiles, take a warp a scheduler 1750; the row tiles take
 // turns at them (left to themselves they meet there, and the tensor cores idle while both wait for products: 132 us instead of 115), so a tile of keys takes
-// 3700 cycles, of which the tensor cores work 2048. 2048 tokens of 32 heads over 8 KV heads of 128 behind 2048 more (103 GFLOP): 117 us, 880 TFLOP/s; with a
-// cap, whose polynomial is as much work again for those warps, 201 us. On mma.sync (attend_kv8.cu) 741 and 940. Steps: bytes expanded by four warps a
-// block and everyone in step 164 us, a warp a block 142, descriptors in the warp's registers and places by turned bits 132, turns 115.
+// 3700 cycles, of which the tensor cores work 2048. 2048 tokens of 32 heads over 8 KV heads of 128 behind 2048 more (103 GFLOP): 108 us, 950 TFLOP/s; with a
+// cap, whose polynomial is as much work again for those warps, 188 us. On mma.sync (attend_kv8.cu) 741 and 940. Steps: bytes expanded by four warps a
+// block and everyone in step 164 us, a warp a block 142, descriptors in the warp's registers and places by turned bits 132, turns 115. Short prompts (16 of 17 to
+// 255 tokens, 28 us of which the tiles are a third) pay for the CTA's start: the largest scale of values is looked for by the warps that expand, while the others
+// take in the queries, sixteen rows in flight (33 us before; the same rows four at a time, fetched one step ahead, 29.4).
 #include <cfloat>
 #include <type_traits>
 
@@ -272,17 +274,6 @@ __global__ void __launch_bounds__(KT_THREADS, 1) attend_kv8_rows_kernel(const __
         mbar_init(&sh->turn[1], 4);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    // the largest scale of values that the rows may see
-    {
-        uint32_t top = 0;
-        for (uint32_t b = b_0 + tid; b < b_end; b += KT_THREADS) {
-            const int id = block_of(a.c, a.sq, s, b, a.status);
-            const float v = ((const Header*)(a.c.units + ((size_t)max(id, 0) * a.c.nkv + head) * L::UNIT))->v_scale;
-            top = max(top, __float_as_uint(fmaxf(v, 0.0f)));
-        }
-        top = __reduce_max_sync(0xffffffffu, top);
-        if (lane == 0 && top) atomicMax(&sh->v_top, top);
-    }
     if (warp == 8) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh->tmem_base)), "r"(KT_TMEM_COLS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -291,7 +282,6 @@ __global__ void __launch_bounds__(KT_THREADS, 1) attend_kv8_rows_kernel(const __
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = __shfl_sync(0xffffffffu, sh->tmem_base, 0);
-    const float v_top = __uint_as_float(sh->v_top);
 
     // 512 threads are launched with 128 registers each: 256 x 208 + 128 x 40 + 128 x 56 of them.
     if (warp >= 12) {
@@ -299,6 +289,19 @@ __global__ void __launch_bounds__(KT_THREADS, 1) attend_kv8_rows_kernel(const __
         // ---------------- bytes to f16: a warp for each block of a tile ----------------
         const uint32_t bq = warp - 12, t = lane & 3, n0 = (lane >> 2) & 1, u2 = lane >> 3;
         const __half2 one = __float2half2_rn(1.0f), off = __float2half2_rn(-1152.0f);
+        {  // the largest scale of values that the rows may see
+            uint32_t top = 0;
+#pragma unroll 4
+            for (uint32_t b = b_beg + tid - 384; b < b_end; b += 128) {
+                const int id = block_of(a.c, a.sq, s, b, a.status);
+                const float v = ((const Header*)(a.c.units + ((size_t)max(id, 0) * a.c.nkv + head) * L::UNIT))->v_scale;
+                top = max(top, __float_as_uint(fmaxf(v, 0.0f)));
+            }
+            top = __reduce_max_sync(0xffffffffu, top);
+            if (lane == 0 && top) atomicMax(&sh->v_top, top);
+            asm volatile("bar.sync 2, 128;" ::: "memory");
+        }
+        const float v_top = __uint_as_float(*(volatile uint32_t*)&sh->v_top);
         const float v_inv = v_top > 0.0f ? V_ONE / v_top : 0.0f;
         const uint8_t* const unit = smem + L::RING + bq * L::UNIT;
         const int skipped = b_0 + bq < b_beg ? 1 : 0;
@@ -447,29 +450,32 @@ __global__ void __launch_bounds__(KT_THREADS, 1) attend_kv8_rows_kernel(const __
         const int w = warp >> 2;
         const bool live = w < tiles;
         {  // the tile's queries as f16: a warp's 32 rows, a row's values over the lanes
-            constexpr int PER = HD / 4, ROWS = 32 / PER, FLIGHT = 8;
+            constexpr int PER = HD / 4, ROWS = 32 / PER, FLIGHT = 16;
             const uint32_t d4 = (uint32_t)(lane % PER), half = d4 >> 4, chunk = (d4 & 15) >> 1, in = (d4 & 1) * 8;
 #pragma unroll 1
             for (int i0 = 0; i0 < 32; i0 += FLIGHT * ROWS) {
-                float v[FLIGHT][4];
+                float x[FLIGHT][4];
 #pragma unroll
                 for (int i = 0; i < FLIGHT; i++) {
                     const uint32_t r = min(r_block + w * KT_TILE + (warp & 3) * 32 + i0 + i * ROWS + lane / PER, rows - 1), tok = kt_token(a, r);
-                    load4(v[i], (const T*)a.q + (size_t)(seq.r0 + tok) * a.q_stride + (size_t)(head * a.G + (r - tok * a.G)) * HD + 4 * d4, a.aligned);
+                    load4(x[i], (const T*)a.q + (size_t)(seq.r0 + tok) * a.q_stride + (size_t)(head * a.G + (r - tok * a.G)) * HD + 4 * d4, a.aligned);
                 }
 #pragma unroll
                 for (int i = 0; i < FLIGHT; i++) {
                     const uint32_t row = (uint32_t)((warp & 3) * 32 + i0 + i * ROWS + lane / PER);
-                    float top = fmaxf(fmaxf(fabsf(v[i][0]), fabsf(v[i][1])), fmaxf(fabsf(v[i][2]), fabsf(v[i][3])));
-                    const float sum = (v[i][0] - v[i][0]) + (v[i][1] - v[i][1]) + (v[i][2] - v[i][2]) + (v[i][3] - v[i][3]);  // NaN where one is not finite
-                    uint32_t bits = sum == 0.0f ? __float_as_uint(top) : 0x7f800000u;
+                    const uint32_t m0 = max(__float_as_uint(x[i][0]) & 0x7fffffffu, __float_as_uint(x[i][1]) & 0x7fffffffu);
+                    uint32_t bits = max(m0, max(__float_as_uint(x[i][2]) & 0x7fffffffu, __float_as_uint(x[i][3]) & 0x7fffffffu));  // (what is not finite is above all else)
+                    if (PER == 32) {
+                        bits = __reduce_max_sync(0xffffffffu, bits);
+                    } else {
 #pragma unroll
-                    for (int o = PER / 2; o > 0; o >>= 1) bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, o));
+                        for (int o = PER / 2; o > 0; o >>= 1) bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, o));
+                    }
                     const int ex = min(max((int)(bits >> 23), 40), 254) - 127;
                     const float f = pow2(-ex) * a.q_sign;
                     if (lane % PER == 0) sh->qf[w * KT_TILE + row] = (bits >= 0x7f800000u ? NAN : pow2(ex)) * a.c2;
                     *(uint2*)(smem + L::Q + w * L::TILE + half * HALF + row * 128 + ((chunk ^ (row & 7)) << 4) + in) =
-                        make_uint2(kt_pack(v[i][0] * f, v[i][1] * f), kt_pack(v[i][2] * f, v[i][3] * f));
+                        make_uint2(kt_pack(x[i][0] * f, x[i][1] * f), kt_pack(x[i][2] * f, x[i][3] * f));
                 }
             }
             fence_proxy_async();
@@ -625,7 +631,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) attend_kv8_rows_kernel(const __
         if (ok && live) {
             tc_fence_after();
             float4* const dst = (float4*)(smem + (size_t)(w * KT_TILE + row) * HD * 4);
-            const float one = v_top * (1.0f / V_ONE);
+            const float one = __uint_as_float(*(volatile uint32_t*)&sh->v_top) * (1.0f / V_ONE);
 #pragma unroll
             for (int h = 0; h < HD / 32; h++) {
                 uint32_t o[32];
@@ -635,7 +641,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) attend_kv8_rows_kernel(const __
 #pragma unroll
                 for (int e = 0; e < 8; e++) dst[(8 * h + e) ^ (row & 7)] = make_float4(f(4 * e), f(4 * e + 1), f(4 * e + 2), f(4 * e + 3));
             }
-            ml[w * KT_TILE + row] = make_float2(m, l);
+            ml[w * KT_TILE + row] = make_float2(m, a.Z > 1 ? l : l > 0.0f || l != l ? 1.0f / l : 0.0f);
         }
         __syncwarp();
         if (a.Z > 1) cluster_sync_all();
@@ -644,15 +650,20 @@ __global__ void __launch_bounds__(KT_THREADS, 1) attend_kv8_rows_kernel(const __
         if (!sh->abort_flag) {
             constexpr int PER = HD / 4, ROWS = 32 / PER;
             const uint32_t f4 = (uint32_t)(lane % PER), count = r_end - r_block;
-#pragma unroll 2
-            for (uint32_t at = (z * 8 + warp) * ROWS + lane / PER; at < count; at += a.Z * 8 * ROWS) {
-                const float4* const from = (const float4*)(smem + (size_t)at * HD * 4) + (f4 ^ (at & 7));
-                float4 o;
-                float den;
-                if (a.Z == 1) {
-                    o = *from;
-                    den = ml[at].y;
-                } else {
+            auto put = [&](uint32_t at, float4 o, float inv) {
+                const uint32_t rr = r_block + at, tk = kt_token(a, rr);
+                kt_store4<T>((T*)a.out + (size_t)(seq.r0 + tk) * a.out_stride + (size_t)(head * a.G + (rr - tk * a.G)) * HD + 4 * f4,
+                             make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv), a.aligned);
+            };
+            auto from_of = [&](uint32_t at) { return (const float4*)(smem + (size_t)at * HD * 4) + (f4 ^ (at & 7)); };
+            if (a.Z == 1) {
+#pragma unroll 4
+                for (uint32_t at = warp * ROWS + lane / PER; at < count; at += 8 * ROWS) put(at, *from_of(at), ml[at].y);
+            } else {
+                for (uint32_t at = (z * 8 + warp) * ROWS + lane / PER; at < count; at += a.Z * 8 * ROWS) {
+                    const float4* const from = from_of(at);
+                    float4 o;
+                    float den;
                     float2 p[8];
                     float4 b[8];
                     float M = -INFINITY;
@@ -672,11 +683,8 @@ __global__ void __launch_bounds__(KT_THREADS, 1) attend_kv8_rows_kernel(const __
                         o = make_float4(fmaf(g, b[k].x, o.x), fmaf(g, b[k].y, o.y), fmaf(g, b[k].z, o.z), fmaf(g, b[k].w, o.w));
                         den = fmaf(g, p[k].y, den);
                     }
+                    put(at, o, den > 0.0f || den != den ? 1.0f / den : 0.0f);
                 }
-                const float inv = den > 0.0f || den != den ? 1.0f / den : 0.0f;
-                const uint32_t rr = r_block + at, tk = kt_token(a, rr);
-                kt_store4<T>((T*)a.out + (size_t)(seq.r0 + tk) * a.out_stride + (size_t)(head * a.G + (rr - tk * a.G)) * HD + 4 * f4,
-                             make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv), a.aligned);
             }
         }
     }
