@@ -154,6 +154,7 @@ class Backend:
             raise BackendError(rc, self._L.b2_open_error().decode())
         self._ctx = ctx
         self.ordinal = ordinal
+        self.stream = 0
 
     def close(self) -> None:
         if getattr(self, "_ctx", None):
@@ -181,6 +182,7 @@ class Backend:
 
     def set_stream(self, cuda_stream: int) -> None:
         self._check(self._L.b2_set_stream(self._ctx, cuda_stream))
+        self.stream = cuda_stream or 0
 
     def launch_count(self) -> int:
         return self._L.b2_launch_count(self._ctx)

@@ -671,7 +671,7 @@ __global__ void __launch_bounds__(2 * HD) attend_kv8_join(const AkArgs a, uint32
 }
 
 template <int HD, int TERMS, bool SPECIAL, typename T>
-cudaError_t attend_p(AkArgs& a, uint32_t units_per_tile, cudaStream_t st, bool pdl) {
+cudaError_t attend_p(AkArgs& a, uint32_t units_per_tile, uint64_t& launched, cudaStream_t st, bool pdl) {
     using L = AkShared<HD, TERMS>;
     constexpr uint32_t R = TERMS == 2 ? 8 : 16;
     auto kern = attend_kv8_kernel<HD, TERMS, T, SPECIAL, false>;
@@ -695,6 +695,7 @@ cudaError_t attend_p(AkArgs& a, uint32_t units_per_tile, cudaStream_t st, bool p
             auto dealt = attend_kv8_kernel<HD, TERMS, T, SPECIAL, true>;
             if (cudaError_t e = ensure_dynamic_smem((const void*)dealt, L::BYTES, 0); e != cudaSuccess) return e;
             if (cudaError_t e = launch_k(dealt, dim3(DEALT_CTAS), dim3(AK_THREADS), L::BYTES, st, pdl, a); e != cudaSuccess) return e;
+            launched++;
             if (units <= 64) return launch_k(attend_kv8_join<HD, true, T>, dim3((unsigned)units * 8), dim3(2 * HD), 0, st, true, a, DEALT_CTAS);
             return launch_k(attend_kv8_join<HD, false, T>, dim3((unsigned)units), dim3(2 * HD), 0, st, true, a, DEALT_CTAS);
         }
@@ -718,16 +719,16 @@ cudaError_t attend_p(AkArgs& a, uint32_t units_per_tile, cudaStream_t st, bool p
     return cudaLaunchKernelEx(&cfg, kern, a);
 }
 template <int HD, int TERMS, typename T>
-cudaError_t attend_t(AkArgs& a, uint32_t units_per_tile, cudaStream_t st, bool pdl) {
-    return a.cap2 > 0.0f || a.slopes ? attend_p<HD, TERMS, true, T>(a, units_per_tile, st, pdl) : attend_p<HD, TERMS, false, T>(a, units_per_tile, st, pdl);
+cudaError_t attend_t(AkArgs& a, uint32_t units_per_tile, uint64_t& launched, cudaStream_t st, bool pdl) {
+    return a.cap2 > 0.0f || a.slopes ? attend_p<HD, TERMS, true, T>(a, units_per_tile, launched, st, pdl) : attend_p<HD, TERMS, false, T>(a, units_per_tile, launched, st, pdl);
 }
 template <int HD>
-cudaError_t attend_hd(AkArgs& a, int dtype, uint32_t units_per_tile, cudaStream_t st, bool pdl) {
+cudaError_t attend_hd(AkArgs& a, int dtype, uint32_t units_per_tile, uint64_t& launched, cudaStream_t st, bool pdl) {
     const bool few = (size_t)a.sq.max_rows * a.G <= 8;
     switch (dtype) {
-        case B2_F32: return attend_t<HD, 2, float>(a, units_per_tile, st, pdl);
-        case B2_F16: return few ? attend_t<HD, 2, __half>(a, units_per_tile, st, pdl) : attend_t<HD, 1, __half>(a, units_per_tile, st, pdl);
-        case B2_BF16: return few ? attend_t<HD, 2, __nv_bfloat16>(a, units_per_tile, st, pdl) : attend_t<HD, 1, __nv_bfloat16>(a, units_per_tile, st, pdl);
+        case B2_F32: return attend_t<HD, 2, float>(a, units_per_tile, launched, st, pdl);
+        case B2_F16: return few ? attend_t<HD, 2, __half>(a, units_per_tile, launched, st, pdl) : attend_t<HD, 1, __half>(a, units_per_tile, launched, st, pdl);
+        case B2_BF16: return few ? attend_t<HD, 2, __nv_bfloat16>(a, units_per_tile, launched, st, pdl) : attend_t<HD, 1, __nv_bfloat16>(a, units_per_tile, launched, st, pdl);
     }
     return cudaErrorInvalidValue;
 }
@@ -737,12 +738,13 @@ cudaError_t attend_hd(AkArgs& a, int dtype, uint32_t units_per_tile, cudaStream_
 size_t attend_kv8_work_bytes(uint32_t hd) { return (size_t)DEALT_CTAS * 2 * (hd == 64 ? DEALT_FLOAT4<64> : DEALT_FLOAT4<128>) * 16; }
 
 cudaError_t launch_attend_kv8(const Kv8Cache& c, const Kv8Seqs& s, const Kv8Attn& p, const void* q, size_t q_stride, void* out, size_t out_stride, int dtype,
-                              uint32_t* status, cudaStream_t st, bool pdl) {
+                              uint32_t* status, uint64_t& launched, cudaStream_t st, bool pdl) {
     if (!kv8_supports(c.nkv, c.hd) || p.nh == 0 || p.nh % c.nkv) return cudaErrorInvalidValue;
     if (s.n_seqs == 0 || s.n_rows == 0 || s.max_rows == 0) return cudaSuccess;
     // Many rows go to the form on tcgen05, from 64 of a KV head and sequence on. mma.sync / tcgen05, us, 4 heads a KV head, 8 KV heads of 128, one sequence behind
     // 4096 keys, eight behind 1024, 32 behind 512: 64 rows 18.1 / 19.7, 22.1 / 18.3, 35.5 / 31.2; 128 rows 26.3 / 21.4, 28.2 / 21.9, 62.8 / 36.1; 512 rows 76 / 30, 84 / 31.
-    if ((dtype != B2_F32 || p.halves) && (size_t)s.max_rows * (p.nh / c.nkv) >= 64)
+    launched++;
+    if ((dtype != B2_F32 || p.halves) && (size_t)s.max_rows * (p.nh / c.nkv) >= 64 && attend_kv8_rows_supports(c, s, p.nh))
         return launch_attend_kv8_rows(c, s, p, q, q_stride, out, out_stride, dtype, status, st, pdl);
     AkArgs a{};
     a.c = c;
@@ -764,7 +766,7 @@ cudaError_t launch_attend_kv8(const Kv8Cache& c, const Kv8Seqs& s, const Kv8Attn
     a.aligned = (((uintptr_t)q | (uintptr_t)out | q_stride * esz | out_stride * esz) & (unit - 1)) == 0;
     const size_t per_tile = (size_t)s.n_seqs * c.nkv;
     if (per_tile > 0x7fffffffu / 16) return cudaErrorInvalidValue;
-    return c.hd == 64 ? attend_hd<64>(a, dtype, (uint32_t)per_tile, st, pdl) : attend_hd<128>(a, dtype, (uint32_t)per_tile, st, pdl);
+    return c.hd == 64 ? attend_hd<64>(a, dtype, (uint32_t)per_tile, launched, st, pdl) : attend_hd<128>(a, dtype, (uint32_t)per_tile, launched, st, pdl);
 }
 
 }  // namespace b2

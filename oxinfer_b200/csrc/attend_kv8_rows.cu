@@ -739,8 +739,13 @@ cudaError_t rows_hd(KtArgs& a, int dtype, cudaStream_t st, bool pdl) {
 
 // Blocks of 256 rows: those of all sequences together are at most one a sequence more than of as many rows in a row.
 static size_t kv8_row_blocks(const Kv8Seqs& s, uint32_t G) {
-    const size_t rows = (size_t)s.n_rows * G, by_seq = s.rows ? s.n_seqs : (size_t)s.n_seqs;
-    return s.n_seqs == 1 ? (rows + 2 * KT_TILE - 1) / (2 * KT_TILE) : rows / (2 * KT_TILE) + by_seq;
+    const size_t rows = (size_t)s.n_rows * G;
+    return s.n_seqs == 1 ? (rows + 2 * KT_TILE - 1) / (2 * KT_TILE) : rows / (2 * KT_TILE) + s.n_seqs;
+}
+// A grid of at most 2^31 CTAs, shares of the keys included; rows times heads a KV head stay exact through g_inv.
+bool attend_kv8_rows_supports(const Kv8Cache& c, const Kv8Seqs& s, uint32_t nh) {
+    const size_t G = nh / c.nkv;
+    return kv8_row_blocks(s, (uint32_t)G) * c.nkv <= 0x7fffffffu / 8 && s.n_rows * G <= 0x7fffffffu / G;
 }
 
 cudaError_t launch_attend_kv8_rows(const Kv8Cache& c, const Kv8Seqs& s, const Kv8Attn& p, const void* q, size_t q_stride, void* out, size_t out_stride, int dtype,
@@ -756,8 +761,8 @@ cudaError_t launch_attend_kv8_rows(const Kv8Cache& c, const Kv8Seqs& s, const Kv
     a.out_stride = out_stride;
     a.G = p.nh / c.nkv;
     a.g_inv = a.G == 1 ? 0u : (uint32_t)(((1ull << 32) + a.G - 1) / a.G);
+    if (!attend_kv8_rows_supports(c, s, p.nh)) return cudaErrorInvalidValue;
     const size_t blocks = kv8_row_blocks(s, a.G);
-    if (blocks * c.nkv > 0x7fffffffu / 8 || (size_t)s.n_rows * a.G > 0x7fffffffu / a.G) return cudaErrorInvalidValue;  // (rows times heads stay exact through g_inv)
     a.blocks = (uint32_t)blocks;
     a.Z = 1;
     // Shares of the keys while two fit the chip beside each other (of clusters of eight no more than fourteen do) and have two tiles each. 32 heads of 8 KV heads of 128

@@ -1566,6 +1566,7 @@ class Backend {
         if (!s->start) return fail(B2_ERR_ARG, "[b200qmm: %s: the sequences' first positions are missing]", who);
         if (s->max_rows == 0 || s->max_rows > s->n_rows || (!s->rows && (uint64_t)s->n_seqs * s->max_rows != s->n_rows))
             return fail(B2_ERR_ARG, "[b200qmm: %s: %u rows in %u sequences of up to %u]", who, s->n_rows, s->n_seqs, s->max_rows);
+        if ((uint64_t)s->n_seqs * p->dev.nkv > 1u << 26) return fail(B2_DECLINED, "[b200qmm: %s: %u sequences of %u KV heads are too many for one call]", who, s->n_seqs, p->dev.nkv);
         if (s->max_blocks == 0 || s->max_blocks >= 1u << 26 || s->n_rows > 0x7fffffffu)
             return fail(B2_ERR_ARG, "[b200qmm: %s: a sequence has 1 to 2^26 - 1 blocks, and a call up to 2^31 - 1 rows]", who);
         if (!s->table && (uint64_t)s->n_seqs * s->max_blocks > p->dev.n_blocks)
@@ -1600,14 +1601,15 @@ class Backend {
         if (!a) return fail(B2_ERR_ARG, "[b200qmm: attend_kv8: null argument]");
         if (!dtype_ok(dtype)) return fail(B2_ERR_ARG, "[b200qmm: attend_kv8: unknown element type %d]", dtype);
         if (a->nh == 0 || a->nh % p->dev.nkv) return fail(B2_ERR_ARG, "[b200qmm: attend_kv8: %u query heads over %u KV heads]", a->nh, p->dev.nkv);
-        if (!std::isfinite(a->scale) || !std::isfinite(a->cap) || a->cap < 0.0f) return fail(B2_ERR_ARG, "[b200qmm: attend_kv8: the scale and the cap are finite, the cap not negative]");
+        // (2^60: far from where the products of scale, cap and powers of two that the kernels multiply by leave f32)
+        if (!(std::fabs(a->scale) <= 0x1p60f) || !(a->cap == 0.0f || (a->cap >= 0x1p-60f && a->cap <= 0x1p60f)))
+            return fail(B2_ERR_ARG, "[b200qmm: attend_kv8: a scale of at most 2^60 and a cap of 2^-60 to 2^60, or none]");
         if (s.n_seqs == 0 || s.n_rows == 0) return B2_OK;
         if (!q || !out) return fail(B2_ERR_ARG, "[b200qmm: attend_kv8: null argument]");
         if ((uintptr_t)a->work & 15) return fail(B2_ERR_ARG, "[b200qmm: attend_kv8: the work memory is not aligned to 16 bytes]");
         if (s.n_rows > 1 && out_stride < (size_t)a->nh * p->dev.hd) return fail(B2_ERR_ARG, "[b200qmm: attend_kv8: rows of the result overlap]");
         if ((uint64_t)s.n_rows * (a->nh / p->dev.nkv) > 0x7fffffffu) return fail(B2_DECLINED, "[b200qmm: attend_kv8: too many rows for one call]");
-        cudaError_t e = launch_attend_kv8(p->dev, s, Kv8Attn{a->nh, a->scale, a->cap, a->window, a->slopes, a->prefix, 0, a->work}, q, q_stride, out, out_stride, dtype, list_status(), stream);
-        launches++;
+        cudaError_t e = launch_attend_kv8(p->dev, s, Kv8Attn{a->nh, a->scale, a->cap, a->window, a->slopes, a->prefix, 0, a->work}, q, q_stride, out, out_stride, dtype, list_status(), launches, stream);
         return e == cudaSuccess ? B2_OK : cuda_fail(e, "attend_kv8");
     }
     int logit_rules(const b2_logit_rules* r, size_t n, const char* who, LogitRulesDev* out) {

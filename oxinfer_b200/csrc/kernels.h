@@ -330,10 +330,12 @@ struct Kv8Attn {
 size_t attend_kv8_work_bytes(uint32_t hd);
 // Row i of a sequence is a query at start + i, and sees the sequence's keys up to its own position and below the prefix, the last `window` of them.
 // attend_kv8_rows.cu: f16 operands, 256 rows a CTA.
+bool attend_kv8_rows_supports(const Kv8Cache& c, const Kv8Seqs& s, uint32_t nh);
 cudaError_t launch_attend_kv8_rows(const Kv8Cache& c, const Kv8Seqs& s, const Kv8Attn& p, const void* q, size_t q_stride, void* out, size_t out_stride, int dtype,
                                    uint32_t* status, cudaStream_t st, bool pdl = false);
+// `launched` goes up by the launches that it took: one, or two.
 cudaError_t launch_attend_kv8(const Kv8Cache& c, const Kv8Seqs& s, const Kv8Attn& p, const void* q, size_t q_stride, void* out, size_t out_stride, int dtype,
-                              uint32_t* status, cudaStream_t st, bool pdl = false);
+                              uint32_t* status, uint64_t& launched, cudaStream_t st, bool pdl = false);
 
 // ---- logits.cu: penalties, biases and masks on rows of logits, and the largest that is left ----
 struct LogitRulesDev {

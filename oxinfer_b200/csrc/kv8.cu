@@ -240,6 +240,7 @@ __global__ void __launch_bounds__(128) append_few_kernel(Kv8Cache c, Kv8Seqs sq,
                 for (int e = 0; e < 4; e++) bytes[value_at(r, 4 * lane + e)] = (uint8_t)q[e];
             }
         }
+        __syncwarp();  // (every lane has read the old header)
         if (lane == 0) *header = make_uint2(__float_as_uint(scale), bad);
     }
 }

@@ -750,10 +750,10 @@ cudaError_t DecodePlanImpl::rope_kv8(const Op& o, const uint32_t* at, uint32_t n
     const Kv8Cache c{(uint8_t*)kv_[o.kv].k, r.nkv, r.hd, (max_len_ + KV8_BLOCK - 1) / KV8_BLOCK};
     return launch_kv8_append(c, kv8_seqs(at, nt), Kv8Rows{k, v, B2_F32, r.hd, (size_t)nt * r.hd}, false, status_, st, pdl);
 }
-cudaError_t DecodePlanImpl::attend_kv8(const Op& o, const uint32_t* at, uint32_t nt, cudaStream_t st, bool pdl) {
+cudaError_t DecodePlanImpl::attend_kv8(const Op& o, const uint32_t* at, uint32_t nt, uint64_t& launched, cudaStream_t st, bool pdl) {
     const Kv8Cache c{(uint8_t*)kv_[o.kv].k, o.attn.nkv, o.attn.hd, (max_len_ + KV8_BLOCK - 1) / KV8_BLOCK};
     return launch_attend_kv8(c, kv8_seqs(at, nt), Kv8Attn{o.attn.nh, o.attn.scale, 0.0f, o.attn.window, nullptr, nullptr, prefill_ ? 1 : 0, kv8_work_}, o.x, block_floats_, o.y, block_floats_,
-                             B2_F32, status_, st, pdl);
+                             B2_F32, status_, launched, st, pdl);
 }
 
 // `chained`: every launch but the first (`first_chained`: the first too) carries the programmatic-dependent-launch
@@ -783,7 +783,8 @@ int DecodePlanImpl::run_ops(cudaStream_t st, std::string& err, bool chained, boo
                 break;
             case B2_OP_ATTEND:
                 if (kv8_) {
-                    e = attend_kv8(o, sp_, 1, st, pdl);
+                    launches_--;
+                    e = attend_kv8(o, sp_, 1, launches_, st, pdl);
                 } else if (o.fr.qkv) {
                     FusedRope fr = o.fr;
                     fr.cs_table = rope_table_;
@@ -861,7 +862,9 @@ int DecodePlanImpl::run_ops_multi(cudaStream_t st, int nt, std::string& err, boo
                 break;
             case B2_OP_ATTEND: {
                 if (kv8_) {
-                    e = attend_kv8(o, sp_multi_, (uint32_t)nt, st, pdl());
+                    const bool dependent = pdl();
+                    count--;
+                    e = attend_kv8(o, sp_multi_, (uint32_t)nt, count, st, dependent);
                     break;
                 }
                 // One launch attends for all tokens, and rotates and appends where the one-token plan's does. Otherwise it is an
@@ -1131,8 +1134,7 @@ int DecodePlanImpl::run_prefill(cudaStream_t st, size_t pos, size_t t, std::stri
                 break;
             case B2_OP_ATTEND:
                 if (kv8_) {
-                    e = attend_kv8(o, sp_, rows, st, false);
-                    count++;
+                    e = attend_kv8(o, sp_, rows, count, st, false);
                 } else if (loop_attend_) {
                     for (size_t tk = 0; tk < t && e == cudaSuccess; tk++, count++)
                         e = launch_attend(o.x + tk * ld, kv_[o.kv].k, kv_[o.kv].v, kv_f16_, o.y + tk * ld, sp_multi_ + 4 * tk, o.attn, status_, att_scratch_, st);

@@ -84,7 +84,7 @@ class DecodePlanImpl {
     int step_prefill(cudaStream_t st, size_t pos, size_t t, const float* x, const float* rope_cs, float* hidden, std::string& err);
     // Rotated queries where the op wants them and the step's rows into an 8-bit cache; attention over it. at: the first token's position on the device.
     cudaError_t rope_kv8(const Op& o, const uint32_t* at, uint32_t nt, bool rows_kernel, cudaStream_t st, bool pdl);
-    cudaError_t attend_kv8(const Op& o, const uint32_t* at, uint32_t nt, cudaStream_t st, bool pdl);
+    cudaError_t attend_kv8(const Op& o, const uint32_t* at, uint32_t nt, uint64_t& launched, cudaStream_t st, bool pdl);
     Kv8Seqs kv8_seqs(const uint32_t* at, uint32_t nt) const { return Kv8Seqs{1, nt, nt, (max_len_ + KV8_BLOCK - 1) / KV8_BLOCK, nullptr, (const int32_t*)at, nullptr}; }
     int put_rules(cudaStream_t st, const b2_generate_rules& r, size_t n_tokens, std::string& err);
     int capture(cudaStream_t st, bool with_head, cudaGraphExec_t* out, std::string& err, int nt = 1);
@@ -163,7 +163,6 @@ class DecodePlanImpl {
     struct GenRules {  // device copies; list lengths are what there is room for, the rows' parts are in the words
         LogitRulesDev dev{};
         void* room = nullptr;        // history | bias ids | biases | mask
-        size_t room_bytes = 0;
         int32_t* words = nullptr;    // history's part (2), the biases' (2), the choice (1)
         int32_t parts[4] = {};       // what they begin with
         uint64_t embed = 0;

@@ -73,6 +73,14 @@ class Kv8Cache:
         except Exception:
             pass
 
+    def _work(self):
+        """Memory of the call's own, from torch's allocator, for the backend's stream: calls on other streams and captured ones have theirs."""
+        torch, stream = self._torch, self.backend.stream
+        if torch._C._cuda_getCurrentRawStream(self.device.index) == stream:
+            return torch.empty(self._work_bytes, dtype=torch.uint8, device=self.device)
+        with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=self.device) if stream else torch.cuda.default_stream(self.device)):
+            return torch.empty(self._work_bytes, dtype=torch.uint8, device=self.device)
+
     def append(self, seqs: Kv8Seqs, k, v) -> bool:
         """Keys and values ``[n_rows][nkv][hd]`` (f32, bf16 or f16; any strides of rows and heads, the same for both)."""
         shape, stride = (seqs.n_rows, self.nkv, self.hd), k.stride()
@@ -99,9 +107,8 @@ class Kv8Cache:
         assert qs[2] == os[2] == 1 and qs[1] == os[1] == hd
         assert slopes is None or (slopes.dtype == self._f32 and slopes.numel() == nh and slopes.is_contiguous() and slopes.device == self.device)
         assert prefix is None or (prefix.dtype == self._torch.int32 and prefix.numel() == seqs.n_seqs and prefix.is_contiguous() and prefix.device == self.device)
-        # (memory of the call's own, from torch's allocator: calls on other streams and captured ones have theirs)
         few = dtype == self._f32 or seqs.max_rows * nh <= 8 * self.nkv
-        work = self._torch.empty(self._work_bytes, dtype=self._torch.uint8, device=self.device) if few and seqs.max_blocks * BLOCK >= DEALT_FROM else None
+        work = self._work() if few and seqs.max_blocks * BLOCK >= DEALT_FROM else None
         a = _lib.Kv8Attention(nh, scale, cap, window or 0, None if slopes is None else slopes.data_ptr(), None if prefix is None else prefix.data_ptr(),
                               None if work is None else work.data_ptr())
         be = self.backend
