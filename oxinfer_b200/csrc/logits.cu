@@ -5,11 +5,12 @@
 // the choice is among what is stored.
 //
 // A cluster of CTAs has a row, a slice of the tokens each. What the lists say of a slice's tokens is counted in shared memory (integers, so the order of the
-// atomics does not matter), every list read once by each CTA; the tokens that are on one are changed first, a thread each, and the pass over the
-// logits, which were asked for before all that, takes those values where there are any. The CTAs' largest values go to the first one's shared memory.
-// What bounds it: a CTA's chain (a list's bounds, its tokens, the counts, the changes, the pass), some 8 us for two to four CTAs an SM at a time, and 25 to 60
-// instructions a token. One row of 128256 7.3 us, 64 rows 21.5 us (3.1 TB/s of 66.8 MB, half of it from L2), 256 bf16 rows of 32064 under all rules 34 us.
-// Changes made in the pass itself, where every warp met one: 8.3 / 32.7 / 39.1.
+// atomics does not matter), every list read once by each CTA; the tokens that are on one are changed first, by the thread that counted one first, and the
+// pass over the logits, which were asked for before all that, takes those values where there are any. The CTAs' largest values go to the first one's shared
+// memory. What bounds it: a CTA's chain for a part (a list's bounds, its tokens, the counts, the changes, the pass), some 6 us for two to four CTAs an SM at a time, and
+// whole waves of them. One row of 128256 with 1500 tokens of history 6.8 us, 64 rows with 700 15.7 us (4.2 TB/s of 66.8 MB, half of it from L2), 256 bf16 rows of 32064
+// under all rules 28 us. Steps: changes made in the pass itself, where every warp met one, 8.3 / 32.7 / 39.1; tokens gathered in shared memory ahead of their
+// change 7.3 / 21.5 / 34 (and of their counting, 8.1 / 25 / 39.5: the barriers cost more than the threads that had nothing to do); a CTA for every part of a row 6.8 / 21.4 / 33.5.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -153,15 +154,16 @@ __global__ void __launch_bounds__(LG_THREADS, 1024 / LG_THREADS) logits_kernel(c
     float best = -INFINITY;
     int at = 0x7fffffff;
     const uint32_t end = min((cta + 1) * a.slice, a.n);
+    // a thread's tokens of the two lists, for every part; what is behind them goes through `listed`
+    constexpr int AHEAD = TIMES ? (LG_THREADS == 512 ? 8 : 4) : 0, BIASES = ENTRY ? 1 : 0;
+    uint32_t ids[AHEAD + BIASES + 1];
     for (uint32_t p0 = cta * a.slice; p0 < end; p0 += a.part) {
         const uint32_t m = min(a.part, end - p0);
-        constexpr int AHEAD = 4;  // of a thread's tokens on the history's list
-        uint32_t ids[AHEAD];
-        if (TIMES) {
+        if (p0 == cta * a.slice) {
 #pragma unroll
-            for (int i = 0; i < AHEAD; i++) {
-                const uint32_t j = h0 + tid + i * LG_THREADS;
-                ids[i] = j < h1 ? (uint32_t)a.r.history[j] : 0xffffffffu;
+            for (int i = 0; i < AHEAD + BIASES; i++) {
+                const uint32_t j = i < AHEAD ? h0 + tid + i * LG_THREADS : b0 + tid + (i - AHEAD) * LG_THREADS;
+                ids[i] = i < AHEAD ? (j < h1 ? (uint32_t)a.r.history[j] : 0xffffffffu) : j < b1 ? (uint32_t)a.r.bias_ids[j] : 0xffffffffu;
             }
         }
         uint4 w[GROUPS];
@@ -185,12 +187,18 @@ __global__ void __launch_bounds__(LG_THREADS, 1024 / LG_THREADS) logits_kernel(c
                 at0 = __shfl_sync(0xffffffffu, at0, 0);
                 if (first) listed[at0 + __popc(all & ((1u << lane) - 1))] = (uint16_t)id;
             };
+            // The first that finds a token has it: own[i] is what lies in the part and is this thread's, m else.
+            float y[AHEAD + BIASES + 1];
+            uint32_t own[AHEAD + BIASES + 1];
+#pragma unroll
+            for (int i = 0; i < AHEAD + BIASES; i++) {
+                own[i] = ids[i] != 0xffffffffu && ids[i] - p0 < m ? ids[i] - p0 : m;
+                y[i] = own[i] < m ? as_f32<T>(x[p0 + own[i]]) : 0.0f;
+            }
             if (TIMES) {
 #pragma unroll
-                for (int i = 0; i < AHEAD; i++) {
-                    const uint32_t id = ids[i] == 0xffffffffu ? m : ids[i] - p0;
-                    if (h0 + tid - lane + i * LG_THREADS < h1) put(id < m && atomicAdd(times + id, 1u) == 0, id);
-                }
+                for (int i = 0; i < AHEAD; i++)
+                    if (own[i] < m && atomicAdd(times + own[i], 1u) != 0) own[i] = m;
                 for (uint32_t i = h0 + tid - lane + AHEAD * LG_THREADS; i < h1; i += LG_THREADS) {
                     const uint32_t id = i + lane < h1 ? (uint32_t)a.r.history[i + lane] - p0 : m;
                     put(id < m && atomicAdd(times + id, 1u) == 0, id);
@@ -198,22 +206,28 @@ __global__ void __launch_bounds__(LG_THREADS, 1024 / LG_THREADS) logits_kernel(c
             }
             if (ENTRY) {
                 if (TIMES) __syncthreads();
-                for (uint32_t i = b0 + tid - lane; i < b1; i += LG_THREADS) {
+#pragma unroll
+                for (int i = AHEAD; i < AHEAD + BIASES; i++)
+                    if (own[i] < m && (atomicMax(entry + own[i], tid + (i - AHEAD) * LG_THREADS + 1) != 0 || (TIMES && times[own[i]]))) own[i] = m;
+                for (uint32_t i = b0 + tid - lane + BIASES * LG_THREADS; i < b1; i += LG_THREADS) {
                     const uint32_t id = i + lane < b1 ? (uint32_t)a.r.bias_ids[i + lane] - p0 : m;
                     put(id < m && atomicMax(entry + id, i + lane - b0 + 1) == 0 && !(TIMES && times[id]), id);
                 }
             }
             __syncthreads();
-            for (uint32_t j = tid; j < n_listed; j += LG_THREADS) {
-                const uint32_t id = listed[j], c = TIMES ? times[id] : 0, b = ENTRY ? entry[id] : 0;
-                float y = as_f32<T>(x[p0 + id]);
+            auto change = [&](uint32_t id, float y) {
+                const uint32_t c = TIMES ? times[id] : 0, b = ENTRY ? entry[id] : 0;
                 if (c) {
                     y = y > 0.0f ? __fdiv_rn(y, a.r.repeat) : __fmul_rn(y, a.r.repeat);
                     y = __fsub_rn(y, __fadd_rn(__fmul_rn((float)c, a.r.frequency), a.r.presence));
                 }
                 if (b) y = __fadd_rn(y, a.r.bias[b0 + b - 1]);
                 lists[id] = ~__float_as_uint(y == y ? y : NAN);
-            }
+            };
+#pragma unroll
+            for (int i = 0; i < AHEAD + BIASES; i++)
+                if (own[i] < m) change(own[i], y[i]);
+            for (uint32_t j = tid; j < n_listed; j += LG_THREADS) change(listed[j], as_f32<T>(x[p0 + listed[j]]));
             __syncthreads();
         }
 #pragma unroll
@@ -278,9 +292,25 @@ __global__ void __launch_bounds__(LG_THREADS, 1024 / LG_THREADS) logits_kernel(c
     if (cta == 0 && tid == 0) a.pick[row] = at == 0x7fffffff ? -1 : at;
 }
 
+// CTAs of a row, as many as end it first: waves of CTAs times their parts, and 0.4 of a part for a CTA's start and end. us, this / as many CTAs as a row has parts: 64 rows
+// of 128256 with 700 tokens of history 21.8 / 31.2 (from memory), 256 bf16 rows of 32064 with 4000 and 300 biases 28.4 / 33.5, 1000 with 500 56 / 67.
+double lg_split(uint32_t t, uint32_t n, uint32_t lists, uint32_t threads, uint32_t* C) {
+    const uint32_t parts = (n + LG_PART - 1) / LG_PART;
+    const uint32_t fit = 148 * std::min<uint32_t>(1024 / threads, lists ? 227 * 1024 / (LG_PART * (4 * lists + 2) + 2048) : 4);
+    double least = 0.0;
+    for (uint32_t c = 1; c <= std::min<uint32_t>(16, parts); c = c == 8 ? 16 : c + 1) {
+        const uint32_t at_once = c == 16 ? fit * 3 / 4 : fit;  // (fourteen clusters of sixteen fit the chip, and hardly more of nine to fifteen)
+        const double cost = (double)(((size_t)t * c + at_once - 1) / at_once) * ((parts + c - 1) / c + 0.4);
+        if (c == 1 || cost < least) {
+            *C = c;
+            least = cost;
+        }
+    }
+    return least;
+}
+
 template <typename T, int LG_THREADS>
-cudaError_t logits_n(LgArgs& a, uint32_t t, cudaStream_t st, bool pdl) {
-    const uint32_t C = std::min<uint32_t>(16, (a.n + LG_PART - 1) / LG_PART);
+cudaError_t logits_n(LgArgs& a, uint32_t t, uint32_t C, cudaStream_t st, bool pdl) {
     if (t > 0x7fffffffu / C) return cudaErrorInvalidValue;
     a.slice = ((a.n + C - 1) / C + 31) & ~31u;
     const uint32_t parts = (a.slice + LG_PART - 1) / LG_PART;
@@ -322,11 +352,13 @@ __global__ void advance_kernel(const int32_t* pick, int* token, int* out_tokens,
 
 template <typename T>
 cudaError_t logits_t(LgArgs& a, uint32_t t, cudaStream_t st, bool pdl) {
-    // CTAs of 256 threads, four an SM, where there is more than a wave of larger ones, two an SM, and the lists are short (they are one CTA's chain of
-    // work, whatever else the SM does). 512 / 256 threads, us: one row of 128256 with 1500 tokens of history 7.3 / 9.2, 64 rows with 700 26.3 / 21.5, 256 rows of
-    // 32064 with 4000 34.0 / 45.6.
-    const bool small = (size_t)t * std::min<uint32_t>(16, (a.n + LG_PART - 1) / LG_PART) > 296 && ((size_t)a.r.n_history + a.r.n_bias) / t < 1024;
-    return small ? logits_n<T, 256>(a, t, st, pdl) : logits_n<T, 512>(a, t, st, pdl);
+    // CTAs of 512 threads, two an SM, or of 256, four an SM (two where shared memory has to hold two lists), which take 1.35 times as long for a part and, with four tokens a thread
+    // at a time, are for short lists. 512 / 256 threads, us: one row of 128256 7.0 / 9.2, 16 rows with 700 tokens of history 11.3 / 8.9, 32 11.6 / 14.0, 64 24.4 / 21.6,
+    // with 4000 30.6 / 34.5; 1000 bf16 rows of 32064 with 500 79 / 56.
+    const uint32_t lists = (a.r.n_history != 0) + (a.r.n_bias != 0);
+    uint32_t C = 1, C_small = 1;
+    const bool small = lg_split(t, a.n, lists, 512, &C) > 1.35 * lg_split(t, a.n, lists, 256, &C_small) && ((size_t)a.r.n_history + a.r.n_bias) / t < 1024;
+    return small ? logits_n<T, 256>(a, t, C_small, st, pdl) : logits_n<T, 512>(a, t, C, st, pdl);
 }
 
 }  // namespace
