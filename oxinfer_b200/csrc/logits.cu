@@ -187,18 +187,22 @@ __global__ void __launch_bounds__(LG_THREADS, 1024 / LG_THREADS) logits_kernel(c
                 at0 = __shfl_sync(0xffffffffu, at0, 0);
                 if (first) listed[at0 + __popc(all & ((1u << lane) - 1))] = (uint16_t)id;
             };
-            // The first that finds a token has it: own[i] is what lies in the part and is this thread's, m else.
-            float y[AHEAD + BIASES + 1];
-            uint32_t own[AHEAD + BIASES + 1];
-#pragma unroll
-            for (int i = 0; i < AHEAD + BIASES; i++) {
-                own[i] = ids[i] != 0xffffffffu && ids[i] - p0 < m ? ids[i] - p0 : m;
-                y[i] = own[i] < m ? as_f32<T>(x[p0 + own[i]]) : 0.0f;
-            }
             if (TIMES) {
+                uint32_t all[AHEAD + 1], mine = 0;  // the first that finds a token puts it on the list
 #pragma unroll
-                for (int i = 0; i < AHEAD; i++)
-                    if (own[i] < m && atomicAdd(times + own[i], 1u) != 0) own[i] = m;
+                for (int i = 0; i < AHEAD; i++) {
+                    const uint32_t id = ids[i] != 0xffffffffu && ids[i] - p0 < m ? ids[i] - p0 : m;
+                    all[i] = __ballot_sync(0xffffffffu, id < m && atomicAdd(times + id, 1u) == 0);
+                    mine += __popc(all[i]);
+                }
+                uint32_t at0 = 0;
+                if (lane == 0 && mine) at0 = atomicAdd(&n_listed, mine);
+                at0 = __shfl_sync(0xffffffffu, at0, 0);
+#pragma unroll
+                for (int i = 0; i < AHEAD; i++) {
+                    if ((all[i] >> lane) & 1) listed[at0 + __popc(all[i] & ((1u << lane) - 1))] = (uint16_t)(ids[i] - p0);
+                    at0 += __popc(all[i]);
+                }
                 for (uint32_t i = h0 + tid - lane + AHEAD * LG_THREADS; i < h1; i += LG_THREADS) {
                     const uint32_t id = i + lane < h1 ? (uint32_t)a.r.history[i + lane] - p0 : m;
                     put(id < m && atomicAdd(times + id, 1u) == 0, id);
@@ -206,11 +210,9 @@ __global__ void __launch_bounds__(LG_THREADS, 1024 / LG_THREADS) logits_kernel(c
             }
             if (ENTRY) {
                 if (TIMES) __syncthreads();
-#pragma unroll
-                for (int i = AHEAD; i < AHEAD + BIASES; i++)
-                    if (own[i] < m && (atomicMax(entry + own[i], tid + (i - AHEAD) * LG_THREADS + 1) != 0 || (TIMES && times[own[i]]))) own[i] = m;
-                for (uint32_t i = b0 + tid - lane + BIASES * LG_THREADS; i < b1; i += LG_THREADS) {
-                    const uint32_t id = i + lane < b1 ? (uint32_t)a.r.bias_ids[i + lane] - p0 : m;
+                for (uint32_t i = b0 + tid - lane; i < b1; i += LG_THREADS) {
+                    const uint32_t given = i == b0 + tid - lane ? ids[AHEAD] : i + lane < b1 ? (uint32_t)a.r.bias_ids[i + lane] : 0xffffffffu;
+                    const uint32_t id = given != 0xffffffffu && given - p0 < m ? given - p0 : m;
                     put(id < m && atomicMax(entry + id, i + lane - b0 + 1) == 0 && !(TIMES && times[id]), id);
                 }
             }
@@ -224,9 +226,6 @@ __global__ void __launch_bounds__(LG_THREADS, 1024 / LG_THREADS) logits_kernel(c
                 if (b) y = __fadd_rn(y, a.r.bias[b0 + b - 1]);
                 lists[id] = ~__float_as_uint(y == y ? y : NAN);
             };
-#pragma unroll
-            for (int i = 0; i < AHEAD + BIASES; i++)
-                if (own[i] < m) change(own[i], y[i]);
             for (uint32_t j = tid; j < n_listed; j += LG_THREADS) change(listed[j], as_f32<T>(x[p0 + listed[j]]));
             __syncthreads();
         }
