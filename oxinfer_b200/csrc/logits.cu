@@ -5,12 +5,13 @@
 // the choice is among what is stored.
 //
 // A cluster of CTAs has a row, a slice of the tokens each. What the lists say of a slice's tokens is counted in shared memory (integers, so the order of the
-// atomics does not matter), every list read once by each CTA; the tokens that are on one are changed first, by the thread that counted one first, and the
-// pass over the logits, which were asked for before all that, takes those values where there are any. The CTAs' largest values go to the first one's shared
-// memory. What bounds it: a CTA's chain for a part (a list's bounds, its tokens, the counts, the changes, the pass), some 6 us for two to four CTAs an SM at a time, and
-// whole waves of them. One row of 128256 with 1500 tokens of history 6.8 us, 64 rows with 700 15.7 us (4.2 TB/s of 66.8 MB, half of it from L2), 256 bf16 rows of 32064
-// under all rules 28 us. Steps: changes made in the pass itself, where every warp met one, 8.3 / 32.7 / 39.1; tokens gathered in shared memory ahead of their
-// change 7.3 / 21.5 / 34 (and of their counting, 8.1 / 25 / 39.5: the barriers cost more than the threads that had nothing to do); a CTA for every part of a row 6.8 / 21.4 / 33.5.
+// atomics does not matter), every list read once by each CTA; the tokens that are on one are listed by whoever counts them first and changed, and the pass over the
+// logits, which were asked for before all that, takes those values where there are any. The CTAs' largest values go to the first one's shared memory.
+// What bounds it: a CTA's chain for a part (a list's bounds, its tokens, the counts, the changes, the pass), some 6 us for two to four CTAs an SM at a time, and
+// whole waves of them. One row of 128256 with 1500 tokens of history 6.9 us, 64 rows with 700 15.5 us (4.3 TB/s of 66.8 MB, half of it from L2), 256 bf16 rows of 32064
+// under all rules 22.6 us. Steps: changes made in the pass itself, where every warp met one, 8.3 / 32.7 / 39.1; tokens listed one warp's vote at a time 7.3 / 21.5 / 34
+// (gathered ahead of their counting, too, 8.1 / 25 / 39.5: the barriers cost more); not a CTA for every part of a row but whole waves of them 6.8 / 15.7 / 28.4; a warp's
+// votes for all of a thread's tokens at once 6.9 / 15.4 / 23.3; 16-bit logits two at a time 7.0 / 15.5 / 22.6.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -52,6 +53,19 @@ __device__ __forceinline__ T rounded(float v) {
     if constexpr (std::is_same<T, float>::value) return v;
     else if constexpr (std::is_same<T, __half>::value) return __float2half_rn(v);
     else return __float2bfloat16_rn(v);
+}
+template <typename T>
+using T2 = std::conditional_t<std::is_same<T, __half>::value, __half2, __nv_bfloat162>;
+template <typename T>
+__device__ __forceinline__ uint32_t bits_of(float v) {
+    const T t = rounded<T>(v);
+    return *(const unsigned short*)&t;
+}
+// What a token of a list has become, never zero: the complement of its bits in f32 (NaN as the one whose complement is not zero), or the bits of its rounding and one more.
+template <typename T>
+__device__ __forceinline__ uint32_t mark(float y) {
+    if constexpr (sizeof(T) == 2) return bits_of<T>(y) | 0x10000u;
+    else return ~__float_as_uint(y == y ? y : NAN);
 }
 __device__ __forceinline__ uint32_t lg_rank() {
     uint32_t r;
@@ -123,7 +137,7 @@ template <typename T, int LG_THREADS, bool TIMES, bool ENTRY>
 __global__ void __launch_bounds__(LG_THREADS, 1024 / LG_THREADS) logits_kernel(const LgArgs a) {
     constexpr uint32_t V = 16 / sizeof(T), GROUPS = LG_PART / (LG_THREADS * V);
     // [part] how often (TIMES), [part] the bias's entry + 1 (ENTRY), and the tokens that are on a list, each once, u16. What the rules make of such a token then
-    // takes the place of its count (or entry): the complement of its bits, which is not zero.
+    // takes the place of its count (or entry), see mark().
     extern __shared__ __align__(16) uint32_t lists[];
     __shared__ uint32_t n_listed;
     __shared__ float best_s[LG_THREADS / 32];
@@ -224,7 +238,7 @@ __global__ void __launch_bounds__(LG_THREADS, 1024 / LG_THREADS) logits_kernel(c
                     y = __fsub_rn(y, __fadd_rn(__fmul_rn((float)c, a.r.frequency), a.r.presence));
                 }
                 if (b) y = __fadd_rn(y, a.r.bias[b0 + b - 1]);
-                lists[id] = ~__float_as_uint(y == y ? y : NAN);
+                lists[id] = mark<T>(y);
             };
             for (uint32_t j = tid; j < n_listed; j += LG_THREADS) change(listed[j], as_f32<T>(x[p0 + listed[j]]));
             __syncthreads();
@@ -234,22 +248,41 @@ __global__ void __launch_bounds__(LG_THREADS, 1024 / LG_THREADS) logits_kernel(c
             const uint32_t i = (gi * LG_THREADS + tid) * V, k = i < m ? min(V, m - i) : 0u;
             if (k == 0) continue;
             alignas(16) T v[V];
-            *(uint4*)v = w[gi];
-            if (TIMES || ENTRY) {
+            float top;
+            if constexpr (sizeof(T) == 2) {  // two at a time
+                uint32_t x[4] = {w[gi].x, w[gi].y, w[gi].z, w[gi].w};
+                const uint32_t none = bits_of<T>(-INFINITY);
+                T2<T> high;
 #pragma unroll
-                for (uint32_t e = 0; e < V; e += 4) {
-                    const uint4 f = *(const uint4*)(lists + i + e);
-                    if (f.x) v[e] = rounded<T>(__uint_as_float(~f.x));
-                    if (f.y) v[e + 1] = rounded<T>(__uint_as_float(~f.y));
-                    if (f.z) v[e + 2] = rounded<T>(__uint_as_float(~f.z));
-                    if (f.w) v[e + 3] = rounded<T>(__uint_as_float(~f.w));
+                for (uint32_t e = 0; e < 4; e++) {
+                    uint32_t lo = x[e], hi = x[e] >> 16;
+                    if (TIMES || ENTRY) {
+                        const uint2 f = *(const uint2*)(lists + i + 2 * e);
+                        lo = f.x ? f.x : lo;
+                        hi = f.y ? f.y : hi;
+                    }
+                    if (!((allowed[gi] >> (2 * e)) & 1)) lo = none;
+                    if (!((allowed[gi] >> (2 * e + 1)) & 1)) hi = none;
+                    x[e] = __byte_perm(lo, hi, 0x5410);
+                    high = e ? __hmax2(high, *(const T2<T>*)&x[e]) : *(const T2<T>*)&x[e];  // (what lies behind the row is -inf; NaN is passed over)
                 }
-            }
-            float top = -INFINITY;
+                top = fmaxf(as_f32<T>(high.x), as_f32<T>(high.y));
+                *(uint4*)v = make_uint4(x[0], x[1], x[2], x[3]);
+            } else {
+                *(uint4*)v = w[gi];
+                if (TIMES || ENTRY) {
+                    const uint4 f = *(const uint4*)(lists + i);
+                    if (f.x) v[0] = __uint_as_float(~f.x);
+                    if (f.y) v[1] = __uint_as_float(~f.y);
+                    if (f.z) v[2] = __uint_as_float(~f.z);
+                    if (f.w) v[3] = __uint_as_float(~f.w);
+                }
+                top = -INFINITY;
 #pragma unroll
-            for (uint32_t e = 0; e < V; e++) {
-                if (!((allowed[gi] >> e) & 1)) v[e] = rounded<T>(-INFINITY);
-                top = fmaxf(top, as_f32<T>(v[e]));  // (what lies behind the row is -inf; NaN is passed over)
+                for (uint32_t e = 0; e < V; e++) {
+                    if (!((allowed[gi] >> e) & 1)) v[e] = -INFINITY;
+                    top = fmaxf(top, v[e]);
+                }
             }
             if (top > best) {  // (seldom, and the first of equals)
                 best = top;
