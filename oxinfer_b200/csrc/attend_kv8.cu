@@ -92,20 +92,33 @@ __device__ __forceinline__ uint32_t pack_rest(float a, float b, uint32_t hi) {
     const float2 f = __half22float2(*(const __half2*)&hi);
     return pack(a - f.x, b - f.y);
 }
-// cap tanh(x / cap), x and the result in powers of two: up to |z| = 1 by an odd polynomial fitted at Chebyshev nodes of z^2 (off by 1.5e-7), beyond by an exponential.
-__device__ __forceinline__ float capped(float x, float cap2, float cap_in) {
-    const float z = 0.5f * 0.69314718f * (x * cap_in), z2 = z * z;
-    float y = fmaf(z2, 1.04555360e-3f, -6.21706992e-3f);
-    y = fmaf(z2, y, 2.03055199e-2f);
-    y = fmaf(z2, y, -5.34651764e-2f);
-    y = fmaf(z2, y, 1.33253977e-1f);
-    y = fmaf(z2, y, -3.33328575e-1f);
-    y = z * fmaf(z2, y, 9.9999994e-1f);
-    if (!(fabsf(z) <= 1.0f)) {
-        const float far = 1.0f - __fdividef(2.0f, 1.0f + ex2(x * cap_in));
-        y = far;
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+// cap tanh(y / cap), y and the result in powers of two, of eight: up to |z| = 1 by an odd polynomial fitted at Chebyshev nodes of z^2 (off by 1.5e-7), beyond by an exponential.
+__device__ __forceinline__ void capped(float2 (&y)[4], float cap2, float cap_in) {
+    float2 z[4], x[4];
+    float most = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        z[j] = mul2(y[j], both(0.5f * 0.69314718f * cap_in));
+        most = max3(most, fabsf(z[j].x), fabsf(z[j].y));
+        const float2 z2 = mul2(z[j], z[j]);
+        float2 p = fma2(z2, both(1.04555360e-3f), both(-6.21706992e-3f));
+        p = fma2(z2, p, both(2.03055199e-2f));
+        p = fma2(z2, p, both(-5.34651764e-2f));
+        p = fma2(z2, p, both(1.33253977e-1f));
+        p = fma2(z2, p, both(-3.33328575e-1f));
+        x[j] = mul2(y[j], fma2(z2, p, both(9.9999994e-1f)));
     }
-    return cap2 * y;
+    if (most > 1.0f) {
+        auto far = [&](float y) { return cap2 * (1.0f - __fdividef(2.0f, 1.0f + ex2(y * cap_in))); };
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            if (fabsf(z[j].x) > 1.0f) x[j].x = far(y[j].x);
+            if (fabsf(z[j].y) > 1.0f) x[j].y = far(y[j].y);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; j++) y[j] = x[j];
 }
 template <typename T>
 __device__ __forceinline__ void store4(T* p, float4 v, bool aligned) {
@@ -416,35 +429,44 @@ __global__ void __launch_bounds__(AK_THREADS, TERMS == 2 ? 3 : 2) attend_kv8_ker
             bool grown = false;
 #pragma unroll
             for (int i = 0; i < RG; i++) {
-                const float f = qf[i] * k_scale;
-                float mx = -INFINITY;
+                float2 y[4];  // keys 16 (j / 2) + 4 t + 2 (j % 2) and the next
 #pragma unroll
-                for (int x = 0; x < 8; x++) {
-                    const uint32_t key = key0 + 16 * (x >> 2) + 4 * t + (x & 3);
-                    float y = sc[i][x] * f;
-                    if (SPECIAL && a.cap2 > 0.0f) y = capped(y, a.cap2, a.cap_in);
-                    if (SPECIAL) y = fmaf(slope[i], (float)(int)(key - pos[i]), y);
-                    if (!whole) {
-                        const bool see = key < len && (key <= pos[i] || key < prefix) && (a.window == 0 || (int)(pos[i] - key) < (int)a.window);
-                        if ((bad >> (key - key0)) & 1) y = NAN;
-                        if (!see) y = -INFINITY;
-                    }
-                    sc[i][x] = y;
-                    mx = fmaxf(mx, y);
+                for (int j = 0; j < 4; j++) y[j] = mul2(make_float2(sc[i][2 * j], sc[i][2 * j + 1]), both(qf[i] * k_scale));
+                if (SPECIAL && a.cap2 > 0.0f) capped(y, a.cap2, a.cap_in);
+                if (SPECIAL && a.slopes) {
+                    const float first = (float)(int)(key0 + 4 * t - pos[i]);
+#pragma unroll
+                    for (int j = 0; j < 4; j++) y[j] = fma2(both(slope[i]), add2(both(first), make_float2(16 * (j >> 1) + 2 * (j & 1), 16 * (j >> 1) + 2 * (j & 1) + 1)), y[j]);
                 }
+                float* const s8 = sc[i];
+#pragma unroll
+                for (int j = 0; j < 4; j++) s8[2 * j] = y[j].x, s8[2 * j + 1] = y[j].y;
+                if (!whole) {
+#pragma unroll
+                    for (int x = 0; x < 8; x++) {
+                        const uint32_t key = key0 + 16 * (x >> 2) + 4 * t + (x & 3);
+                        const bool see = key < len && (key <= pos[i] || key < prefix) && (a.window == 0 || (int)(pos[i] - key) < (int)a.window);
+                        if ((bad >> (key - key0)) & 1) s8[x] = NAN;
+                        if (!see) s8[x] = -INFINITY;
+                    }
+                }
+                float mx = fmaxf(s8[0], s8[1]);
+#pragma unroll
+                for (int x = 2; x < 8; x += 2) mx = max3(mx, s8[x], s8[x + 1]);
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
                 const float mn = fmaxf(m[i], mx), base = mn == -INFINITY ? 0.0f : mn;
                 shrink[i] = ex2(m[i] - base);
                 grown = grown || mn > m[i];
                 m[i] = mn;
-                float add = 0.0f;
+                float2 add = both(0.0f);
 #pragma unroll
-                for (int x = 0; x < 8; x++) {
-                    sc[i][x] = ex2(sc[i][x] - base + P_BITS);
-                    add += sc[i][x];
+                for (int x = 0; x < 8; x += 2) {
+                    const float2 e = add2(make_float2(s8[x], s8[x + 1]), both(P_BITS - base));
+                    s8[x] = ex2(e.x), s8[x + 1] = ex2(e.y);
+                    add = add2(add, make_float2(s8[x], s8[x + 1]));
                 }
-                l[i] = fmaf(l[i], shrink[i], add);
+                l[i] = fmaf(l[i], shrink[i], add.x + add.y);
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
                     ph[i][j] = pack(sc[i][2 * j], sc[i][2 * j + 1]);

@@ -120,28 +120,6 @@ __device__ __forceinline__ void kt_mma_ts(uint32_t d, uint32_t a, uint64_t bdesc
         "r"(a), "l"(bdesc), "r"(idesc), "r"(accumulate)
         : "memory");
 }
-__device__ __forceinline__ float kt_max3(float a, float b, float c) {
-    float d;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-    return d;
-}
-__device__ __forceinline__ float2 kt_fma2(float2 a, float2 b, float2 c) {
-    float2 d;
-    asm("{\n\t.reg .b64 a, b, c;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\tfma.rn.f32x2 a, a, b, c;\n\tmov.b64 {%0, %1}, a;\n\t}"
-        : "=f"(d.x), "=f"(d.y)
-        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-    return d;
-}
-__device__ __forceinline__ float2 kt_mul2(float2 a, float2 b) {
-    float2 d;
-    asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmul.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}" : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-    return d;
-}
-__device__ __forceinline__ float2 kt_add2(float2 a, float2 b) {
-    float2 d;
-    asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}" : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-    return d;
-}
 __device__ __forceinline__ float kt_exp2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -516,7 +494,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) attend_kv8_rows_kernel(const __
                         const float fz = fh * a.cap_z, fz2 = fz * fz;
                         float most = 0.0f;
 #pragma unroll
-                        for (int e = 0; e < 32; e += 2) most = kt_max3(most, fabsf(__uint_as_float(v[h][e])), fabsf(__uint_as_float(v[h][e + 1])));
+                        for (int e = 0; e < 32; e += 2) most = max3(most, fabsf(__uint_as_float(v[h][e])), fabsf(__uint_as_float(v[h][e + 1])));
                         if (__any_sync(0xffffffffu, !(most * fz <= 0.75f) || fz > 1.0f)) {
 #pragma unroll
                             for (int e = 0; e < 32; e++) {
@@ -532,8 +510,8 @@ __global__ void __launch_bounds__(KT_THREADS, 1) attend_kv8_rows_kernel(const __
                             const float2 c0 = k(g0 * K0), c1 = k(g1 * K1), c2 = k(g2 * K2), c3 = k(g3 * K3), c4 = k(g4 * K4);
 #pragma unroll
                             for (int e = 0; e < 32; e += 2) {
-                                const float2 x = make_float2(__uint_as_float(v[h][e]), __uint_as_float(v[h][e + 1])), x2 = kt_mul2(x, x);
-                                const float2 y = kt_mul2(x, kt_fma2(x2, kt_fma2(x2, kt_fma2(x2, kt_fma2(x2, c4, c3), c2), c1), c0));
+                                const float2 x = make_float2(__uint_as_float(v[h][e]), __uint_as_float(v[h][e + 1])), x2 = mul2(x, x);
+                                const float2 y = mul2(x, fma2(x2, fma2(x2, fma2(x2, fma2(x2, c4, c3), c2), c1), c0));
                                 v[h][e] = __float_as_uint(y.x);
                                 v[h][e + 1] = __float_as_uint(y.y);
                             }
@@ -545,8 +523,8 @@ __global__ void __launch_bounds__(KT_THREADS, 1) attend_kv8_rows_kernel(const __
                         const float2 g2 = make_float2(g, g), s2 = make_float2(slope, slope), at2 = make_float2(at, at);
 #pragma unroll
                         for (int e = 0; e < 32; e += 2) {
-                            const float2 bias = kt_fma2(s2, make_float2((float)kt_tok(e), (float)kt_tok(e + 1)), at2);
-                            const float2 y = kt_fma2(make_float2(__uint_as_float(v[h][e]), __uint_as_float(v[h][e + 1])), g2, bias);
+                            const float2 bias = fma2(s2, make_float2((float)kt_tok(e), (float)kt_tok(e + 1)), at2);
+                            const float2 y = fma2(make_float2(__uint_as_float(v[h][e]), __uint_as_float(v[h][e + 1])), g2, bias);
                             v[h][e] = __float_as_uint(y.x);
                             v[h][e + 1] = __float_as_uint(y.y);
                         }
@@ -578,7 +556,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) attend_kv8_rows_kernel(const __
             for (int h = 0; h < 4; h++) {
                 mx[h] = fmaxf(__uint_as_float(v[h][0]), __uint_as_float(v[h][1]));
 #pragma unroll
-                for (int e = 2; e < 32; e += 2) mx[h] = kt_max3(mx[h], __uint_as_float(v[h][e]), __uint_as_float(v[h][e + 1]));
+                for (int e = 2; e < 32; e += 2) mx[h] = max3(mx[h], __uint_as_float(v[h][e]), __uint_as_float(v[h][e + 1]));
                 mx[h] *= f[h];
             }
             const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
@@ -611,9 +589,9 @@ __global__ void __launch_bounds__(KT_THREADS, 1) attend_kv8_rows_kernel(const __
                 for (int e = 0; e < 32; e++) {
                     const uint32_t* at = &v[2 * h + (e >> 4)][2 * (e & 15)];
                     const float g = f[2 * h + (e >> 4)];
-                    float2 x = kt_fma2(make_float2(__uint_as_float(at[0]), __uint_as_float(at[1])), make_float2(g, g), make_float2(base, base));
+                    float2 x = fma2(make_float2(__uint_as_float(at[0]), __uint_as_float(at[1])), make_float2(g, g), make_float2(base, base));
                     x = make_float2(kt_exp2(x.x), kt_exp2(x.y));
-                    part[e & 1] = kt_add2(part[e & 1], x);
+                    part[e & 1] = add2(part[e & 1], x);
                     pk[e] = kt_pack(x.x, x.y);
                 }
                 kt_st32(s_at + 32 * h, pk);
