@@ -89,8 +89,8 @@ __device__ __forceinline__ uint32_t pack(float a, float b) {
 }
 // What f16 leaves of two values.
 __device__ __forceinline__ uint32_t pack_rest(float a, float b, uint32_t hi) {
-    const float2 f = __half22float2(*(const __half2*)&hi);
-    return pack(a - f.x, b - f.y);
+    const float2 f = __half22float2(*(const __half2*)&hi), rest = add2(make_float2(a, b), make_float2(-f.x, -f.y));
+    return pack(rest.x, rest.y);
 }
 __device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
 // cap tanh(y / cap), y and the result in powers of two, of eight: up to |z| = 1 by an odd polynomial fitted at Chebyshev nodes of z^2 (off by 1.5e-7), beyond by an exponential.
@@ -413,15 +413,10 @@ __global__ void __launch_bounds__(AK_THREADS, TERMS == 2 ? 3 : 2) attend_kv8_ker
                     mma16816(d0, qa[4 * hf + 2], low_half(w.z), high_half(w.z));
                     mma16816(d1, qa[4 * hf + 3], low_half(w.w), high_half(w.w));
                 }
-#pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    if constexpr (TERMS == 2) {
-                        sc[0][2 * j + e] = (d0[e] + d1[e]) + (d0[2 + e] + d1[2 + e]);
-                    } else {
-                        sc[0][2 * j + e] = d0[e] + d1[e];
-                        sc[RG - 1][2 * j + e] = d0[2 + e] + d1[2 + e];
-                    }
-                }
+                const float2 low = add2(make_float2(d0[0], d0[1]), make_float2(d1[0], d1[1])), high = add2(make_float2(d0[2], d0[3]), make_float2(d1[2], d1[3]));
+                const float2 first = TERMS == 2 ? add2(low, high) : low;
+                sc[0][2 * j] = first.x, sc[0][2 * j + 1] = first.y;
+                if (TERMS == 1) sc[RG - 1][2 * j] = high.x, sc[RG - 1][2 * j + 1] = high.y;
             }
             const bool whole = key0 >= in_lo && key0 + KV8_BLOCK <= in_end && bad == 0;  // every row sees every key
             uint32_t ph[RG][4], pl[4];  // probabilities of keys 4 t + 2 j .. : tile j's two
@@ -477,7 +472,10 @@ __global__ void __launch_bounds__(AK_THREADS, TERMS == 2 ? 3 : 2) attend_kv8_ker
 #pragma unroll
                 for (int n = 0; n < NT; n++)
 #pragma unroll
-                    for (int e = 0; e < 2 * RG; e++) o[n][e] *= shrink[e >> 1];
+                    for (int i = 0; i < RG; i++) {
+                        const float2 x = mul2(make_float2(o[n][2 * i], o[n][2 * i + 1]), both(shrink[i]));
+                        o[n][2 * i] = x.x, o[n][2 * i + 1] = x.y;
+                    }
             }
             uint32_t pa[2][4];
 #pragma unroll
@@ -500,17 +498,18 @@ __global__ void __launch_bounds__(AK_THREADS, TERMS == 2 ? 3 : 2) attend_kv8_ker
                 mma16816_first(d1, pa[0], low_half(w.z), high_half(w.z));
                 mma16816(d0, pa[1], low_half(w.y), high_half(w.y));
                 mma16816(d1, pa[1], low_half(w.w), high_half(w.w));
-#pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    if constexpr (TERMS == 2) {
-                        o[n][e] = fmaf(d0[e] + d0[2 + e], v_scale, o[n][e]);
-                        o[n + 1][e] = fmaf(d1[e] + d1[2 + e], v_scale, o[n + 1][e]);
-                    } else {
-                        o[n][e] = fmaf(d0[e], v_scale, o[n][e]);
-                        o[n][2 * RG - 2 + e] = fmaf(d0[2 + e], v_scale, o[n][2 * RG - 2 + e]);
-                        o[n + 1][e] = fmaf(d1[e], v_scale, o[n + 1][e]);
-                        o[n + 1][2 * RG - 2 + e] = fmaf(d1[2 + e], v_scale, o[n + 1][2 * RG - 2 + e]);
-                    }
+                auto add = [&](float* to, float2 d) {
+                    const float2 sum = fma2(d, both(v_scale), make_float2(to[0], to[1]));
+                    to[0] = sum.x, to[1] = sum.y;
+                };
+                if constexpr (TERMS == 2) {
+                    add(o[n], add2(make_float2(d0[0], d0[1]), make_float2(d0[2], d0[3])));
+                    add(o[n + 1], add2(make_float2(d1[0], d1[1]), make_float2(d1[2], d1[3])));
+                } else {
+                    add(o[n], make_float2(d0[0], d0[1]));
+                    add(o[n] + 2 * RG - 2, make_float2(d0[2], d0[3]));
+                    add(o[n + 1], make_float2(d1[0], d1[1]));
+                    add(o[n + 1] + 2 * RG - 2, make_float2(d1[2], d1[3]));
                 }
             }
             __syncwarp();  // the slot has been read by the whole warp
