@@ -87,7 +87,7 @@ __global__ void __launch_bounds__(256) qk_rope_kernel(const float* __restrict__ 
     __shared__ float red[32];
     pdl_launch_dependents();
     pdl_wait();
-    rope_head<T>(blockIdx.x, threadIdx.x, sp[0], sp[1], p.staged ? 0 : sp[0], qkv, qo, kc, vc, qn, kn, cs_table, p, buf, red);
+    rope_head<T>(blockIdx.x, threadIdx.x, sp[0], sp[1], sp[0], qkv, qo, kc, vc, qn, kn, cs_table, p, buf, red);
 }
 
 // ---- act(g) * u ---------------------------------------------------------------------------------

@@ -316,6 +316,9 @@ struct Kv8Rows {
     size_t rs, hs;
 };
 cudaError_t launch_kv8_append(const Kv8Cache& c, const Kv8Seqs& s, const Kv8Rows& x, bool keep_behind, uint32_t* status, cudaStream_t st, bool pdl = false);
+// One token at position sp[0] (launch_qk_rope's arithmetic and arguments): its rotated queries to qo, its keys and values to the cache's blocks 0 ..
+cudaError_t launch_rope_kv8(const Kv8Cache& c, const float* qkv, float* qo, const float* qn, const float* kn, const float* cs_table, const uint32_t* sp, const DecRope& p,
+                            cudaStream_t st, bool pdl = false);
 // The values that the rows stand for, f32 [n_rows][nkv][hd] each.
 cudaError_t launch_kv8_read(const Kv8Cache& c, const Kv8Seqs& s, float* k, float* v, uint32_t* status, cudaStream_t st);
 struct Kv8Attn {

@@ -9,6 +9,7 @@
 #include <algorithm>
 #include <cfloat>
 
+#include "attend_core.cuh"
 #include "pdl.cuh"
 
 namespace b2 {
@@ -17,6 +18,7 @@ using namespace kv8;
 
 namespace {
 
+constexpr uint32_t FEW = 4;  // rows of a sequence that a warp a block has
 constexpr size_t KV_WAVE = 8;  // CTAs an SM of a launch over many blocks
 constexpr int KV_THREADS = 256;  // eight threads a token: thread i has dimensions 4 i .. 4 i + 3 and every 32nd behind them
 
@@ -183,66 +185,106 @@ __global__ void __launch_bounds__(KV_THREADS, 4) append_kernel(Kv8Cache c, Kv8Se
     }
 }
 
-// A few rows a sequence (a decoding step): a warp for each (sequence, block, KV head, keys or values), bytes written where they lie. The rows are read twice, for
-// the scale and for the bytes.
+// Rows lo .. hi - 1 of a block, of one head and kind, into its unit, by a warp; row lo begins at `from`, and `old` is the unit's scale and tokens that are not finite.
+// Bytes are written where they lie. Rows behind the first four are read twice, for the scale and for the bytes.
+template <int HD, typename T>
+__device__ __forceinline__ void append_rows(uint8_t* unit, uint32_t kind, uint2 old, int lo, int hi, uint32_t staying, const T* from, size_t rs, bool aligned) {
+    constexpr int WORDS = (int)KV8_BLOCK * HD / 16, LANES = HD / 4, KEEP = (int)FEW;  // lanes of a row, four dimensions each; rows that are asked for at once
+    const int lane = threadIdx.x & 31;
+    auto load = [&](float (&v)[4], int r) { load4(v, from + (size_t)(r - lo) * rs + 4 * (lane % LANES), aligned); };
+    uint8_t* const bytes = unit + KV8_HEADER + kind * (KV8_BLOCK * HD);
+    float kept[KEEP][4];
+#pragma unroll
+    for (int i = 0; i < KEEP; i++)
+        if (lo + i < hi) load(kept[i], lo + i);
+    uint32_t top = 0, bad = old.y & staying;
+    auto look = [&](const float (&v)[4], int r) {
+        const float m = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
+        const bool fine = fabsf(v[0]) <= FLT_MAX && fabsf(v[1]) <= FLT_MAX && fabsf(v[2]) <= FLT_MAX && fabsf(v[3]) <= FLT_MAX;
+        if (__all_sync(0xffffffffu, fine)) top = max(top, __reduce_max_sync(0xffffffffu, __float_as_uint(m)));
+        else bad |= 1u << r;
+    };
+#pragma unroll
+    for (int i = 0; i < KEEP; i++)
+        if (lo + i < hi) look(kept[i], lo + i);
+    for (int r = lo + KEEP; r < hi; r++) {
+        float v[4];
+        load(v, r);
+        look(v, r);
+    }
+    const float was = __uint_as_float(old.x), scale = fmaxf(pow2(scale_exponent(__uint_as_float(top))), was);
+    const float inv = 1.0f / scale, most = inv == 0x1p-122f ? 63.0f : 127.0f;
+    if (staying && was < scale) {
+        const float shrink = was * inv;
+#pragma unroll 4
+        for (int o = lane; o < WORDS; o += 32) ((uint4*)bytes)[o] = requantized<HD>(((const uint4*)bytes)[o], 16 * o, kind, staying, shrink, most);
+        __syncwarp();
+    }
+    auto write = [&](const float (&v)[4], int r) {
+        uint32_t q[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) q[e] = (bad >> r) & 1 ? 128u : to_byte(v[e] * inv, most);
+        if (lane >= LANES) return;
+        if (kind == 0) {
+            *(uint32_t*)(bytes + key_at<HD>(r, 4 * lane)) = q[0] | q[1] << 8 | q[2] << 16 | q[3] << 24;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; e++) bytes[value_at(r, 4 * lane + e)] = (uint8_t)q[e];
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < KEEP; i++)
+        if (lo + i < hi) write(kept[i], lo + i);
+    for (int r = lo + KEEP; r < hi; r++) {
+        float v[4];
+        load(v, r);
+        write(v, r);
+    }
+    __syncwarp();  // (every lane has the old header)
+    if (lane == 0) *((uint2*)unit + kind) = make_uint2(__float_as_uint(scale), bad);
+}
+
+// A few rows a sequence (a decoding step): a warp for each (sequence, block, KV head, keys or values).
 template <int HD, typename T>
 __global__ void __launch_bounds__(128) append_few_kernel(Kv8Cache c, Kv8Seqs sq, Kv8Rows x, uint32_t tiles, uint32_t units, int keep_behind, int aligned, uint32_t* status) {
-    constexpr int UNIT = (int)unit_bytes(HD), WORDS = (int)KV8_BLOCK * HD / 16, LANES = HD / 4;  // lanes of a row, four dimensions each
     pdl_launch_dependents();
-    const int lane = threadIdx.x & 31;
     const uint32_t at = blockIdx.x * 4 + (threadIdx.x >> 5), kind = at & 1, head = (at >> 1) % c.nkv, rest = (at >> 1) / c.nkv, tile = rest % tiles, s = rest / tiles;
     pdl_wait();
     Seq seq;
     if (at >= units || !sequence(sq, s, &seq, status) || seq.count == 0) return;
     const uint32_t end = seq.start + seq.count, b_end = (end - 1) / KV8_BLOCK + 1;
-    const T* const from = (const T*)(kind ? x.v : x.k) + (size_t)head * x.hs + 4 * (lane % LANES);
+    const T* const from = (const T*)(kind ? x.v : x.k) + (size_t)head * x.hs;
     for (uint32_t b = seq.start / KV8_BLOCK + tile; b < b_end; b += tiles) {
         const int base = (int)(b * KV8_BLOCK), lo = max((int)seq.start - base, 0), hi = min((int)end - base, (int)KV8_BLOCK);
         const uint32_t staying = rows_staying(lo, hi, keep_behind);
-        auto load = [&](float (&v)[4], int r) { load4(v, from + (size_t)(seq.r0 + (uint32_t)(base + r) - seq.start) * x.rs, aligned); };
-        float first[4];
-        load(first, lo);
         const int id = block_of(c, sq, s, b, status);
         if (id < 0) continue;
-        uint8_t* const unit = c.units + ((size_t)id * c.nkv + head) * UNIT;
-        uint2* const header = (uint2*)unit + kind;
-        uint8_t* const bytes = unit + KV8_HEADER + kind * (KV8_BLOCK * HD);
-        uint2 old = make_uint2(0, 0);
-        if (staying) old = *header;
-        uint32_t top = 0, bad = old.y & staying;
-        for (int r = lo; r < hi; r++) {
-            float v[4] = {first[0], first[1], first[2], first[3]};
-            if (r > lo) load(v, r);
-            const float m = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
-            const bool fine = fabsf(v[0]) <= FLT_MAX && fabsf(v[1]) <= FLT_MAX && fabsf(v[2]) <= FLT_MAX && fabsf(v[3]) <= FLT_MAX;
-            if (__all_sync(0xffffffffu, fine)) top = max(top, __reduce_max_sync(0xffffffffu, __float_as_uint(m)));
-            else bad |= 1u << r;
-        }
-        const float was = __uint_as_float(old.x), scale = fmaxf(pow2(scale_exponent(__uint_as_float(top))), was);
-        const float inv = 1.0f / scale, most = inv == 0x1p-122f ? 63.0f : 127.0f;
-        if (staying && was < scale) {
-            const float shrink = was * inv;
-#pragma unroll 4
-            for (int o = lane; o < WORDS; o += 32) ((uint4*)bytes)[o] = requantized<HD>(((const uint4*)bytes)[o], 16 * o, kind, staying, shrink, most);
-            __syncwarp();
-        }
-        for (int r = lo; r < hi; r++) {
-            float v[4] = {first[0], first[1], first[2], first[3]};
-            if (r > lo) load(v, r);
-            uint32_t q[4];
-#pragma unroll
-            for (int e = 0; e < 4; e++) q[e] = (bad >> r) & 1 ? 128u : to_byte(v[e] * inv, most);
-            if (lane >= LANES) continue;
-            if (kind == 0) {
-                *(uint32_t*)(bytes + key_at<HD>(r, 4 * lane)) = q[0] | q[1] << 8 | q[2] << 16 | q[3] << 24;
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; e++) bytes[value_at(r, 4 * lane + e)] = (uint8_t)q[e];
-            }
-        }
-        __syncwarp();  // (every lane has read the old header)
-        if (lane == 0) *header = make_uint2(__float_as_uint(scale), bad);
+        uint8_t* const unit = c.units + ((size_t)id * c.nkv + head) * unit_bytes(HD);
+        append_rows<HD, T>(unit, kind, staying ? *((const uint2*)unit + kind) : make_uint2(0, 0), lo, hi, staying,
+                           from + (size_t)(seq.r0 + (uint32_t)(base + lo) - seq.start) * x.rs, x.rs, aligned);
     }
+}
+
+// A decoding step's token: its queries rotated, its keys and values into the cache; a CTA a head, a thread a dimension (rope_head).
+template <int HD>
+__global__ void __launch_bounds__(HD) rope_append_kernel(Kv8Cache c, const float* __restrict__ qkv, float* __restrict__ qo, const float* __restrict__ qn,
+                                                         const float* __restrict__ kn, const float* __restrict__ cs_table, const uint32_t* __restrict__ sp, DecRope p) {
+    __shared__ __align__(16) float row[HD];
+    __shared__ float buf[256], red[32];
+    pdl_launch_dependents();
+    pdl_wait();
+    const uint32_t h = blockIdx.x, pos = sp[0];
+    const bool is_query = h < p.nh;
+    const uint32_t kind = h >= p.nh + p.nkv, head = is_query ? 0 : h - p.nh - kind * p.nkv, b = pos / KV8_BLOCK;
+    if (!is_query && b >= c.n_blocks) return;  // (the host refuses the step before this)
+    uint8_t* const unit = c.units + ((size_t)b * c.nkv + head) * unit_bytes(HD);
+    const int lo = (int)(pos % KV8_BLOCK);
+    const uint32_t staying = rows_staying(lo, lo + 1, 0);
+    uint2 old = make_uint2(0, 0);
+    if (!is_query && staying && threadIdx.x < 32) old = *((const uint2*)unit + kind);
+    p.max_len = 1;  // (heads one behind the other: this one's row)
+    attend_core::rope_head<float>(h, threadIdx.x, pos, sp[1], 0, qkv, qo, row - (size_t)head * HD, row - (size_t)head * HD, qn, kn, cs_table, p, buf, red);
+    if (!is_query && threadIdx.x < 32) append_rows<HD, float>(unit, kind, old, lo, lo + 1, staying, row, HD, true);
 }
 
 template <int HD>
@@ -283,6 +325,33 @@ __global__ void __launch_bounds__(KV_THREADS) read_kernel(Kv8Cache c, Kv8Seqs sq
     }
 }
 
+// The same of a few rows a sequence: a warp for each (sequence, block, KV head, keys or values), and no more of a unit than they have.
+template <int HD>
+__global__ void __launch_bounds__(128) read_few_kernel(Kv8Cache c, Kv8Seqs sq, float* __restrict__ k, float* __restrict__ v, uint32_t tiles, uint32_t units, uint32_t* status) {
+    constexpr int UNIT = (int)unit_bytes(HD), LANES = HD / 4;
+    const int lane = threadIdx.x & 31, d = 4 * (lane % LANES);
+    const uint32_t at = blockIdx.x * 4 + (threadIdx.x >> 5), kind = at & 1, head = (at >> 1) % c.nkv, rest = (at >> 1) / c.nkv, tile = rest % tiles, s = rest / tiles;
+    Seq seq;
+    if (at >= units || !sequence(sq, s, &seq, status) || seq.count == 0) return;
+    const uint32_t end = seq.start + seq.count, b_end = (end - 1) / KV8_BLOCK + 1;
+    for (uint32_t b = seq.start / KV8_BLOCK + tile; b < b_end; b += tiles) {
+        const int id = block_of(c, sq, s, b, status);
+        if (id < 0) continue;
+        const uint8_t* const unit = c.units + ((size_t)id * c.nkv + head) * UNIT;
+        const uint2 header = *((const uint2*)unit + kind);
+        const uint8_t* const bytes = unit + KV8_HEADER + kind * (KV8_BLOCK * HD);
+        const int base = (int)(b * KV8_BLOCK), lo = max((int)seq.start - base, 0), hi = min((int)end - base, (int)KV8_BLOCK);
+        for (int r = lo + lane / LANES; r < hi; r += 32 / LANES) {
+            const float scale = (header.y >> r) & 1 ? NAN : __uint_as_float(header.x);
+            uchar4 q;
+            if (kind == 0) q = *(const uchar4*)(bytes + key_at<HD>(r, d));
+            else q = make_uchar4(bytes[value_at(r, d)], bytes[value_at(r, d + 1)], bytes[value_at(r, d + 2)], bytes[value_at(r, d + 3)]);
+            const auto value = [&](unsigned char x) { return (float)((int)x - 128) * scale; };
+            *(float4*)((kind ? v : k) + ((size_t)(seq.r0 + (uint32_t)(base + r) - seq.start) * c.nkv + head) * HD + d) = make_float4(value(q.x), value(q.y), value(q.z), value(q.w));
+        }
+    }
+}
+
 // Blocks that the rows of one sequence may reach into.
 uint32_t tiles_of(const Kv8Seqs& s) { return (uint32_t)(((size_t)s.max_rows + 2 * KV8_BLOCK - 2) / KV8_BLOCK); }
 
@@ -294,8 +363,9 @@ cudaError_t append_t(const Kv8Cache& c, const Kv8Seqs& s, const Kv8Rows& x, bool
     if (tiles > most) tiles = (uint32_t)most;
     const size_t unit = 4 * sizeof(T);
     const int aligned = (((uintptr_t)x.k | (uintptr_t)x.v | x.rs * sizeof(T) | x.hs * sizeof(T)) & (unit - 1)) == 0;
-    // Up to eight rows a sequence. 64 sequences, 8 KV heads of 128, us, a warp / a CTA a block: one row 2.9 / 8.1, four 6.2 / 10.4, eight 9.0 / 10.9, sixteen 13.0 / 11.3.
-    if (s.max_rows <= 8) {
+    // 8 KV heads of 128, us, a warp / a CTA a block: a sequence's one row 2.5 / 2.9, four 3.2 / 3.1, eight 5.4 / 3.2; 64 sequences 2.9 / 6.9, 5.1 / 6.9, 8.8 / 7.0; 256 sequences of
+    // eight 16.8 / 20.9.
+    if (s.max_rows <= FEW || (s.max_rows <= 2 * FEW && (size_t)s.n_seqs * c.nkv >= 1024)) {
         const uint32_t units = 2 * tiles * c.nkv * s.n_seqs;
         return launch_k(append_few_kernel<HD, T>, dim3((units + 3) / 4), dim3(128), 0, st, pdl, c, s, x, tiles, units, keep_behind ? 1 : 0, aligned, status);
     }
@@ -324,13 +394,28 @@ cudaError_t launch_kv8_append(const Kv8Cache& c, const Kv8Seqs& s, const Kv8Rows
     return c.hd == 64 ? append_hd<64>(c, s, x, keep_behind, status, st, pdl) : append_hd<128>(c, s, x, keep_behind, status, st, pdl);
 }
 
+cudaError_t launch_rope_kv8(const Kv8Cache& c, const float* qkv, float* qo, const float* qn, const float* kn, const float* cs_table, const uint32_t* sp, const DecRope& p,
+                            cudaStream_t st, bool pdl) {
+    if (!kv8_supports(c.nkv, c.hd) || p.hd != c.hd || p.nkv != c.nkv) return cudaErrorInvalidValue;
+    const dim3 grid(p.nh + 2 * p.nkv);
+    return c.hd == 64 ? launch_k(rope_append_kernel<64>, grid, dim3(64), 0, st, pdl, c, qkv, qo, qn, kn, cs_table, sp, p)
+                      : launch_k(rope_append_kernel<128>, grid, dim3(128), 0, st, pdl, c, qkv, qo, qn, kn, cs_table, sp, p);
+}
+
 cudaError_t launch_kv8_read(const Kv8Cache& c, const Kv8Seqs& s, float* k, float* v, uint32_t* status, cudaStream_t st) {
     if (!kv8_supports(c.nkv, c.hd)) return cudaErrorInvalidValue;
     if (s.n_seqs == 0 || s.n_rows == 0 || s.max_rows == 0) return cudaSuccess;
     uint32_t tiles = tiles_of(s);
-    const size_t most = 0x7fffffffu / ((size_t)c.nkv * s.n_seqs);
+    const size_t most = 0x7fffffffu / ((size_t)c.nkv * s.n_seqs * 2);
     if (most == 0) return cudaErrorInvalidValue;
     if (tiles > most) tiles = (uint32_t)most;
+    // 64 sequences, 8 KV heads of 128, us, a warp / a CTA a block: one row 2.1 / 3.1, four 3.6 / 4.0, eight 5.4 / 4.2.
+    if (s.max_rows <= FEW) {
+        const uint32_t units = 2 * tiles * c.nkv * s.n_seqs;
+        if (c.hd == 64) read_few_kernel<64><<<(units + 3) / 4, 128, 0, st>>>(c, s, k, v, tiles, units, status);
+        else read_few_kernel<128><<<(units + 3) / 4, 128, 0, st>>>(c, s, k, v, tiles, units, status);
+        return cudaGetLastError();
+    }
     if (c.hd == 64) read_kernel<64><<<tiles * c.nkv * s.n_seqs, KV_THREADS, 0, st>>>(c, s, k, v, tiles, status);
     else read_kernel<128><<<tiles * c.nkv * s.n_seqs, KV_THREADS, 0, st>>>(c, s, k, v, tiles, status);
     return cudaGetLastError();

@@ -739,13 +739,12 @@ GemvIn DecodePlanImpl::product_in(const Op& o, bool self) const {
     return in;
 }
 
-cudaError_t DecodePlanImpl::rope_kv8(const Op& o, const uint32_t* at, uint32_t nt, bool rows_kernel, cudaStream_t st, bool pdl) {
+cudaError_t DecodePlanImpl::rope_kv8(const Op& o, const uint32_t* at, uint32_t nt, cudaStream_t st, bool pdl) {
     DecRope r = o.rope;
     r.max_len = nt;
     r.staged = 1;
     float *k = kv8_rows_, *v = kv8_rows_ + kv8_row_floats_;
-    cudaError_t e = rows_kernel ? launch_qk_rope_rows(o.x, o.y, block_floats_, nt, k, v, 0, o.p0, o.p1, rope_table_, at, r, st)
-                                : launch_qk_rope(o.x, o.y, k, v, 0, o.p0, o.p1, rope_table_, at, r, st, pdl);
+    cudaError_t e = launch_qk_rope_rows(o.x, o.y, block_floats_, nt, k, v, 0, o.p0, o.p1, rope_table_, at, r, st);
     if (e != cudaSuccess) return e;
     const Kv8Cache c{(uint8_t*)kv_[o.kv].k, r.nkv, r.hd, (max_len_ + KV8_BLOCK - 1) / KV8_BLOCK};
     return launch_kv8_append(c, kv8_seqs(at, nt), Kv8Rows{k, v, B2_F32, r.hd, (size_t)nt * r.hd}, false, status_, st, pdl);
@@ -775,8 +774,8 @@ int DecodePlanImpl::run_ops(cudaStream_t st, std::string& err, bool chained, boo
                 break;
             case B2_OP_QK_ROPE:
                 if (kv8_) {
-                    e = rope_kv8(o, sp_, 1, false, st, pdl);
-                    launches_++;
+                    const Kv8Cache c{(uint8_t*)kv_[o.kv].k, o.rope.nkv, o.rope.hd, (max_len_ + KV8_BLOCK - 1) / KV8_BLOCK};
+                    e = launch_rope_kv8(c, o.x, o.y, o.p0, o.p1, rope_table_, sp_, o.rope, st, pdl);
                     break;
                 }
                 e = launch_qk_rope(o.x, o.y, kv_[o.kv].k, kv_[o.kv].v, kv_f16_, o.p0, o.p1, rope_table_, sp_, o.rope, st, pdl);
@@ -850,7 +849,7 @@ int DecodePlanImpl::run_ops_multi(cudaStream_t st, int nt, std::string& err, boo
                 break;
             case B2_OP_QK_ROPE:  // all tokens in one launch (the one-token arithmetic per head)
                 if (kv8_) {
-                    e = rope_kv8(o, sp_multi_, (uint32_t)nt, true, st, chained);
+                    e = rope_kv8(o, sp_multi_, (uint32_t)nt, st, chained);
                     first = false;
                     count += 2;
                     break;
@@ -1125,7 +1124,7 @@ int DecodePlanImpl::run_prefill(cudaStream_t st, size_t pos, size_t t, std::stri
             }
             case B2_OP_QK_ROPE:
                 if (kv8_) {
-                    e = rope_kv8(o, sp_, rows, true, st, false);
+                    e = rope_kv8(o, sp_, rows, st, false);
                     count++;
                 } else
                     e = launch_qk_rope_rows(o.x, o.y, ld, rows, kv_[o.kv].k, kv_[o.kv].v, kv_f16_, o.p0, o.p1, rope_table_, sp_, o.rope, st);

@@ -82,8 +82,8 @@ class DecodePlanImpl {
     int run_ops_multi(cudaStream_t st, int nt, std::string& err, bool chained);
     int run_prefill(cudaStream_t st, size_t pos, size_t t, std::string& err);
     int step_prefill(cudaStream_t st, size_t pos, size_t t, const float* x, const float* rope_cs, float* hidden, std::string& err);
-    // Rotated queries where the op wants them and the step's rows into an 8-bit cache; attention over it. at: the first token's position on the device.
-    cudaError_t rope_kv8(const Op& o, const uint32_t* at, uint32_t nt, bool rows_kernel, cudaStream_t st, bool pdl);
+    // Rotated queries where the op wants them and the rows of a step of several tokens into an 8-bit cache; attention over it. at: the first token's position on the device.
+    cudaError_t rope_kv8(const Op& o, const uint32_t* at, uint32_t nt, cudaStream_t st, bool pdl);
     cudaError_t attend_kv8(const Op& o, const uint32_t* at, uint32_t nt, uint64_t& launched, cudaStream_t st, bool pdl);
     Kv8Seqs kv8_seqs(const uint32_t* at, uint32_t nt) const { return Kv8Seqs{1, nt, nt, (max_len_ + KV8_BLOCK - 1) / KV8_BLOCK, nullptr, (const int32_t*)at, nullptr}; }
     int put_rules(cudaStream_t st, const b2_generate_rules& r, size_t n_tokens, std::string& err);
