@@ -145,7 +145,7 @@ class DecodePlan:
     def step_multi(self, pos: int, x: np.ndarray, rope_cs: np.ndarray, want_logits: bool = True, hidden_out: np.ndarray | None = None):
         """``t`` tokens at positions ``pos .. pos + t - 1`` (``Step::t``, ``src/gpu_decode.rs:538-570``): ``x`` is ``[t][n_input]``,
         ``rope_cs`` holds, for each RoPE table in turn, ``t`` rows of cos then sin. Returns (hidden ``[t][n_hidden]``, logits
-        ``[t][n_logits]`` or None); every row equals the result of a one-token step, bit for bit (a prefill plan's: up to
+        ``[t][n_logits]`` or None); every row equals the result of a one-token step, bit for bit (8-bit caches: up to the rounding of their blocks; a prefill plan's: up to
         rounding). ``hidden_out``: a caller's ``[t][n_hidden]`` f32 array to fill (page-locked memory makes the copies faster)."""
         x = np.ascontiguousarray(x, dtype=np.float32)
         t = x.shape[0]
