@@ -105,6 +105,31 @@ def test_vocabularies_of_more_than_a_cluster_counts_at_once(backend):
     check(backend, x, rules, lists)
 
 
+@pytest.mark.parametrize("t,n,dtype,history,biases,mask", [(64, 70000, "f32", 900, 0, None), (40, 131077, "bf16", 0, 700, 0.5), (300, 32064, "bf16", 1500, 600, 0.6),
+                                                            (150, 40000, "f16", 6000, 0, 0.3), (700, 9000, "f32", 100, 0, None), (620, 17000, "f16", 0, 0, 0.4), (30, 128256, "f32", 5000, 20, None)])
+def test_many_rows_with_lists_all_over_them(backend, t, n, dtype, history, biases, mask):
+    """Rows of several parts a CTA, lists of more tokens than a CTA's threads look at together, infinities and NaN among the logits; over the rows themselves, too."""
+    rng = np.random.default_rng(t + n)
+    x = torch.from_numpy((rng.standard_normal((t, n)) * 3).astype(np.float32))
+    x[torch.from_numpy(rng.integers(0, t, 200)), torch.from_numpy(rng.integers(0, n, 200))] = math.nan
+    x[torch.from_numpy(rng.integers(0, t, 50)), torch.from_numpy(rng.integers(0, n, 50))] = -math.inf
+    x[t // 2, n - 2:] = math.inf
+    x = x.to(TYPES[dtype]).to(DEV)
+    rules, lists = make(t, n, t, mask=mask, **PENALTIES)
+    if history:
+        lists["history"] = [rng.integers(-3, n + 3, m).tolist() for m in rng.integers(0, history + 1, t)]
+        lists["history"][0] = [n - 2] * history + [-1, n, n - 2]
+        rules.history, rules.history_ptr = i32(sum(lists["history"], [])), i32(np.concatenate([[0], np.cumsum([len(h) for h in lists["history"]])]))
+    if biases:
+        lists["bias"] = [list(zip(rng.integers(-3, n + 3, m).tolist(), rng.uniform(-4, 4, m).astype(np.float32).tolist())) for m in rng.integers(0, biases + 1, t)]
+        lists["bias"][t - 1] = [(n - 1, float(i)) for i in range(biases)]
+        flat = sum(lists["bias"], [])
+        rules.bias_ids, rules.bias = i32([i for i, _ in flat]), torch.tensor([b for _, b in flat], dtype=torch.float32, device=DEV)
+        rules.bias_ptr = i32(np.concatenate([[0], np.cumsum([len(b) for b in lists["bias"]])]))
+    check(backend, x, rules, lists)
+    check(backend, x, rules, lists, out=x)
+
+
 def test_ties_go_to_the_lower_token_and_nan_to_nobody(backend):
     x = torch.zeros((4, 70000), device=DEV)
     x[0, [40000, 9, 69999]] = 2.0
