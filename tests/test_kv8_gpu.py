@@ -107,6 +107,44 @@ def test_ragged_sequences_share_a_pool_through_their_tables(backend):
     backend.check_status()
 
 
+@pytest.mark.parametrize("hd,n_seqs,most", [(64, 5, 4), (128, 5, 6), (128, 130, 3), (64, 130, 8), (128, 130, 9)])
+def test_a_few_rows_of_every_sequence(backend, hd, n_seqs, most):
+    """Steps of up to `most` rows, some without one and some with one that is not finite: written, and read back alone, across the ends of blocks."""
+    nkv, max_blocks = 8, 3
+    rng = np.random.default_rng(n_seqs + most)
+    cache, models = backend.kv8(nkv, hd, n_seqs * max_blocks), [Model(nkv, hd, max_blocks) for _ in range(n_seqs)]
+    held = [int(v) for v in rng.integers(0, 40, n_seqs)]
+    first = np.concatenate([[0], np.cumsum(held)])
+    k, v = (rows_of(rng, first[-1], nkv, hd, torch.float32) for _ in range(2))
+    assert cache.append(Kv8Seqs(start=i32([0] * n_seqs), rows=i32(first), n_rows=int(first[-1]), max_rows=40, max_blocks=max_blocks), k.to(DEV), v.to(DEV))
+    for s in range(n_seqs):
+        if held[s]:
+            models[s].append(0, k[first[s]:first[s + 1]].numpy(), v[first[s]:first[s + 1]].numpy())
+    for step in range(3):
+        counts = [int(c) for c in rng.integers(0, most + 1, n_seqs)]
+        counts[step] = most
+        first = np.concatenate([[0], np.cumsum(counts)])
+        k, v = (rows_of(rng, first[-1], nkv, hd, torch.float32) for _ in range(2))
+        k[first[step], 2, 5], v[first[step], 7, 63] = np.inf, np.nan
+        seqs = Kv8Seqs(start=i32(held), rows=i32(first), n_rows=int(first[-1]), max_rows=most, max_blocks=max_blocks)
+        assert cache.append(seqs, k.to(DEV), v.to(DEV))
+        got = [torch.full((int(first[-1]), nkv, hd), -7.0, device=DEV) for _ in range(2)]
+        assert cache.read(seqs, *got)
+        got = [x.cpu().numpy().astype(np.float64) for x in got]
+        for s in range(n_seqs):
+            if counts[s]:
+                models[s].append(held[s], k[first[s]:first[s + 1]].numpy(), v[first[s]:first[s + 1]].numpy())
+                for g, w in zip(got, models[s].values(held[s] + counts[s])):
+                    assert np.array_equal(g[first[s]:first[s + 1]], w[held[s]:], equal_nan=True), (step, s)
+            held[s] += counts[s]
+    got = read(cache, [0] * n_seqs, held, max_blocks)
+    first = np.concatenate([[0], np.cumsum(held)])
+    for s in range(n_seqs):
+        for g, w in zip(got, models[s].values(held[s])):
+            assert np.array_equal(g[first[s]:first[s + 1]], w, equal_nan=True), s
+    backend.check_status()
+
+
 def test_magnitudes_from_zero_to_the_largest(backend):
     nkv, hd = 1, 64
     tops = [0.0, 1e-45, 1e-38, 127 * 2.0 ** -100, 126.9999 * 2.0 ** -100, 127.0, np.nextafter(np.float32(127.0), np.float32(200)), 128.0, 254.0, 1e30, np.finfo(np.float32).max]
