@@ -69,7 +69,7 @@ struct KtArgs {
     float c2, q_sign, cap2, cap_z;      // |scale| in powers of two and its sign; cap in powers of two, and what brings scores in powers of two to score / cap
     const float* slopes;
     const int32_t* prefix;
-    int aligned;
+    int aligned, wide;                  // queries and results: four values to their size, eight 16-bit ones to 16 bytes
     uint32_t Z;
     uint32_t* status;
 };
@@ -428,32 +428,62 @@ __global__ void __launch_bounds__(KT_THREADS, 1) attend_kv8_rows_kernel(const __
         const int w = warp >> 2;
         const bool live = w < tiles;
         {  // the tile's queries as f16: a warp's 32 rows, a row's values over the lanes
-            constexpr int PER = HD / 4, ROWS = 32 / PER, FLIGHT = 16;
-            const uint32_t d4 = (uint32_t)(lane % PER), half = d4 >> 4, chunk = (d4 & 15) >> 1, in = (d4 & 1) * 8;
+            auto from = [&](uint32_t in_warp, uint32_t d) {
+                const uint32_t r = min(r_block + w * KT_TILE + (warp & 3) * 32 + in_warp, rows - 1), tok = kt_token(a, r);
+                return (const T*)a.q + (size_t)(seq.r0 + tok) * a.q_stride + (size_t)(head * a.G + (r - tok * a.G)) * HD + d;
+            };
+            auto factor = [&](uint32_t row, uint32_t bits, bool first) {  // of a row whose largest magnitude has those bits (what is not finite is above all else)
+                const int ex = min(max((int)(bits >> 23), 40), 254) - 127;
+                if (first) sh->qf[w * KT_TILE + row] = (bits >= 0x7f800000u ? NAN : pow2(ex)) * a.c2;
+                return pow2(-ex) * a.q_sign;
+            };
+            if (sizeof(T) == 2 && a.wide) {  // eight a lane: half the instructions of the form below
+                constexpr int PER = HD / 8, ROWS = 32 / PER, FLIGHT = 8;
+                const uint32_t d8 = (uint32_t)(lane % PER);
+                uint8_t* const to = smem + L::Q + w * L::TILE + (d8 >> 3) * HALF;
 #pragma unroll 1
-            for (int i0 = 0; i0 < 32; i0 += FLIGHT * ROWS) {
-                float x[FLIGHT][4];
+                for (int i0 = 0; i0 < 32; i0 += FLIGHT * ROWS) {
+                    uint4 eight[FLIGHT];
 #pragma unroll
-                for (int i = 0; i < FLIGHT; i++) {
-                    const uint32_t r = min(r_block + w * KT_TILE + (warp & 3) * 32 + i0 + i * ROWS + lane / PER, rows - 1), tok = kt_token(a, r);
-                    load4(x[i], (const T*)a.q + (size_t)(seq.r0 + tok) * a.q_stride + (size_t)(head * a.G + (r - tok * a.G)) * HD + 4 * d4, a.aligned);
-                }
+                    for (int i = 0; i < FLIGHT; i++) eight[i] = *(const uint4*)from((uint32_t)(i0 + i * ROWS + lane / PER), 8 * d8);
 #pragma unroll
-                for (int i = 0; i < FLIGHT; i++) {
-                    const uint32_t row = (uint32_t)((warp & 3) * 32 + i0 + i * ROWS + lane / PER);
-                    const uint32_t m0 = max(__float_as_uint(x[i][0]) & 0x7fffffffu, __float_as_uint(x[i][1]) & 0x7fffffffu);
-                    uint32_t bits = max(m0, max(__float_as_uint(x[i][2]) & 0x7fffffffu, __float_as_uint(x[i][3]) & 0x7fffffffu));  // (what is not finite is above all else)
-                    if (PER == 32) {
-                        bits = __reduce_max_sync(0xffffffffu, bits);
-                    } else {
+                    for (int i = 0; i < FLIGHT; i++) {
+                        const uint32_t row = (uint32_t)((warp & 3) * 32 + i0 + i * ROWS + lane / PER);
+                        const T* const v = (const T*)&eight[i];
+                        float x[8];
+                        uint32_t bits = 0;
+#pragma unroll
+                        for (int e = 0; e < 8; e++) {
+                            x[e] = to_f32<T>(v[e]);
+                            bits = max(bits, __float_as_uint(x[e]) & 0x7fffffffu);
+                        }
 #pragma unroll
                         for (int o = PER / 2; o > 0; o >>= 1) bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, o));
+                        const float f = factor(row, bits, d8 == 0);
+                        *(uint4*)(to + row * 128 + (((d8 & 7) ^ (row & 7)) << 4)) =
+                            make_uint4(kt_pack(x[0] * f, x[1] * f), kt_pack(x[2] * f, x[3] * f), kt_pack(x[4] * f, x[5] * f), kt_pack(x[6] * f, x[7] * f));
                     }
-                    const int ex = min(max((int)(bits >> 23), 40), 254) - 127;
-                    const float f = pow2(-ex) * a.q_sign;
-                    if (lane % PER == 0) sh->qf[w * KT_TILE + row] = (bits >= 0x7f800000u ? NAN : pow2(ex)) * a.c2;
-                    *(uint2*)(smem + L::Q + w * L::TILE + half * HALF + row * 128 + ((chunk ^ (row & 7)) << 4) + in) =
-                        make_uint2(kt_pack(x[i][0] * f, x[i][1] * f), kt_pack(x[i][2] * f, x[i][3] * f));
+                }
+            } else {
+                constexpr int PER = HD / 4, ROWS = 32 / PER, FLIGHT = 8;
+                const uint32_t d4 = (uint32_t)(lane % PER), half = d4 >> 4, chunk = (d4 & 15) >> 1, in = (d4 & 1) * 8;
+#pragma unroll 1
+                for (int i0 = 0; i0 < 32; i0 += FLIGHT * ROWS) {
+                    float x[FLIGHT][4];
+#pragma unroll
+                    for (int i = 0; i < FLIGHT; i++) load4(x[i], from((uint32_t)(i0 + i * ROWS + lane / PER), 4 * d4), a.aligned);
+#pragma unroll
+                    for (int i = 0; i < FLIGHT; i++) {
+                        const uint32_t row = (uint32_t)((warp & 3) * 32 + i0 + i * ROWS + lane / PER);
+                        uint32_t bits = 0;
+#pragma unroll
+                        for (int e = 0; e < 4; e++) bits = max(bits, __float_as_uint(x[i][e]) & 0x7fffffffu);
+#pragma unroll
+                        for (int o = PER / 2; o > 0; o >>= 1) bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, o));
+                        const float f = factor(row, bits, d4 == 0);
+                        *(uint2*)(smem + L::Q + w * L::TILE + half * HALF + row * 128 + ((chunk ^ (row & 7)) << 4) + in) =
+                            make_uint2(kt_pack(x[i][0] * f, x[i][1] * f), kt_pack(x[i][2] * f, x[i][3] * f));
+                    }
                 }
             }
             fence_proxy_async();
@@ -634,7 +664,24 @@ __global__ void __launch_bounds__(KT_THREADS, 1) attend_kv8_rows_kernel(const __
                              make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv), a.aligned);
             };
             auto from_of = [&](uint32_t at) { return (const float4*)(smem + (size_t)at * HD * 4) + (f4 ^ (at & 7)); };
-            if (a.Z == 1) {
+            if (sizeof(T) == 2 && a.Z == 1 && a.wide) {
+                constexpr uint32_t PER8 = HD / 8, ROWS8 = 32 / PER8;
+                const uint32_t d8 = (uint32_t)lane % PER8;
+#pragma unroll 4
+                for (uint32_t at = warp * ROWS8 + lane / PER8; at < count; at += 8 * ROWS8) {
+                    const float4* const row = (const float4*)(smem + (size_t)at * HD * 4);
+                    const float4 x = row[(2 * d8) ^ (at & 7)], y = row[(2 * d8 + 1) ^ (at & 7)];
+                    const float inv = ml[at].y, v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+                    const uint32_t rr = r_block + at, tk = kt_token(a, rr);
+                    alignas(16) T o[8];
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        if constexpr (std::is_same<T, __half>::value) o[e] = __float2half_rn(v[e] * inv);
+                        else if constexpr (sizeof(T) == 2) o[e] = __float2bfloat16_rn(v[e] * inv);
+                    }
+                    *(uint4*)((T*)a.out + (size_t)(seq.r0 + tk) * a.out_stride + (size_t)(head * a.G + (rr - tk * a.G)) * HD + 8 * d8) = *(const uint4*)o;
+                }
+            } else if (a.Z == 1) {
 #pragma unroll 4
                 for (uint32_t at = warp * ROWS + lane / PER; at < count; at += 8 * ROWS) put(at, *from_of(at), ml[at].y);
             } else {
@@ -756,6 +803,7 @@ cudaError_t launch_attend_kv8_rows(const Kv8Cache& c, const Kv8Seqs& s, const Kv
     a.status = status;
     const size_t esz = dtype == B2_F32 ? 4 : 2, unit = 4 * esz;
     a.aligned = (((uintptr_t)q | (uintptr_t)out | q_stride * esz | out_stride * esz) & (unit - 1)) == 0;
+    a.wide = (((uintptr_t)q | (uintptr_t)out | q_stride * esz | out_stride * esz) & 15) == 0;
     return c.hd == 64 ? rows_hd<64>(a, dtype, st, pdl) : rows_hd<128>(a, dtype, st, pdl);
 }
 
