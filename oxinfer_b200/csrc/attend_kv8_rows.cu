@@ -14,11 +14,12 @@
 //
 // What bounds it: a tile's exponentials, 1024 cycles of the exponential unit for each of the two row tiles, take a warp a scheduler 1750; the row tiles take
 // turns at them (left to themselves they meet there, and the tensor cores idle while both wait for products: 132 us instead of 115), so a tile of keys takes
-// 3700 cycles, of which the tensor cores work 2048. 2048 tokens of 32 heads over 8 KV heads of 128 behind 2048 more (103 GFLOP): 108 us, 950 TFLOP/s; with a
-// cap, whose polynomial is as much work again for those warps, 188 us. On mma.sync (attend_kv8.cu) 741 and 940. Steps: bytes expanded by four warps a
-// block and everyone in step 164 us, a warp a block 142, descriptors in the warp's registers and places by turned bits 132, turns 115. Short prompts (16 of 17 to
-// 255 tokens, 28 us of which the tiles are a third) pay for the CTA's start: the largest scale of values is looked for by the warps that expand, while the others
-// take in the queries, sixteen rows in flight (33 us before; the same rows four at a time, fetched one step ahead, 29.4).
+// 3700 cycles, of which the tensor cores work 2048. 2048 tokens of 32 heads over 8 KV heads of 128 behind 2048 more (103 GFLOP): 106 us, 970 TFLOP/s; with a
+// cap, whose polynomial is as much work again for those warps, 187 us. On mma.sync (attend_kv8.cu) 741 and 940. Steps: bytes expanded by four warps a
+// block and everyone in step 164 us, a warp a block 142, descriptors in the warp's registers and places by turned bits 132, turns 115. Short prompts (five of 185 to
+// 542 tokens with 12 heads 27.8 us, half of it in the tiles) pay for the CTA's start: the largest scale of values is looked for by the warps that expand, while the others
+// take in the queries, sixteen rows in flight (33 us before; the same rows four at a time, fetched one step ahead, 29.4)
+// with eight values a lane. What goes into the exponentials made ahead of a tile's turn and their sums behind it: no gain.
 #include <cfloat>
 #include <type_traits>
 

@@ -73,7 +73,7 @@ def test_scales_of_values_that_differ(backend):
     assert (y[:32].abs().amax() < 2.0 ** -11) and torch.isfinite(out).all() and j.numel() == n
 
 
-@pytest.mark.parametrize("shift", [0, 1])
+@pytest.mark.parametrize("shift", [0, 1, 4])
 def test_strides_and_results_in_place(backend, shift):
     s = Setting(backend, [100, 177], [70, 150], 4, 2, 64, "f16", seed=12)
     want = s.check()
