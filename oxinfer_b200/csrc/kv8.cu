@@ -3,8 +3,8 @@
 //
 // append: scale = 2^e, e the smallest with largest magnitude <= 127 * 2^e over the block's new rows (not below 2^-100), and not below the scale of the
 // rows of the block that stay; q = round half to even (x / scale), exact but for that rounding (at the scale 2^122 at most 63, so that the value is finite). Rows that stay are brought to a larger scale the same way.
-// What bounds it: a prompt of 8192 rows of 8 KV heads of 128 HBM, f32 rows appended in 19.3 us (84 MB, 4.4 TB/s) and read back in 14.2 (5.9 TB/s); a step of 64 sequences a launch and three
-// dependent reads, 2.9 and 2.3 us.
+// What bounds it: a prompt of 8192 rows of 8 KV heads of 128 the issue slots beside HBM, f32 rows appended in 15.1 us (84 MB, 5.6 TB/s), bf16 in 12.7 (50 MB, 4 TB/s), read back in 14.2
+// (84 MB, 5.9 TB/s); a step of 64 sequences a launch and three dependent reads, 2.8 and 2.3 us.
 // A row with a value that is not finite is marked, and counts as NaN: it does not enter the scale, and the block's other rows are as they would be without it.
 #include "kv8.cuh"
 
@@ -21,7 +21,8 @@ using namespace kv8;
 namespace {
 
 constexpr uint32_t FEW = 4;  // rows of a sequence that a warp a block has
-constexpr size_t KV_WAVE = 12;  // CTAs an SM of a launch over many blocks
+constexpr int KV_CTAS = 4;       // of an SM
+constexpr size_t KV_WAVE = 8;    // of a launch over many blocks, which fetch a block's rows while they write the one ahead
 constexpr int KV_THREADS = 256;  // eight threads a token
 
 // e of the largest magnitude: mantissas up to 127 / 64 fit 127 * 2^(exponent - 6).
@@ -68,46 +69,50 @@ __device__ __forceinline__ uint32_t top_bits(uint32_t top) {
     return __float_as_uint(to_f32<T>(*(const T*)&m));
 }
 
-// Grid: (sequence, block of the rows', KV head, keys or values), a CTA each: the block's image in shared memory, then out of it 16 bytes a thread. A thread has eight
-// dimensions (and eight of the other half of 128) of a token. Six CTAs an SM, two waves, which fetch a block's rows while they write the one ahead (four, with four dimensions
-// at a time and a barrier more a block: 8192 rows of 8 KV heads of 128 19.2 us f32, 19.3 bf16).
+// Grid: (sequence, block of the rows', KV head), a CTA each: the unit's image in shared memory, then out of it 16 bytes a thread at a time. A thread has eight
+// dimensions (and eight of the other half of 128) of a token's keys and values. 8192 rows of 8 KV heads of 128, us, f32 and bf16: keys and values
+// a CTA each, four dimensions at a time and a barrier more a block 19.2 and 19.3, eight dimensions and six CTAs an SM 17.9 and 16.1, both kinds by one CTA 15.1 and 12.7 (that
+// halves what is done once a block; issue slots bound it, 78 % of them).
 template <int HD, typename T>
-__global__ void __launch_bounds__(KV_THREADS, 6) append_kernel(Kv8Cache c, Kv8Seqs sq, Kv8Rows x, uint32_t tiles, int keep_behind, int wide, uint32_t* status) {
-    constexpr int J = HD / 64, UNIT = (int)unit_bytes(HD), WARPS = KV_THREADS / 32, WORDS = (int)KV8_BLOCK * HD / 16, V = 16 / (int)sizeof(T), PARTS = 8 / V;
-    __shared__ __align__(16) uint8_t images[2][KV8_BLOCK * HD];  // (in turn: a block's is written while the one ahead's may still be on its way out)
-    __shared__ __align__(16) uint32_t warp_top[WARPS], warp_bad[WARPS];
+__global__ void __launch_bounds__(KV_THREADS, KV_CTAS) append_kernel(Kv8Cache c, Kv8Seqs sq, Kv8Rows x, uint32_t tiles, int keep_behind, int wide, uint32_t* status) {
+    constexpr int J = HD / 64, UNIT = (int)unit_bytes(HD), WARPS = KV_THREADS / 32, IMAGE = (int)KV8_BLOCK * HD, WORDS = IMAGE / 16, V = 16 / (int)sizeof(T), PARTS = 8 / V;
+    __shared__ __align__(16) uint8_t images[2][2 * IMAGE];  // keys, then values (in turn: a block's is written while the one ahead's may still be on its way out)
+    __shared__ __align__(16) uint32_t warp_top[2][WARPS], warp_bad[2][WARPS];
     pdl_launch_dependents();
     const int tid = threadIdx.x, r = tid >> 3, d8 = (tid & 7) * 8, warp = tid >> 5, lane = tid & 31;
-    const uint32_t kind = blockIdx.x & 1, head = (blockIdx.x >> 1) % c.nkv, rest = (blockIdx.x >> 1) / c.nkv, tile = rest % tiles, s = rest / tiles;
+    const uint32_t head = blockIdx.x % c.nkv, rest = blockIdx.x / c.nkv, tile = rest % tiles, s = rest / tiles;
     pdl_wait();
     Seq seq;
     if (!sequence(sq, s, &seq, status) || seq.count == 0) return;
     const uint32_t end = seq.start + seq.count, b_end = (end - 1) / KV8_BLOCK + 1;
     uint32_t b = seq.start / KV8_BLOCK + tile;
     if (b >= b_end) return;
-    const T* const from = (const T*)(kind ? x.v : x.k) + (size_t)head * x.hs + d8;
+    const size_t from = (size_t)head * x.hs + d8;
     auto rows_of = [&](uint32_t b, int* lo, int* hi) {
         const int base = (int)(b * KV8_BLOCK);  // (positions are below 2^31)
         *lo = max((int)seq.start - base, 0);
         *hi = min((int)end - base, (int)KV8_BLOCK);
     };
-    uint4 v[J * PARTS];
+    uint4 v[2][J * PARTS];
     int id;
     auto fetch = [&](uint32_t b) {  // a block's rows and its place
         int lo, hi;
         rows_of(b, &lo, &hi);
+        const bool is_new = r >= lo && r < hi;
+        const size_t row = from + (size_t)(is_new ? seq.r0 + b * KV8_BLOCK + (uint32_t)r - seq.start : 0u) * x.rs;
 #pragma unroll
-        for (int j = 0; j < J * PARTS; j++) v[j] = make_uint4(0, 0, 0, 0);
-        if (r >= lo && r < hi) {
-            const T* const row = from + (size_t)(seq.r0 + b * KV8_BLOCK + (uint32_t)r - seq.start) * x.rs;
-            if (wide) {
+        for (int kind = 0; kind < 2; kind++) {
+            const T* const at = (const T*)(kind ? x.v : x.k) + row;
 #pragma unroll
-                for (int j = 0; j < J * PARTS; j++) v[j] = *(const uint4*)(row + 64 * (j / PARTS) + V * (j % PARTS));
-            } else {
+            for (int j = 0; j < J * PARTS; j++) v[kind][j] = make_uint4(0, 0, 0, 0);
+            if (is_new && wide) {
+#pragma unroll
+                for (int j = 0; j < J * PARTS; j++) v[kind][j] = *(const uint4*)(at + 64 * (j / PARTS) + V * (j % PARTS));
+            } else if (is_new) {
 #pragma unroll
                 for (int j = 0; j < J * PARTS; j++)
 #pragma unroll
-                    for (int e = 0; e < V; e++) ((T*)&v[j])[e] = row[64 * (j / PARTS) + V * (j % PARTS) + e];
+                    for (int e = 0; e < V; e++) ((T*)&v[kind][j])[e] = at[64 * (j / PARTS) + V * (j % PARTS) + e];
             }
         }
         id = block_of(c, sq, s, b, status);
@@ -122,88 +127,94 @@ __global__ void __launch_bounds__(KV_THREADS, 6) append_kernel(Kv8Cache c, Kv8Se
             if (b + tiles < b_end) fetch(b + tiles);
             continue;
         }
-        uint8_t* const unit = c.units + ((size_t)id * c.nkv + head) * UNIT;
-        uint2* const header = (uint2*)unit + kind;  // the kind's scale and tokens that are not finite
-        uint8_t* const bytes = unit + KV8_HEADER + kind * (KV8_BLOCK * HD);
+        uint8_t* const unit = c.units + ((size_t)id * c.nkv + head) * UNIT;  // (begins with the keys' scale and tokens that are not finite, and the values')
         uint8_t* const image = images[turn ^= 1];
-        uint2 old = make_uint2(0, 0);
-        if (staying) old = *header;
-        uint32_t top = 0;
+        uint4 old = make_uint4(0, 0, 0, 0);
+        if (staying) old = *(const uint4*)unit;
+        bool fine[2];
 #pragma unroll
-        for (int j = 0; j < J * PARTS; j++) top = top_of<T>(top_of<T>(top_of<T>(top_of<T>(top, v[j].x), v[j].y), v[j].z), v[j].w);
-        top = top_bits<T>(top);
-        bool fine = top < 0x7f800000u;
-        {
-            const uint32_t odd = __ballot_sync(0xffffffffu, !fine);  // a byte for each of the warp's four rows
+        for (int kind = 0; kind < 2; kind++) {
+            uint32_t top = 0;
+#pragma unroll
+            for (int j = 0; j < J * PARTS; j++) top = top_of<T>(top_of<T>(top_of<T>(top_of<T>(top, v[kind][j].x), v[kind][j].y), v[kind][j].z), v[kind][j].w);
+            top = top_bits<T>(top);
+            fine[kind] = top < 0x7f800000u;
+            const uint32_t odd = __ballot_sync(0xffffffffu, !fine[kind]);  // a byte for each of the warp's four rows
             uint32_t bad = 0;
             if (odd) {
 #pragma unroll
                 for (int w = 0; w < 4; w++) bad |= ((odd >> (8 * w)) & 0xffu) ? 1u << w : 0u;
-                fine = !((bad >> (lane >> 3)) & 1u);
+                fine[kind] = !((bad >> (lane >> 3)) & 1u);
             }
-            const uint32_t m = __reduce_max_sync(0xffffffffu, fine ? top : 0u);
+            const uint32_t m = __reduce_max_sync(0xffffffffu, fine[kind] ? top : 0u);
             if (lane == 0) {
-                warp_top[warp] = m;
-                warp_bad[warp] = bad << (4 * warp);
+                warp_top[kind][warp] = m;
+                warp_bad[kind][warp] = bad << (4 * warp);
             }
         }
         __syncthreads();  // (the old header has been read by everyone, too)
-        const uint4 t0 = *(const uint4*)warp_top, t1 = *(const uint4*)(warp_top + 4), b0 = *(const uint4*)warp_bad, b1 = *(const uint4*)(warp_bad + 4);
-        static_assert(WARPS == 8);
-        const uint32_t m = max(max(max(t0.x, t0.y), max(t0.z, t0.w)), max(max(t1.x, t1.y), max(t1.z, t1.w)));
-        const uint32_t bad = (old.y & staying) | b0.x | b0.y | b0.z | b0.w | b1.x | b1.y | b1.z | b1.w;
-        const float was = __uint_as_float(old.x), scale = fmaxf(pow2(scale_exponent(__uint_as_float(m))), was);
-        const float inv = __uint_as_float((254u << 23) - __float_as_uint(scale)), most = inv == 0x1p-122f ? 63.0f : 127.0f;  // (powers of two)
+        float was[2] = {__uint_as_float(old.x), __uint_as_float(old.z)}, scale[2], inv[2], most[2];
+        uint32_t bad[2] = {old.y & staying, old.w & staying};
+#pragma unroll
+        for (int kind = 0; kind < 2; kind++) {
+            static_assert(WARPS == 8);
+            const uint4 t0 = *(const uint4*)warp_top[kind], t1 = *(const uint4*)(warp_top[kind] + 4), b0 = *(const uint4*)warp_bad[kind], b1 = *(const uint4*)(warp_bad[kind] + 4);
+            const uint32_t m = max(max(max(t0.x, t0.y), max(t0.z, t0.w)), max(max(t1.x, t1.y), max(t1.z, t1.w)));
+            bad[kind] |= b0.x | b0.y | b0.z | b0.w | b1.x | b1.y | b1.z | b1.w;
+            scale[kind] = fmaxf(pow2(scale_exponent(__uint_as_float(m))), was[kind]);
+            inv[kind] = __uint_as_float((254u << 23) - __float_as_uint(scale[kind]));  // (powers of two)
+            most[kind] = inv[kind] == 0x1p-122f ? 63.0f : 127.0f;
+        }
         if (hi - lo < (int)KV8_BLOCK) {  // what the image has of other rows
-            const float shrink = was * inv;
-            for (int o = tid; o < WORDS; o += KV_THREADS) {
-                uint4 w = make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
-                if (staying) {
-                    w = ((const uint4*)bytes)[o];
-                    if (was < scale) w = requantized<HD>(w, 16 * o, kind, staying, shrink, most);
+#pragma unroll
+            for (int kind = 0; kind < 2; kind++)
+                for (int o = tid; o < WORDS; o += KV_THREADS) {
+                    uint4 w = make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
+                    if (staying) {
+                        w = ((const uint4*)(unit + KV8_HEADER + kind * IMAGE))[o];
+                        if (was[kind] < scale[kind]) w = requantized<HD>(w, 16 * o, kind, staying, was[kind] * inv[kind], most[kind]);
+                    }
+                    ((uint4*)(image + kind * IMAGE))[o] = w;
                 }
-                ((uint4*)image)[o] = w;
-            }
             __syncthreads();
         }
-        uint32_t w[2 * J];  // of four dimensions
+        uint32_t w[2][2 * J];  // of four dimensions
 #pragma unroll
-        for (int j = 0; j < 2 * J; j++) {
-            const T* const four = (const T*)v + 4 * j;
-            if (!fine) {
-                w[j] = 0x80808080u;
-            } else if (most == 127.0f) {  // a sum with 1.5 * 2^23 is rounded to a whole number, to even, and its last byte is the byte
-                uint32_t q[4];
+        for (int kind = 0; kind < 2; kind++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) q[e] = __float_as_uint(fmaf(to_f32<T>(four[e]), inv, 12582912.0f + 128.0f));
-                w[j] = __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
-            } else {
-                w[j] = 0;
+            for (int j = 0; j < 2 * J; j++) {
+                const T* const four = (const T*)v[kind] + 4 * j;
+                if (!fine[kind]) {
+                    w[kind][j] = 0x80808080u;
+                } else if (most[kind] == 127.0f) {  // a sum with 1.5 * 2^23 is rounded to a whole number, to even, and its last byte is the byte
+                    uint32_t q[4];
 #pragma unroll
-                for (int e = 0; e < 4; e++) w[j] |= to_byte(to_f32<T>(four[e]) * inv, most) << (8 * e);
-            }
-        }
-        if (b + tiles < b_end) fetch(b + tiles);  // (under this block's way out)
-        if (kind == 0) {
+                    for (int e = 0; e < 4; e++) q[e] = __float_as_uint(fmaf(to_f32<T>(four[e]), inv[kind], 12582912.0f + 128.0f));
+                    w[kind][j] = __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
+                } else {
+                    w[kind][j] = 0;
 #pragma unroll
-            for (int j = 0; j < J; j++)
-                if (is_new) *(uint2*)(image + key_at<HD>(r, d8 + 64 * j)) = make_uint2(w[2 * j], w[2 * j + 1]);
-        } else {
-            const uint32_t l0 = (lane >> 3) & 1, l1 = lane >> 4, quad = (rows_between(lo, hi) >> (4 * warp)) & 0xfu;  // the warp's four tokens
-            const uint32_t keep = ~(((quad & 1) | (quad & 2) << 7 | (quad & 4) << 14 | (quad & 8) << 21) * 0xffu);
-            if (quad) {
-#pragma unroll
-                for (int j = 0; j < 2 * J; j++) {  // four dimensions of a token to four tokens of a dimension, over the lanes of the four tokens
-                    const uint32_t p = __shfl_xor_sync(0xffffffffu, w[j], 8), z = __byte_perm(w[j], p, l0 ? 0x3715 : 0x6240);
-                    const uint32_t p2 = __shfl_xor_sync(0xffffffffu, z, 16), y = __byte_perm(z, p2, l1 ? 0x3276 : 0x5410);
-                    uint32_t* const to = (uint32_t*)(image + value_at(4 * warp, d8 + 64 * (j >> 1) + 4 * (j & 1) + 2 * l1 + l0));
-                    *to = keep ? (*to & keep) | (y & ~keep) : y;
+                    for (int e = 0; e < 4; e++) w[kind][j] |= to_byte(to_f32<T>(four[e]) * inv[kind], most[kind]) << (8 * e);
                 }
             }
+        if (b + tiles < b_end) fetch(b + tiles);  // (under this block's way out)
+#pragma unroll
+        for (int j = 0; j < J; j++)
+            if (is_new) *(uint2*)(image + key_at<HD>(r, d8 + 64 * j)) = make_uint2(w[0][2 * j], w[0][2 * j + 1]);
+        const uint32_t l0 = (lane >> 3) & 1, l1 = lane >> 4, quad = (rows_between(lo, hi) >> (4 * warp)) & 0xfu;  // the warp's four tokens
+        if (quad) {
+            const uint32_t keep = ~(((quad & 1) | (quad & 2) << 7 | (quad & 4) << 14 | (quad & 8) << 21) * 0xffu);
+#pragma unroll
+            for (int j = 0; j < 2 * J; j++) {  // four dimensions of a token to four tokens of a dimension, over the lanes of the four tokens
+                const uint32_t p = __shfl_xor_sync(0xffffffffu, w[1][j], 8), z = __byte_perm(w[1][j], p, l0 ? 0x3715 : 0x6240);
+                const uint32_t p2 = __shfl_xor_sync(0xffffffffu, z, 16), y = __byte_perm(z, p2, l1 ? 0x3276 : 0x5410);
+                uint32_t* const to = (uint32_t*)(image + IMAGE + value_at(4 * warp, d8 + 64 * (j >> 1) + 4 * (j & 1) + 2 * l1 + l0));
+                *to = keep ? (*to & keep) | (y & ~keep) : y;
+            }
         }
-        if (tid == 0) *header = make_uint2(__float_as_uint(scale), bad);
+        if (tid == 0) *(uint4*)unit = make_uint4(__float_as_uint(scale[0]), bad[0], __float_as_uint(scale[1]), bad[1]);
         __syncthreads();
-        for (int o = tid; o < WORDS; o += KV_THREADS) ((uint4*)bytes)[o] = ((const uint4*)image)[o];
+        for (int o = tid; o < 2 * WORDS; o += KV_THREADS) ((uint4*)(unit + KV8_HEADER))[o] = ((const uint4*)image)[o];
     }
 }
 
@@ -386,14 +397,14 @@ cudaError_t append_t(const Kv8Cache& c, const Kv8Seqs& s, const Kv8Rows& x, bool
     const size_t unit = 4 * sizeof(T);
     const size_t places = (uintptr_t)x.k | (uintptr_t)x.v | x.rs * sizeof(T) | x.hs * sizeof(T);
     const int aligned = (places & (unit - 1)) == 0, wide = (places & 15) == 0;
-    // 8 KV heads of 128, us, a warp / a CTA a block: a sequence's one row 2.5 / 2.9, four 3.2 / 3.1, eight 5.4 / 3.2; 64 sequences 2.9 / 6.9, 5.1 / 6.9, 8.8 / 7.0; 256 sequences of
-    // eight 16.8 / 20.9.
-    if (s.max_rows <= FEW || (s.max_rows <= 2 * FEW && (size_t)s.n_seqs * c.nkv >= 1024)) {
+    // 8 KV heads of 128, us, a warp / a CTA a block: a sequence's one row 2.3 / 3.2, four 3.0 / 3.3; 64 sequences 2.8 / 5.4, 5.3 / 6.3; 256 sequences of one row 5.4 / 14.3, four
+    // 9.5 / 14.2, six 13.2 / 14.4, eight 16.8 / 14.3.
+    if (s.max_rows <= FEW) {
         const uint32_t units = 2 * tiles * c.nkv * s.n_seqs;
         return launch_k(append_few_kernel<HD, T>, dim3((units + 3) / 4), dim3(128), 0, st, pdl, c, s, x, tiles, units, keep_behind ? 1 : 0, aligned, status);
     }
-    tiles = std::min<uint32_t>(tiles, std::max<uint32_t>(1, (uint32_t)(KV_WAVE * 148 / (2 * (size_t)c.nkv * s.n_seqs))));
-    return launch_k(append_kernel<HD, T>, dim3(2 * tiles * c.nkv * s.n_seqs), dim3(KV_THREADS), 0, st, pdl, c, s, x, tiles, keep_behind ? 1 : 0, wide, status);
+    tiles = std::min<uint32_t>(tiles, std::max<uint32_t>(1, (uint32_t)(KV_WAVE * 148 / ((size_t)c.nkv * s.n_seqs))));
+    return launch_k(append_kernel<HD, T>, dim3(tiles * c.nkv * s.n_seqs), dim3(KV_THREADS), 0, st, pdl, c, s, x, tiles, keep_behind ? 1 : 0, wide, status);
 }
 template <int HD>
 cudaError_t append_hd(const Kv8Cache& c, const Kv8Seqs& s, const Kv8Rows& x, bool keep_behind, uint32_t* status, cudaStream_t st, bool pdl) {
