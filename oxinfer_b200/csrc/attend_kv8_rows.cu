@@ -678,7 +678,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) attend_kv8_rows_kernel(const __
 #pragma unroll
                     for (int e = 0; e < 8; e++) {
                         if constexpr (std::is_same<T, __half>::value) o[e] = __float2half_rn(v[e] * inv);
-                        else if constexpr (sizeof(T) == 2) o[e] = __float2bfloat16_rn(v[e] * inv);
+                        else o[e] = (T)(v[e] * inv);  // (to nearest even)
                     }
                     *(uint4*)((T*)a.out + (size_t)(seq.r0 + tk) * a.out_stride + (size_t)(head * a.G + (rr - tk * a.G)) * HD + 8 * d8) = *(const uint4*)o;
                 }
