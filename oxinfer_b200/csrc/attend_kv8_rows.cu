@@ -34,7 +34,7 @@ using namespace kv8;
 
 namespace {
 
-constexpr int KT_THREADS = 512, KT_TILE = 128, KT_BLOCKS = KT_TILE / (int)KV8_BLOCK;
+constexpr int KT_THREADS = 768, KT_TILE = 128, KT_BLOCKS = KT_TILE / (int)KV8_BLOCK;
 constexpr uint32_t KT_TMEM_COLS = 512;
 // tanh(z) / z by powers of z^2
 constexpr float K0 = 0.999999464f, K1 = -0.333283484f, K2 = 0.132598311f, K3 = -0.0500801913f, K4 = 0.0129507277f;
@@ -42,11 +42,11 @@ constexpr float LAZY_BITS = 8.0f;  // the sums are brought to a new largest scor
 constexpr float V_ONE = 32.0f;  // the largest scale of values as it enters the f16 values: 1152 of it has to be an f16, too
 
 struct __align__(16) KtShared {
-    float qf[2 * KT_TILE];                  // what the rows' scores are multiplied by, and in the end what their sums are
+    float told[2][2 * KT_TILE];             // what the two warps of a row tell one another, a half of the keys each; in the beginning [0] is what the rows' scores are multiplied by
     // of a tile's blocks, four tiles in turn: a tile's are written once the scores of two tiles ahead have been made, so the softmax of three tiles ahead is done
     float k_scale[4][KT_BLOCKS];
     uint32_t bad[4][KT_BLOCKS];             // tokens that count as NaN
-    uint64_t k_full[2], v_full[2], k_empty[2], v_empty[2], q_full, s_full[2], p_full[2][2], o_full, u_full[KT_BLOCKS], u_empty[KT_BLOCKS], turn[2];
+    uint64_t k_full[2], v_full[2], k_empty[2], v_empty[2], q_full, s_full[2], p_full[2][2], o_full, u_full[KT_BLOCKS], u_empty[KT_BLOCKS], turn[2], pair[2][4];
     uint32_t tmem_base, v_top, item_seq, item_block;
     volatile uint32_t abort_flag;
 };
@@ -55,9 +55,10 @@ template <int HD>
 struct KtSizes {
     static constexpr uint32_t TILE = KT_TILE * HD * 2, UNIT = unit_bytes(HD);
     static constexpr uint32_t Q = 0, K = 2 * TILE, V = 4 * TILE, RING = 6 * TILE;
-    static constexpr size_t NEED = RING + KT_BLOCKS * UNIT + 1024;
+    static constexpr uint32_t SHARED = RING + KT_BLOCKS * UNIT;
+    static constexpr size_t NEED = SHARED + sizeof(KtShared);
     static constexpr size_t BYTES = NEED < TMEM_512_SMEM ? TMEM_512_SMEM : NEED;  // (one CTA an SM: it takes all of the tensor memory)
-    static_assert(BYTES + sizeof(KtShared) <= 227 * 1024);
+    static_assert(BYTES <= 227 * 1024 && SHARED % alignof(KtShared) == 0);
 };
 
 struct KtArgs {
@@ -103,14 +104,20 @@ __device__ __forceinline__ void kt_ld32(uint32_t taddr, uint32_t (&v)[32]) {
           "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
         : "r"(taddr));
 }
-__device__ __forceinline__ void kt_st32(uint32_t taddr, const uint32_t (&v)[32]) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, "
-        "%21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
-        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]),
-        "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]),
-        "r"(v[29]), "r"(v[30]), "r"(v[31])
-        : "memory");
+__device__ __forceinline__ void kt_ld8(uint32_t taddr, uint32_t (&v)[8]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+                 : "r"(taddr));
+}
+__device__ __forceinline__ void kt_st8(uint32_t taddr, const uint32_t (&v)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]),
+                 "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
+}
+__device__ __forceinline__ void kt_st16(uint32_t taddr, const uint32_t (&v)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr), "r"(v[0]), "r"(v[1]),
+                 "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+                 : "memory");
 }
 __device__ __forceinline__ void kt_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void kt_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -180,10 +187,8 @@ template <int HD, bool SPECIAL, typename T>
 __global__ void __launch_bounds__(KT_THREADS, 1) attend_kv8_rows_kernel(const __grid_constant__ KtArgs a) {
     using L = KtSizes<HD>;
     constexpr uint32_t HALF = KT_TILE * 128, VHALF = HD * 128;  // 64 dimensions of all keys; 64 keys of all dimensions
-    extern __shared__ uint8_t smem_raw[];
-    uint8_t* const smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-    __shared__ KtShared shared;
-    KtShared* const sh = &shared;
+    extern __shared__ __align__(1024) uint8_t smem[];  // (the kernel has no other shared memory: tiles begin on the 1024 bytes that their swizzle needs)
+    KtShared* const sh = (KtShared*)(smem + L::SHARED);
     // (what the instructions' descriptors are made of is known to be the warp's: registers of the warp, no moves into them ahead of every instruction)
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     const uint32_t z = blockIdx.x % a.Z, unit_no = blockIdx.x / a.Z, head = unit_no % a.c.nkv, want = unit_no / a.c.nkv;
@@ -240,20 +245,21 @@ __global__ void __launch_bounds__(KT_THREADS, 1) attend_kv8_rows_kernel(const __
             mbar_init(&sh->k_empty[i], tiles);
             mbar_init(&sh->v_empty[i], tiles);
             mbar_init(&sh->s_full[i], 1);
-            mbar_init(&sh->p_full[i][0], 4);
-            mbar_init(&sh->p_full[i][1], 4);
+            mbar_init(&sh->p_full[i][0], 8);
+            mbar_init(&sh->p_full[i][1], 8);
+            for (int q = 0; q < 4; q++) mbar_init(&sh->pair[i][q], 2);
         }
         for (int i = 0; i < KT_BLOCKS; i++) {
             mbar_init(&sh->u_full[i], 1);
             mbar_init(&sh->u_empty[i], 1);
         }
-        mbar_init(&sh->q_full, 8);
+        mbar_init(&sh->q_full, 16);
         mbar_init(&sh->o_full, 2);
-        mbar_init(&sh->turn[0], 4);
-        mbar_init(&sh->turn[1], 4);
+        mbar_init(&sh->turn[0], 8);
+        mbar_init(&sh->turn[1], 8);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 8) {
+    if (warp == 16) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh->tmem_base)), "r"(KT_TMEM_COLS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -262,16 +268,16 @@ __global__ void __launch_bounds__(KT_THREADS, 1) attend_kv8_rows_kernel(const __
     tc_fence_after();
     const uint32_t tmem = __shfl_sync(0xffffffffu, sh->tmem_base, 0);
 
-    // 512 threads are launched with 128 registers each: 256 x 208 + 128 x 40 + 128 x 56 of them.
-    if (warp >= 12) {
+    // 768 threads are launched with 80 registers each: 512 x 96 + 128 x 40 + 128 x 56 of them.
+    if (warp >= 20) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 56;" ::: "memory");
         // ---------------- bytes to f16: a warp for each block of a tile ----------------
-        const uint32_t bq = warp - 12, t = lane & 3, n0 = (lane >> 2) & 1, u2 = lane >> 3;
+        const uint32_t bq = warp - 20, t = lane & 3, n0 = (lane >> 2) & 1, u2 = lane >> 3;
         const __half2 one = __float2half2_rn(1.0f), off = __float2half2_rn(-1152.0f);
         {  // the largest scale of values that the rows may see
             uint32_t top = 0;
 #pragma unroll 4
-            for (uint32_t b = b_beg + tid - 384; b < b_end; b += 128) {
+            for (uint32_t b = b_beg + tid - 640; b < b_end; b += 128) {
                 const int id = block_of(a.c, a.sq, s, b, a.status);
                 const float v = ((const Header*)(a.c.units + ((size_t)max(id, 0) * a.c.nkv + head) * L::UNIT))->v_scale;
                 top = max(top, __float_as_uint(fmaxf(v, 0.0f)));
@@ -349,9 +355,9 @@ __global__ void __launch_bounds__(KT_THREADS, 1) attend_kv8_rows_kernel(const __
                 if (there) mbar_arrive(&sh->u_empty[bq]);
             }
         }
-    } else if (warp >= 8) {
+    } else if (warp >= 16) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 40;" ::: "memory");
-        if (warp == 10) {
+        if (warp == 18) {
             // ---------------- units: block q of a tile into place q ----------------
             int ids = 0;
             bool ok = true;
@@ -374,11 +380,11 @@ __global__ void __launch_bounds__(KT_THREADS, 1) attend_kv8_rows_kernel(const __
                     kt_wait(&sh->u_full[q], before & 1, sh, a.status, false);
                 }
             }
-        } else if (warp < 10) {
+        } else if (warp < 18) {
             // ---------------- instructions ----------------
             constexpr uint32_t idesc_qk = (1u << 4) | ((KT_TILE >> 3) << 17) | ((KT_TILE >> 4) << 24);
             constexpr uint32_t idesc_pv = (1u << 4) | ((HD >> 3) << 17) | ((KT_TILE >> 4) << 24);
-            const int w = warp - 8;
+            const int w = warp - 16;
             const uint64_t qd = smem_desc_sw128(smem_u32(smem + L::Q) + w * L::TILE), kd = smem_desc_sw128(smem_u32(smem + L::K)), vd = smem_desc_sw128(smem_u32(smem + L::V));
             const uint32_t s_at = tmem + w * KT_TILE, o_at = tmem + 2 * KT_TILE + w * HD;
             auto scores = [&](int slot) {
@@ -424,32 +430,33 @@ __global__ void __launch_bounds__(KT_THREADS, 1) attend_kv8_rows_kernel(const __
             if (n > 0 && w < tiles && !ok) kt_wait(&sh->o_full, 0, sh, a.status, false);
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;" ::: "memory");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 96;" ::: "memory");
         // ---------------- softmax ----------------
-        const int w = warp >> 2;
+        // two warps a row: 0 .. 7 have the first and the third block of a tile's keys, 8 .. 15 the others
+        const int w = (warp >> 2) & 1, hc = warp >> 3;
         const bool live = w < tiles;
         {  // the tile's queries as f16: a warp's 32 rows, a row's values over the lanes
             auto from = [&](uint32_t in_warp, uint32_t d) {
-                const uint32_t r = min(r_block + w * KT_TILE + (warp & 3) * 32 + in_warp, rows - 1), tok = kt_token(a, r);
+                const uint32_t r = min(r_block + w * KT_TILE + (warp & 3) * 32 + hc * 16 + in_warp, rows - 1), tok = kt_token(a, r);
                 return (const T*)a.q + (size_t)(seq.r0 + tok) * a.q_stride + (size_t)(head * a.G + (r - tok * a.G)) * HD + d;
             };
             auto factor = [&](uint32_t row, uint32_t bits, bool first) {  // of a row whose largest magnitude has those bits (what is not finite is above all else)
                 const int ex = min(max((int)(bits >> 23), 40), 254) - 127;
-                if (first) sh->qf[w * KT_TILE + row] = (bits >= 0x7f800000u ? NAN : pow2(ex)) * a.c2;
+                if (first) sh->told[0][w * KT_TILE + row] = (bits >= 0x7f800000u ? NAN : pow2(ex)) * a.c2;
                 return pow2(-ex) * a.q_sign;
             };
             if (sizeof(T) == 2 && a.wide) {  // eight a lane: half the instructions of the form below
-                constexpr int PER = HD / 8, ROWS = 32 / PER, FLIGHT = 8;
+                constexpr int PER = HD / 8, ROWS = 32 / PER, FLIGHT = 16 / ROWS;
                 const uint32_t d8 = (uint32_t)(lane % PER);
                 uint8_t* const to = smem + L::Q + w * L::TILE + (d8 >> 3) * HALF;
 #pragma unroll 1
-                for (int i0 = 0; i0 < 32; i0 += FLIGHT * ROWS) {
+                for (int i0 = 0; i0 < 16; i0 += FLIGHT * ROWS) {
                     uint4 eight[FLIGHT];
 #pragma unroll
                     for (int i = 0; i < FLIGHT; i++) eight[i] = *(const uint4*)from((uint32_t)(i0 + i * ROWS + lane / PER), 8 * d8);
 #pragma unroll
                     for (int i = 0; i < FLIGHT; i++) {
-                        const uint32_t row = (uint32_t)((warp & 3) * 32 + i0 + i * ROWS + lane / PER);
+                        const uint32_t row = (uint32_t)((warp & 3) * 32 + hc * 16 + i0 + i * ROWS + lane / PER);
                         const T* const v = (const T*)&eight[i];
                         float x[8];
                         uint32_t bits = 0;
@@ -469,13 +476,13 @@ __global__ void __launch_bounds__(KT_THREADS, 1) attend_kv8_rows_kernel(const __
                 constexpr int PER = HD / 4, ROWS = 32 / PER, FLIGHT = 8;
                 const uint32_t d4 = (uint32_t)(lane % PER), half = d4 >> 4, chunk = (d4 & 15) >> 1, in = (d4 & 1) * 8;
 #pragma unroll 1
-                for (int i0 = 0; i0 < 32; i0 += FLIGHT * ROWS) {
+                for (int i0 = 0; i0 < 16; i0 += FLIGHT * ROWS) {
                     float x[FLIGHT][4];
 #pragma unroll
                     for (int i = 0; i < FLIGHT; i++) load4(x[i], from((uint32_t)(i0 + i * ROWS + lane / PER), 4 * d4), a.aligned);
 #pragma unroll
                     for (int i = 0; i < FLIGHT; i++) {
-                        const uint32_t row = (uint32_t)((warp & 3) * 32 + i0 + i * ROWS + lane / PER);
+                        const uint32_t row = (uint32_t)((warp & 3) * 32 + hc * 16 + i0 + i * ROWS + lane / PER);
                         uint32_t bits = 0;
 #pragma unroll
                         for (int e = 0; e < 4; e++) bits = max(bits, __float_as_uint(x[i][e]) & 0x7fffffffu);
@@ -496,28 +503,35 @@ __global__ void __launch_bounds__(KT_THREADS, 1) attend_kv8_rows_kernel(const __
         const uint32_t tile_end = seq.start + kt_token(a, min(r_block + w * KT_TILE + KT_TILE - 1, rows - 1));       // and its last
         const uint32_t see_to = max(qp + 1, prefix), my_lo = first_key(qp);                                           // keys my_lo .. see_to - 1
         const uint32_t all_to = max(tile_qp + 1, prefix), all_from = first_key(tile_end);
-        const float qf = sh->qf[w * KT_TILE + row];
+        bool ok = __all_sync(0xffffffffu, kt_wait(&sh->q_full, 0, sh, a.status));
+        const float qf = sh->told[0][w * KT_TILE + row];
+        // Both warps of a row: false when the CTA gives up. step: how often they have met.
+        auto meet = [&](int step) {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh->pair[w][warp & 3]);
+            return (bool)__all_sync(0xffffffffu, kt_wait(&sh->pair[w][warp & 3], (uint32_t)(step & 1), sh, a.status));
+        };
+        ok = ok && meet(0);
         const float slope = SPECIAL && a.slopes ? a.slopes[head * a.G + (r - tok * a.G)] * 1.44269504f : 0.0f;
         const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16, s_at = tmem + lane_base + w * KT_TILE, o_at = tmem + lane_base + 2 * KT_TILE + w * HD;
         float m = -INFINITY, l = 0.0f;
-        bool ok = true;
-        for (int i = 0; i < n && live; i++) {
+        for (int i = 0; i < n && live && ok; i++) {
             ok = __all_sync(0xffffffffu, kt_wait(&sh->s_full[w], (uint32_t)(i & 1), sh, a.status));
             if (!ok) break;
             tc_fence_after();
-            uint32_t v[4][32];
+            uint32_t v[2][32];
 #pragma unroll
-            for (int h = 0; h < 4; h++) kt_ld32(s_at + 32 * h, v[h]);
-            const float4 ks = *(const float4*)sh->k_scale[i & 3];
-            const uint4 bad = *(const uint4*)sh->bad[i & 3];
+            for (int h = 0; h < 2; h++) kt_ld32(s_at + 64 * h + 32 * hc, v[h]);
+            const float ks[2] = {sh->k_scale[i & 3][hc], sh->k_scale[i & 3][2 + hc]};
+            const uint32_t bad[2] = {sh->bad[i & 3][hc], sh->bad[i & 3][2 + hc]};
             // (not zero: a key that is not seen stays at -inf)
-            float f[4] = {fmaxf(qf * ks.x, 1e-37f), fmaxf(qf * ks.y, 1e-37f), fmaxf(qf * ks.z, 1e-37f), fmaxf(qf * ks.w, 1e-37f)};
-            if (qf != qf) f[0] = f[1] = f[2] = f[3] = qf;
+            float f[2] = {fmaxf(qf * ks[0], 1e-37f), fmaxf(qf * ks[1], 1e-37f)};
+            if (qf != qf) f[0] = f[1] = qf;
             kt_ld_wait();
-            const uint32_t j0 = (b_0 + i * KT_BLOCKS) * KV8_BLOCK;
+            const uint32_t j0 = (b_0 + i * KT_BLOCKS + hc) * KV8_BLOCK;  // the warp's first key; its second block is 64 behind
             if (SPECIAL) {
 #pragma unroll
-                for (int h = 0; h < 4; h++) {
+                for (int h = 0; h < 2; h++) {
                     const float fh = f[h];
                     if (a.cap2 > 0.0f) {
                         // cap tanh(z), z = score / cap: by an odd polynomial fitted at Chebyshev nodes of z^2, off by 4.4e-7 up to |z| = 0.75, with the powers of what
@@ -550,7 +564,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) attend_kv8_rows_kernel(const __
                         f[h] = 1.0f;
                     }
                     if (a.slopes) {
-                        const float at = slope * (float)((int)(j0 + 32 * h) - (int)qp), g = f[h];
+                        const float at = slope * (float)((int)(j0 + 64 * h) - (int)qp), g = f[h];
                         const float2 g2 = make_float2(g, g), s2 = make_float2(slope, slope), at2 = make_float2(at, at);
 #pragma unroll
                         for (int e = 0; e < 32; e += 2) {
@@ -563,48 +577,53 @@ __global__ void __launch_bounds__(KT_THREADS, 1) attend_kv8_rows_kernel(const __
                     }
                 }
             }
-            if ((bad.x | bad.y | bad.z | bad.w) != 0) {
-                const uint32_t bb[4] = {bad.x, bad.y, bad.z, bad.w};
+            if ((bad[0] | bad[1]) != 0) {
 #pragma unroll
-                for (int h = 0; h < 4; h++)
+                for (int h = 0; h < 2; h++)
 #pragma unroll
                     for (int e = 0; e < 32; e++)
-                        if (bb[h] & (1u << kt_tok(e))) v[h][e] = 0x7fffffffu;
+                        if (bad[h] & (1u << kt_tok(e))) v[h][e] = 0x7fffffffu;
             }
-            if (j0 + KT_TILE > all_to || j0 < all_from) {  // some row does not see some key
-                const uint32_t hi = see_to > j0 ? min(see_to - j0, (uint32_t)KT_TILE) : 0u, from = my_lo > j0 ? my_lo - j0 : 0u;  // keys from .. hi - 1 of the tile
-                auto below = [](uint32_t n, int h) { return n >= 32u * h + 32 ? 0xffffffffu : n <= 32u * h ? 0u : (1u << (n - 32 * h)) - 1; };  // a bit per key below n
+            if (j0 + 96 > all_to || j0 < all_from) {  // some row does not see some key
+                auto below = [](uint32_t n, uint32_t from) { return n >= from + 32 ? 0xffffffffu : n <= from ? 0u : (1u << (n - from)) - 1; };  // a bit per key of a block below n
 #pragma unroll
-                for (int h = 0; h < 4; h++) {
-                    const uint32_t seen = below(hi, h) & ~below(from, h);
+                for (int h = 0; h < 2; h++) {
+                    const uint32_t seen = below(see_to, j0 + 64 * h) & ~below(my_lo, j0 + 64 * h);
 #pragma unroll
                     for (int e = 0; e < 32; e++)
                         if (!(seen & (1u << kt_tok(e)))) v[h][e] = 0xff800000u;
                 }
             }
-            float mx[4];
+            float mx[2];
 #pragma unroll
-            for (int h = 0; h < 4; h++) {
+            for (int h = 0; h < 2; h++) {
                 mx[h] = fmaxf(__uint_as_float(v[h][0]), __uint_as_float(v[h][1]));
 #pragma unroll
                 for (int e = 2; e < 32; e += 2) mx[h] = max3(mx[h], __uint_as_float(v[h][e]), __uint_as_float(v[h][e + 1]));
                 mx[h] *= f[h];
             }
-            const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+            // the row's other half (which has its scores, too, by then: probabilities take their place)
+            sh->told[hc][w * KT_TILE + row] = fmaxf(mx[0], mx[1]);  // (the step ahead's has been read: its probabilities have been multiplied)
+            tc_fence_before();
+            ok = meet(i + 1);
+            if (!ok) break;
+            tc_fence_after();
+            const float top = fmaxf(sh->told[0][w * KT_TILE + row], sh->told[1][w * KT_TILE + row]);
             if (i == 0) {
                 m = top;
             } else if (__any_sync(0xffffffffu, top > m + LAZY_BITS)) {
                 const float mn = fmaxf(m, top), g = m == -INFINITY ? 0.0f : kt_exp2(m - mn);
                 m = mn;
                 l *= g;
-#pragma unroll
-                for (int h = 0; h < HD / 32; h++) {
-                    uint32_t o[32];
-                    kt_ld32(o_at + 32 * h, o);
+#pragma unroll 1
+                for (int h = 0; h < HD / 16; h++) {  // (the warp's half of the dimensions, eight at a time: its scores are in registers)
+                    uint32_t o[8];
+                    const uint32_t at = o_at + hc * (HD / 2) + 8 * h;
+                    kt_ld8(at, o);
                     kt_ld_wait();
 #pragma unroll
-                    for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * g);
-                    kt_st32(o_at + 32 * h, o);
+                    for (int e = 0; e < 8; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * g);
+                    kt_st8(at, o);
                 }
             }
             const float base = m == -INFINITY ? 0.0f : -m;
@@ -615,17 +634,16 @@ __global__ void __launch_bounds__(KT_THREADS, 1) attend_kv8_rows_kernel(const __
             }
 #pragma unroll
             for (int h = 0; h < 2; h++) {
-                uint32_t pk[32];
+                uint32_t pk[16];
 #pragma unroll
-                for (int e = 0; e < 32; e++) {
-                    const uint32_t* at = &v[2 * h + (e >> 4)][2 * (e & 15)];
-                    const float g = f[2 * h + (e >> 4)];
-                    float2 x = fma2(make_float2(__uint_as_float(at[0]), __uint_as_float(at[1])), make_float2(g, g), make_float2(base, base));
+                for (int e = 0; e < 16; e++) {
+                    const float g = f[h];
+                    float2 x = fma2(make_float2(__uint_as_float(v[h][2 * e]), __uint_as_float(v[h][2 * e + 1])), make_float2(g, g), make_float2(base, base));
                     x = make_float2(kt_exp2(x.x), kt_exp2(x.y));
                     part[e & 1] = add2(part[e & 1], x);
                     pk[e] = kt_pack(x.x, x.y);
                 }
-                kt_st32(s_at + 32 * h, pk);
+                kt_st16(s_at + 32 * h + 16 * hc, pk);
                 if (h && tiles == 2 && lane == 0) mbar_arrive(&sh->turn[w ^ 1]);
                 kt_st_wait();
                 tc_fence_before();
@@ -642,7 +660,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) attend_kv8_rows_kernel(const __
             float4* const dst = (float4*)(smem + (size_t)(w * KT_TILE + row) * HD * 4);
             const float one = __uint_as_float(*(volatile uint32_t*)&sh->v_top) * (1.0f / V_ONE);
 #pragma unroll
-            for (int h = 0; h < HD / 32; h++) {
+            for (int h = hc * (HD / 64); h < (hc + 1) * (HD / 64); h++) {
                 uint32_t o[32];
                 kt_ld32(o_at + 32 * h, o);
                 kt_ld_wait();
@@ -650,11 +668,15 @@ __global__ void __launch_bounds__(KT_THREADS, 1) attend_kv8_rows_kernel(const __
 #pragma unroll
                 for (int e = 0; e < 8; e++) dst[(8 * h + e) ^ (row & 7)] = make_float4(f(4 * e), f(4 * e + 1), f(4 * e + 2), f(4 * e + 3));
             }
-            ml[w * KT_TILE + row] = make_float2(m, a.Z > 1 ? l : l > 0.0f || l != l ? 1.0f / l : 0.0f);
+            sh->told[hc][w * KT_TILE + row] = l;
+            if (meet(n + 1) && hc == 0) {
+                l += sh->told[1][w * KT_TILE + row];
+                ml[w * KT_TILE + row] = make_float2(m, a.Z > 1 ? l : l > 0.0f || l != l ? 1.0f / l : 0.0f);
+            }
         }
         __syncwarp();
         if (a.Z > 1) cluster_sync_all();
-        else asm volatile("bar.sync 1, 256;" ::: "memory");
+        else asm volatile("bar.sync 1, 512;" ::: "memory");
         // ---------------- the rows out: CTA z every Z-th run of them ----------------
         if (!sh->abort_flag) {
             constexpr int PER = HD / 4, ROWS = 32 / PER;
@@ -669,7 +691,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) attend_kv8_rows_kernel(const __
                 constexpr uint32_t PER8 = HD / 8, ROWS8 = 32 / PER8;
                 const uint32_t d8 = (uint32_t)lane % PER8;
 #pragma unroll 4
-                for (uint32_t at = warp * ROWS8 + lane / PER8; at < count; at += 8 * ROWS8) {
+                for (uint32_t at = warp * ROWS8 + lane / PER8; at < count; at += 16 * ROWS8) {
                     const float4* const row = (const float4*)(smem + (size_t)at * HD * 4);
                     const float4 x = row[(2 * d8) ^ (at & 7)], y = row[(2 * d8 + 1) ^ (at & 7)];
                     const float inv = ml[at].y, v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
@@ -684,9 +706,9 @@ __global__ void __launch_bounds__(KT_THREADS, 1) attend_kv8_rows_kernel(const __
                 }
             } else if (a.Z == 1) {
 #pragma unroll 4
-                for (uint32_t at = warp * ROWS + lane / PER; at < count; at += 8 * ROWS) put(at, *from_of(at), ml[at].y);
+                for (uint32_t at = warp * ROWS + lane / PER; at < count; at += 16 * ROWS) put(at, *from_of(at), ml[at].y);
             } else {
-                for (uint32_t at = (z * 8 + warp) * ROWS + lane / PER; at < count; at += a.Z * 8 * ROWS) {
+                for (uint32_t at = (z * 16 + warp) * ROWS + lane / PER; at < count; at += a.Z * 16 * ROWS) {
                     const float4* const from = from_of(at);
                     float4 o;
                     float den;
@@ -715,12 +737,12 @@ __global__ void __launch_bounds__(KT_THREADS, 1) attend_kv8_rows_kernel(const __
         }
     }
     if (a.Z > 1) {  // no CTA leaves while another reads its sums
-        if (warp >= 8) cluster_sync_all();
+        if (warp >= 16) cluster_sync_all();
         cluster_sync_all();
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 8) {
+    if (warp == 16) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(KT_TMEM_COLS) : "memory");
     }
