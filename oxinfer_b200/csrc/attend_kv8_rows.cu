@@ -46,7 +46,7 @@ struct __align__(16) KtShared {
     // of a tile's blocks, four tiles in turn: a tile's are written once the scores of two tiles ahead have been made, so the softmax of three tiles ahead is done
     float k_scale[4][KT_BLOCKS];
     uint32_t bad[4][KT_BLOCKS];             // tokens that count as NaN
-    uint64_t k_full[2], v_full[2], k_empty[2], v_empty[2], q_full, s_full[2], p_full[2][2], o_full, u_full[KT_BLOCKS], u_empty[KT_BLOCKS], turn[2], pair[2][4];
+    uint64_t k_full[2], v_full[2], k_empty[2], v_empty[2], q_full, s_full[2][2], s_free[2], p_full[2][2], o_full, u_full[KT_BLOCKS], u_empty[KT_BLOCKS], turn[2], pair[2][4];
     uint32_t tmem_base, v_top, item_seq, item_block;
     volatile uint32_t abort_flag;
 };
@@ -244,7 +244,9 @@ __global__ void __launch_bounds__(KT_THREADS, 1) attend_kv8_rows_kernel(const __
             mbar_init(&sh->v_full[i], 4);
             mbar_init(&sh->k_empty[i], tiles);
             mbar_init(&sh->v_empty[i], tiles);
-            mbar_init(&sh->s_full[i], 1);
+            mbar_init(&sh->s_full[i][0], 1);
+            mbar_init(&sh->s_full[i][1], 1);
+            mbar_init(&sh->s_free[i], 8);
             mbar_init(&sh->p_full[i][0], 8);
             mbar_init(&sh->p_full[i][1], 8);
             for (int q = 0; q < 4; q++) mbar_init(&sh->pair[i][q], 2);
@@ -382,21 +384,21 @@ __global__ void __launch_bounds__(KT_THREADS, 1) attend_kv8_rows_kernel(const __
             }
         } else if (warp < 18) {
             // ---------------- instructions ----------------
-            constexpr uint32_t idesc_qk = (1u << 4) | ((KT_TILE >> 3) << 17) | ((KT_TILE >> 4) << 24);
+            constexpr uint32_t idesc_qk = (1u << 4) | ((KT_TILE / 2 >> 3) << 17) | ((KT_TILE >> 4) << 24);
             constexpr uint32_t idesc_pv = (1u << 4) | ((HD >> 3) << 17) | ((KT_TILE >> 4) << 24);
             const int w = warp - 16;
             const uint64_t qd = smem_desc_sw128(smem_u32(smem + L::Q) + w * L::TILE), kd = smem_desc_sw128(smem_u32(smem + L::K)), vd = smem_desc_sw128(smem_u32(smem + L::V));
             const uint32_t s_at = tmem + w * KT_TILE, o_at = tmem + 2 * KT_TILE + w * HD;
-            auto scores = [&](int slot) {
+            auto scores = [&](int slot, int h) {  // of a half of a tile's keys
                 if (elect_one()) {
-                    const uint64_t k = kd + (slot * L::TILE >> 4);
+                    const uint64_t k = kd + ((slot * L::TILE + h * (HALF / 2)) >> 4);
 #pragma unroll
                     for (int kk = 0; kk < HD / 16; kk++) {
                         const uint32_t at = (uint32_t)(kk >> 2) * (HALF >> 4) + 2 * (kk & 3);
-                        mma_f16(s_at, qd + at, k + at, idesc_qk, kk > 0);
+                        mma_f16(s_at + 64 * h, qd + at, k + at, idesc_qk, kk > 0);
                     }
-                    mma_commit(&sh->s_full[w]);
-                    mma_commit(&sh->k_empty[slot]);
+                    mma_commit(&sh->s_full[w][h]);
+                    if (!h) mma_commit(&sh->k_empty[slot]);
                 }
                 __syncwarp();
             };
@@ -406,9 +408,17 @@ __global__ void __launch_bounds__(KT_THREADS, 1) attend_kv8_rows_kernel(const __
                 tc_fence_after();
                 return ok;
             };
-            if (ok && wait(&sh->q_full, 0) && wait(&sh->k_full[0], 0)) scores(0);
+            if (ok && wait(&sh->q_full, 0) && wait(&sh->k_full[0], 0)) {
+                scores(0, 1);
+                scores(0, 0);
+            }
             for (int i = 0; i < n && ok; i++) {
                 const int slot = i & 1, next = slot ^ 1;
+                // The next tile's second half of the keys while this one's exponentials are made: probabilities take the first half's place.
+                if (i + 1 < n) {
+                    if (!wait(&sh->s_free[w], (uint32_t)(i & 1)) || !wait(&sh->k_full[next], (uint32_t)(((i + 1) >> 1) & 1))) break;
+                    scores(next, 1);
+                }
                 if (!wait(&sh->v_full[slot], (uint32_t)((i >> 1) & 1))) break;
 #pragma unroll
                 for (int h = 0; h < 2; h++) {  // (the first half's products run under the second half's exponentials)
@@ -421,7 +431,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) attend_kv8_rows_kernel(const __
                     }
                     __syncwarp();
                 }
-                if (ok && i + 1 < n && wait(&sh->k_full[next], (uint32_t)(((i + 1) >> 1) & 1))) scores(next);
+                if (ok && i + 1 < n) scores(next, 0);
             }
             // (a share without keys: its sums, zeros, take the queries' place, which other warps may still be writing)
             if (n == 0) kt_wait(&sh->q_full, 0, sh, a.status);
@@ -516,22 +526,25 @@ __global__ void __launch_bounds__(KT_THREADS, 1) attend_kv8_rows_kernel(const __
         const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16, s_at = tmem + lane_base + w * KT_TILE, o_at = tmem + lane_base + 2 * KT_TILE + w * HD;
         float m = -INFINITY, l = 0.0f;
         for (int i = 0; i < n && live && ok; i++) {
-            ok = __all_sync(0xffffffffu, kt_wait(&sh->s_full[w], (uint32_t)(i & 1), sh, a.status));
-            if (!ok) break;
-            tc_fence_after();
             uint32_t v[2][32];
-#pragma unroll
-            for (int h = 0; h < 2; h++) kt_ld32(s_at + 64 * h + 32 * hc, v[h]);
-            const float ks[2] = {sh->k_scale[i & 3][hc], sh->k_scale[i & 3][2 + hc]};
-            const uint32_t bad[2] = {sh->bad[i & 3][hc], sh->bad[i & 3][2 + hc]};
-            // (not zero: a key that is not seen stays at -inf)
-            float f[2] = {fmaxf(qf * ks[0], 1e-37f), fmaxf(qf * ks[1], 1e-37f)};
-            if (qf != qf) f[0] = f[1] = qf;
-            kt_ld_wait();
+            float f[2], mx[2];
             const uint32_t j0 = (b_0 + i * KT_BLOCKS + hc) * KV8_BLOCK;  // the warp's first key; its second block is 64 behind
-            if (SPECIAL) {
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
+            auto take = [&](const int h) {  // a block's scores, as far as they go without the row's largest
+                ok = __all_sync(0xffffffffu, kt_wait(&sh->s_full[w][h], (uint32_t)(i & 1), sh, a.status));
+                if (!ok) return;
+                tc_fence_after();
+                kt_ld32(s_at + 64 * h + 32 * hc, v[h]);
+                const uint32_t bad = sh->bad[i & 3][2 * h + hc];
+                // (not zero: a key that is not seen stays at -inf)
+                f[h] = fmaxf(qf * sh->k_scale[i & 3][2 * h + hc], 1e-37f);
+                if (qf != qf) f[h] = qf;
+                kt_ld_wait();
+                if (!h) {  // both are in registers
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sh->s_free[w]);
+                }
+                if (SPECIAL) {
                     const float fh = f[h];
                     if (a.cap2 > 0.0f) {
                         // cap tanh(z), z = score / cap: by an odd polynomial fitted at Chebyshev nodes of z^2, off by 4.4e-7 up to |z| = 0.75, with the powers of what
@@ -576,32 +589,26 @@ __global__ void __launch_bounds__(KT_THREADS, 1) attend_kv8_rows_kernel(const __
                         f[h] = 1.0f;
                     }
                 }
-            }
-            if ((bad[0] | bad[1]) != 0) {
-#pragma unroll
-                for (int h = 0; h < 2; h++)
+                if (bad) {
 #pragma unroll
                     for (int e = 0; e < 32; e++)
-                        if (bad[h] & (1u << kt_tok(e))) v[h][e] = 0x7fffffffu;
-            }
-            if (j0 + 96 > all_to || j0 < all_from) {  // some row does not see some key
-                auto below = [](uint32_t n, uint32_t from) { return n >= from + 32 ? 0xffffffffu : n <= from ? 0u : (1u << (n - from)) - 1; };  // a bit per key of a block below n
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
+                        if (bad & (1u << kt_tok(e))) v[h][e] = 0x7fffffffu;
+                }
+                if (j0 + 64 * h + 32 > all_to || j0 + 64 * h < all_from) {  // some row does not see some key
+                    auto below = [](uint32_t n, uint32_t from) { return n >= from + 32 ? 0xffffffffu : n <= from ? 0u : (1u << (n - from)) - 1; };  // a bit per key of the block below n
                     const uint32_t seen = below(see_to, j0 + 64 * h) & ~below(my_lo, j0 + 64 * h);
 #pragma unroll
                     for (int e = 0; e < 32; e++)
                         if (!(seen & (1u << kt_tok(e)))) v[h][e] = 0xff800000u;
                 }
-            }
-            float mx[2];
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
                 mx[h] = fmaxf(__uint_as_float(v[h][0]), __uint_as_float(v[h][1]));
 #pragma unroll
                 for (int e = 2; e < 32; e += 2) mx[h] = max3(mx[h], __uint_as_float(v[h][e]), __uint_as_float(v[h][e + 1]));
                 mx[h] *= f[h];
-            }
+            };
+            take(1);
+            if (ok) take(0);
+            if (!ok) break;
             // the row's other half (which has its scores, too, by then: probabilities take their place)
             sh->told[hc][w * KT_TILE + row] = fmaxf(mx[0], mx[1]);  // (the step ahead's has been read: its probabilities have been multiplied)
             tc_fence_before();
