@@ -1,25 +1,26 @@
-// Attention over the 8-bit cache for many rows of a sequence on tcgen05: S = Q K^T and O += P V with f16 operands and f32 sums in tensor memory, softmax by a
-// thread a row (attend_rows.cu has the form for f16 caches). The integers are exact as f16; a block's scale of keys multiplies its 32 columns of scores, a
+// Attention over the 8-bit cache for many rows of a sequence on tcgen05: S = Q K^T and O += P V with f16 operands and f32 sums in tensor memory, softmax by two
+// threads a row (attend_rows.cu has the form for f16 caches). The integers are exact as f16; a block's scale of keys multiplies its 32 columns of scores, a
 // block's scale of values, over the largest that the CTA's rows see, goes into the f16 values (a power of two, exact down to 2^-29 of the largest, zero below).
 // Queries are rounded to f16 after a power of two that brings each row's largest to 1 .. 2, probabilities to f16.
 //
 // A CTA takes 256 rows of a KV head (query heads token by token, two tiles of 128) and key tiles of 128, four blocks:
-//   warps 0..3, 4..7 : a tile's softmax and its rows out;
-//   warps 8, 9       : issue a tile's instructions;
-//   warp 10          : copies the blocks' units as they lie in the cache (bulk copies), a place for each block of a tile;
-//   warps 12..15     : expand them, a warp a block: bytes to f16, into swizzled tiles, keys as rows, values as rows of a dimension with the keys along them. Key r of a block in
-//                      both is token 16 (r / 4 % 2) + 4 (r / 8) + r % 4: eight keys of a dimension are eight bytes of a lane's word, one store of 16 bytes.
+//   warps 0..15  : softmax, two warps a row, a thread each: 0..3 and 4..7 have the first and the third block of the two tiles' rows, 8..15 the others; and the rows out;
+//   warps 16, 17 : issue a tile's instructions;
+//   warp 18      : copies the blocks' units as they lie in the cache (bulk copies), a place for each block of a tile;
+//   warps 20..23 : expand them, a warp a block: bytes to f16, into swizzled tiles, keys as rows, values as rows of a dimension with the keys along them. Key r of a block in
+//                  both is token 16 (r / 4 % 2) + 4 (r / 8) + r % 4: eight keys of a dimension are eight bytes of a lane's word, one store of 16 bytes.
 // Expanded tiles are two slots deep, so the next tile is expanded under the current one's products. A warp's reads and its stores of 16 bytes meet no bank
-// twice. Few rows over many keys: Z CTAs of a cluster take a share of the key tiles each, and add their sums through shared memory.
+// twice. Probabilities take the place of the first half of a tile's scores; the next tile's second half is multiplied, and taken in, while they are still at work. Few rows over
+// many keys: Z CTAs of a cluster take a share of the key tiles each, and add their sums through shared memory.
 //
-// What bounds it: a tile's exponentials, 1024 cycles of the exponential unit for each of the two row tiles, take a warp a scheduler 1750; the row tiles take
-// turns at them (left to themselves they meet there, and the tensor cores idle while both wait for products: 132 us instead of 115), so a tile of keys takes
-// 3700 cycles, of which the tensor cores work 2048. 2048 tokens of 32 heads over 8 KV heads of 128 behind 2048 more (103 GFLOP): 106 us, 970 TFLOP/s; with a
-// cap, whose polynomial is as much work again for those warps, 187 us. On mma.sync (attend_kv8.cu) 741 and 940. Steps: bytes expanded by four warps a
-// block and everyone in step 164 us, a warp a block 142, descriptors in the warp's registers and places by turned bits 132, turns 115. Short prompts (five of 185 to
-// 542 tokens with 12 heads 27.8 us, half of it in the tiles) pay for the CTA's start: the largest scale of values is looked for by the warps that expand, while the others
-// take in the queries, sixteen rows in flight (33 us before; the same rows four at a time, fetched one step ahead, 29.4)
-// with eight values a lane. What goes into the exponentials made ahead of a tile's turn and their sums behind it: no gain.
+// What bounds it: a softmax warp's chain for a tile of keys, 3700 cycles without a cap (scores out of tensor memory and their largest 830, the row's two warps' meeting and the turn 870,
+// exponentials 1330 of which the exponential unit needs 1024, the rest waits for products), 5600 with one. The row tiles take turns at the exponentials: left to themselves they
+// meet there, and the tensor cores, 2048 cycles of 3700, idle while both wait for products (136 us instead of 110, turns handed on at half of them 119). 2048 tokens of 32 heads over 8 KV heads
+// of 128 behind 2048 more (103 GFLOP): 110 us, 940 TFLOP/s; with a cap 170 us. On mma.sync (attend_kv8.cu) 741 and 940. Steps, without / with a cap: bytes expanded by four
+// warps a block and everyone in step 164 us, a warp a block 142, descriptors in the warp's registers and places by turned bits 132, turns 115, a shorter start 106 / 187, two
+// warps a row 120 / 181, each with a block of both halves of the keys 110 / 170. Short prompts (five of 185 to 542 tokens with 12 heads 25.3 us, half of it in the
+// tiles) pay for the CTA's start: the largest scale of values is looked for by the warps that expand, while the others take in the queries, eight values a lane (33 us before; one warp
+// a row 27.8). No gain: what goes into the exponentials made ahead of a tile's turn, their sums behind it; the two warps of a row at a barrier of the hardware's (110 -> 109.4).
 #include <cfloat>
 #include <type_traits>
 
@@ -445,7 +446,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) attend_kv8_rows_kernel(const __
         // two warps a row: 0 .. 7 have the first and the third block of a tile's keys, 8 .. 15 the others
         const int w = (warp >> 2) & 1, hc = warp >> 3;
         const bool live = w < tiles;
-        {  // the tile's queries as f16: a warp's 32 rows, a row's values over the lanes
+        {  // the tile's queries as f16: sixteen rows a warp, a row's values over the lanes
             auto from = [&](uint32_t in_warp, uint32_t d) {
                 const uint32_t r = min(r_block + w * KT_TILE + (warp & 3) * 32 + hc * 16 + in_warp, rows - 1), tok = kt_token(a, r);
                 return (const T*)a.q + (size_t)(seq.r0 + tok) * a.q_stride + (size_t)(head * a.G + (r - tok * a.G)) * HD + d;
