@@ -29,6 +29,14 @@ def test_shares_of_long_contexts(backend, length, count):
         s.check(window=37, prefix=[500])
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("nh,nkv,count", [(8, 8, 64), (16, 8, 33), (32, 8, 16), (40, 8, 13), (8, 8, 127), (32, 8, 63)])
+def test_less_than_a_tile_of_several_sequences(backend, nh, nkv, count, hd):
+    counts = [count, 1, 0, count - 3, count, 2]
+    Setting(backend, [c + 40 * i + 1 for i, c in enumerate(counts)], counts, nh, nkv, hd, "bf16", seed=count, spread=2.0).check(cap=25.0)
+    Setting(backend, [c + 40 * i + 1 for i, c in enumerate(counts)], counts, nh, nkv, hd, "f16", seed=count + 1).check()
+
+
 def test_many_ragged_sequences(backend):
     """More than a warp looks through at once, some without rows, some with one."""
     counts = [(7 * i * i) % 90 for i in range(75)]
