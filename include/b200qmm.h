@@ -250,8 +250,8 @@ int b2_kv8_free(b2_ctx* ctx, b2_kv8 kv);
 size_t b2_kv8_bytes(b2_ctx* ctx, b2_kv8 kv);
 /* The sequences of a call; the arrays are on the device. Rows rows[s] .. rows[s + 1] - 1 of the call's arrays are sequence s's (rows == NULL: max_rows each,
  * n_rows = n_seqs * max_rows), at positions start[s], start[s] + 1, ...; a sequence may have none. Its block b (positions 32 b ..) is block
- * table[s * max_blocks + b] of the pool (table == NULL: s * max_blocks + b). max_rows is the most rows of a sequence as far as the host knows (more rows
- * cost time, nothing else). What the arrays say is checked where it is used: a sequence outside n_rows or max_blocks * 32 positions is left out, a block
+ * table[s * max_blocks + b] of the pool (table == NULL: s * max_blocks + b). max_rows is the most rows of a sequence as far as the host knows (it chooses
+ * the kernels; more rows cost time). What the arrays say is checked where it is used: a sequence outside n_rows or max_blocks * 32 positions is left out, a block
  * that the pool does not have is not touched, and b2_check_status returns B2_ERR_ARG once the stream is synchronized; the call's results are not valid then. */
 typedef struct b2_kv8_seqs {
     uint32_t n_seqs;
@@ -272,7 +272,7 @@ int b2_kv8_read_dev(b2_ctx* ctx, b2_kv8 kv, const b2_kv8_seqs* seqs, float* k_de
  *   score = cap * tanh(scale * q.k / cap) + slopes[h] * (j - p)
  * (cap 0: scale * q.k; slopes NULL: no bias; prefix NULL: 0 each; window 0: none). q_dev and out_dev of `dtype`, rows of nh * hd values, a row q_stride /
  * out_stride elements behind the one ahead; out_dev may be q_dev. |scale| is at most 2^60, a cap 2^-60 to 2^60. f32 results, and those of up to eight rows a KV head, have
- * f32-like accuracy (22 bits of queries and probabilities); more f16 / bf16 rows are multiplied as f16 with f32 sums, from 64 or 128 rows a KV head on with the values of
+ * f32-like accuracy (22 bits of queries and probabilities); more f16 / bf16 rows are multiplied as f16 with f32 sums, from 64 rows a KV head on with the values of
  * blocks whose scale is below 2^-29 of the sequence's largest as zeros. A row that sees nothing gives zeros; rows that no sequence has stay as they were. */
 typedef struct b2_kv8_attention {
     uint32_t nh;

@@ -767,12 +767,11 @@ cudaError_t launch_attend_kv8(const Kv8Cache& c, const Kv8Seqs& s, const Kv8Attn
                               uint32_t* status, uint64_t& launched, cudaStream_t st, bool pdl) {
     if (!kv8_supports(c.nkv, c.hd) || p.nh == 0 || p.nh % c.nkv) return cudaErrorInvalidValue;
     if (s.n_seqs == 0 || s.n_rows == 0 || s.max_rows == 0) return cudaSuccess;
-    // Many rows go to the form on tcgen05, from 64 of a KV head and sequence on, 16-bit rows of a few sequences (whose keys the other form shares out over more CTAs) from 128 on.
+    // Many rows go to the form on tcgen05, from 64 of a KV head and sequence on.
     // mma.sync / tcgen05, us, 4 heads a KV head, 8 KV heads of 128, one sequence behind 4096 keys, eight behind 1024, 32 behind 512: 32 rows 14.2 / 17.7, 13.7 / 15.4, 22.9 / 28.6; 64 rows
     // 14.9 / 18.3, 17.3 / 15.7, 29.0 / 25.8; 128 rows 19.8 / 19.5, 21.7 / 19.0, 50.7 / 29.9; 512 rows 50.5 / 30.5, 64.8 / 26.7, 167 / 52.
-    const size_t many = dtype != B2_F32 && (size_t)s.n_seqs * c.nkv < 32 ? 128 : 64;
     launched++;
-    if ((dtype != B2_F32 || p.halves) && (size_t)s.max_rows * (p.nh / c.nkv) >= many && attend_kv8_rows_supports(c, s, p.nh))
+    if ((dtype != B2_F32 || p.halves) && (size_t)s.max_rows * (p.nh / c.nkv) >= 64 && attend_kv8_rows_supports(c, s, p.nh))
         return launch_attend_kv8_rows(c, s, p, q, q_stride, out, out_stride, dtype, status, st, pdl);
     AkArgs a{};
     a.c = c;
