@@ -39,7 +39,8 @@ constexpr int KT_THREADS = 768, KT_TILE = 128, KT_BLOCKS = KT_TILE / (int)KV8_BL
 constexpr uint32_t KT_TMEM_COLS = 512;
 // tanh(z) / z by powers of z^2
 constexpr float K0 = 0.999999464f, K1 = -0.333283484f, K2 = 0.132598311f, K3 = -0.0500801913f, K4 = 0.0129507277f;
-constexpr float LAZY_BITS = 8.0f;  // the sums are brought to a new largest score only where it is 2^8 times the one they are at (probabilities stay far below an f16's largest)
+constexpr float LAZY_BITS = 8.0f;  // the sums are brought to a new largest score only where it is 2^8 times the one they are at
+constexpr float KT_P_BITS = 7.0f;  // probabilities are held 2^7 times as large, up to 2^15: those below 2^-21 of the largest lose bits, below 2^-32 they are zeros (at 2^0 a long flat tail got lost)
 constexpr float V_ONE = 32.0f;  // the largest scale of values as it enters the f16 values: 1152 of it has to be an f16, too
 
 struct __align__(16) KtShared {
@@ -634,7 +635,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) attend_kv8_rows_kernel(const __
                     kt_st8(at, o);
                 }
             }
-            const float base = m == -INFINITY ? 0.0f : -m;
+            const float base = m == -INFINITY ? 0.0f : KT_P_BITS - m;
             float2 part[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
             if (tiles == 2 && (w == 1 || i > 0)) {
                 ok = __all_sync(0xffffffffu, kt_wait(&sh->turn[w], (uint32_t)((w == 1 ? i : i - 1) & 1), sh, a.status));

@@ -1,0 +1,35 @@
+"""Attention over the 8-bit cache where queries, values and probabilities are as far apart as their types allow."""
+import math
+
+import pytest
+import torch
+
+from oxinfer_b200.kv8 import Kv8Seqs
+
+from test_attend_kv8_gpu import DEV, Setting, i32
+
+pytestmark = pytest.mark.gpu
+
+
+def test_a_dominant_key_ahead_of_a_long_flat_tail(backend):
+    """131072 keys of 2^-26 of the first one's probability each are 2^-9 of the result together. 80 sequences of 64 rows share the keys, so a CTA has all of them."""
+    n, seqs, t, hd = 131072, 80, 64, 64
+    g = torch.Generator(device=DEV)
+    g.manual_seed(31)
+    cache = backend.kv8(1, hd, n // 32)
+    k = torch.zeros((n, 1, hd), device=DEV)
+    k[0, 0, 0] = 144.0  # (72 * 2 in the cache)
+    v = 0.5 + 0.5 * torch.rand((n, 1, hd), device=DEV, generator=g)
+    v[0] = 0.0
+    assert cache.append(Kv8Seqs(start=i32([0]), max_rows=n, max_blocks=n // 32), k, v) and cache.read(Kv8Seqs(start=i32([0]), max_rows=n, max_blocks=n // 32), k, v)
+    table = torch.arange(n // 32, dtype=torch.int32, device=DEV).expand(seqs, -1).contiguous()
+    q = torch.zeros((seqs * t, 1, hd), dtype=torch.bfloat16, device=DEV)
+    q[:, 0, 0] = 1.0
+    out = torch.empty_like(q)
+    assert cache.attend(Kv8Seqs(start=i32([n - t] * seqs), max_rows=t, max_blocks=n // 32, table=table), q, out, scale=0.125)
+    w = torch.ones(n, dtype=torch.float64, device=DEV)
+    w[0] = math.exp(18.0)
+    y = (torch.cumsum(w[:, None] * v[:, 0].double(), 0) / torch.cumsum(w, 0)[:, None])[n - t:]
+    # a probability's f16 rounding is at most 2^-11 of it (2^-25 of what the row's largest is at least 2^7 of, for the smallest), the scores' 2^-18.5 of 18, half a step of the result
+    tol = (2.0 ** -11 + 18 * 2.0 ** -18.5 + torch.finfo(torch.bfloat16).eps / 2) * y + n * 2.0 ** -32
+    assert ((out.view(seqs, t, hd).double() - y).abs() <= tol).all(), ((out.view(seqs, t, hd).double() - y).abs() / y).max()
