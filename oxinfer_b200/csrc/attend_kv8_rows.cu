@@ -455,7 +455,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) attend_kv8_rows_kernel(const __
             auto factor = [&](uint32_t row, uint32_t bits, bool first) {  // of a row whose largest magnitude has those bits (what is not finite is above all else)
                 const int ex = min(max((int)(bits >> 23), 40), 254) - 127;
                 if (first) sh->told[0][w * KT_TILE + row] = (bits >= 0x7f800000u ? NAN : pow2(ex)) * a.c2;
-                return pow2(-ex) * a.q_sign;
+                return (ex == 127 ? 0x1p-127f : pow2(-ex)) * a.q_sign;  // (2^-127 has no exponent of its own: pow2 does not make it)
             };
             if (sizeof(T) == 2 && a.wide) {  // eight a lane: half the instructions of the form below
                 constexpr int PER = HD / 8, ROWS = 32 / PER, FLIGHT = 16 / ROWS;

@@ -33,3 +33,14 @@ def test_a_dominant_key_ahead_of_a_long_flat_tail(backend):
     # a probability's f16 rounding is at most 2^-11 of it (2^-25 of what the row's largest is at least 2^7 of, for the smallest), the scores' 2^-18.5 of 18, half a step of the result
     tol = (2.0 ** -11 + 18 * 2.0 ** -18.5 + torch.finfo(torch.bfloat16).eps / 2) * y + n * 2.0 ** -32
     assert ((out.view(seqs, t, hd).double() - y).abs() <= tol).all(), ((out.view(seqs, t, hd).double() - y).abs() / y).max()
+
+
+@pytest.mark.parametrize("dtype,count", [("f32", 1), ("f32", 70), ("bf16", 1), ("bf16", 20), ("bf16", 140)])
+def test_queries_up_to_the_largest(backend, dtype, count):
+    for hd in (64, 128):
+        s = Setting(backend, [300], [count], 4, 2, hd, dtype, seed=32, spread=1e-10)
+        s.q = (s.q.float().clamp(-3.0, 3.0) * 1.1e38).to(s.dtype)
+        s.q[0, 0, 5] = -3.3e38
+        s.scale = 1e-28
+        out = s.check()
+        assert float((out[:, 0] - out[:, 1]).abs().max()) > 0.05
