@@ -35,6 +35,8 @@ constexpr uint32_t DEALT_CTAS = 3 * 148, DEALT_LEAST = 4;  // three an SM; block
 template <int HD>
 constexpr size_t DEALT_FLOAT4 = 8 * HD / 4 + 8;  // of a place: the sums of eight rows, their largest scores and denominators
 constexpr float P_BITS = 14.0f;  // probabilities are held 2^14 times as large: what is below 2^-28 of a row's largest loses bits, not before
+// Sums of probabilities times values are held 2^40 times as small, so that they stay finite where the values are (P_BITS, and up to 2^26 keys of a row); a scale is at least 2^-100.
+constexpr float SUM_DOWN = 0x1p-40f, SUM_UP = 0x1p40f;
 
 template <int HD, int TERMS>
 struct AkShared {
@@ -399,7 +401,7 @@ __global__ void __launch_bounds__(AK_THREADS, TERMS == 2 ? 3 : 2) attend_kv8_ker
             if (!ok) break;
             const uint8_t* const unit = ring + slot * L::UNIT;
             const uint4 hd = *(const uint4*)unit;
-            const float k_scale = __uint_as_float(hd.x), v_scale = __uint_as_float(hd.z);
+            const float k_scale = __uint_as_float(hd.x), v_scale = __uint_as_float(hd.z) * SUM_DOWN;
             const uint32_t bad = hd.y | hd.w;
             float sc[RG][8];  // [row][key 2 t + e of tile j]: 2 j + e
 #pragma unroll
@@ -555,7 +557,7 @@ __global__ void __launch_bounds__(AK_THREADS, TERMS == 2 ? 3 : 2) attend_kv8_ker
         auto finish = [&](int item, float4 v, float den) {
             const uint32_t r = row0 + item / (HD / 4);
             if (r >= rows) return;
-            const float inv = den > 0.0f || den != den ? 1.0f / den : 0.0f;  // (a row that sees nothing: zeros)
+            const float inv = den > 0.0f || den != den ? SUM_UP / den : 0.0f;  // (a row that sees nothing: zeros)
             T* const to = (T*)a.out + (size_t)(seq.r0 + r / a.G) * a.out_stride + (size_t)(head * a.G + r % a.G) * HD + item % (HD / 4) * 4;
             store4<T>(to, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv), a.aligned);
         };
@@ -688,7 +690,7 @@ __global__ void __launch_bounds__(2 * HD) attend_kv8_join(const AkArgs a, uint32
                     den += part_l[k];
                 }
             }
-            const float inv = den > 0.0f || den != den ? 1.0f / den : 0.0f;
+            const float inv = den > 0.0f || den != den ? SUM_UP / den : 0.0f;
             T* const to = (T*)a.out + (size_t)(seq.r0 + row / a.G) * a.out_stride + (size_t)(head * a.G + row % a.G) * HD + f * 4;
             store4<T>(to, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv), a.aligned);
         }

@@ -41,6 +41,8 @@ constexpr uint32_t KT_TMEM_COLS = 512;
 constexpr float K0 = 0.999999464f, K1 = -0.333283484f, K2 = 0.132598311f, K3 = -0.0500801913f, K4 = 0.0129507277f;
 constexpr float LAZY_BITS = 8.0f;  // the sums are brought to a new largest score only where it is 2^8 times the one they are at
 constexpr float KT_P_BITS = 7.0f;  // probabilities are held 2^7 times as large, up to 2^15: those below 2^-21 of the largest lose bits, below 2^-32 they are zeros (at 2^0 a long flat tail got lost)
+// The sums leave tensor memory 2^32 times as small, so that they stay finite where the values are (KT_P_BITS + LAZY_BITS, and up to 2^17 keys of a row).
+constexpr float KT_SUM_DOWN = 0x1p-32f, KT_SUM_UP = 0x1p32f;
 constexpr float V_ONE = 32.0f;  // the largest scale of values as it enters the f16 values: 1152 of it has to be an f16, too
 
 struct __align__(16) KtShared {
@@ -667,7 +669,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) attend_kv8_rows_kernel(const __
         if (ok && live) {
             tc_fence_after();
             float4* const dst = (float4*)(smem + (size_t)(w * KT_TILE + row) * HD * 4);
-            const float one = __uint_as_float(*(volatile uint32_t*)&sh->v_top) * (1.0f / V_ONE);
+            const float one = __uint_as_float(*(volatile uint32_t*)&sh->v_top) * (KT_SUM_DOWN / V_ONE);
 #pragma unroll
             for (int h = hc * (HD / 64); h < (hc + 1) * (HD / 64); h++) {
                 uint32_t o[32];
@@ -680,7 +682,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) attend_kv8_rows_kernel(const __
             sh->told[hc][w * KT_TILE + row] = l;
             if (meet(n + 1) && hc == 0) {
                 l += sh->told[1][w * KT_TILE + row];
-                ml[w * KT_TILE + row] = make_float2(m, a.Z > 1 ? l : l > 0.0f || l != l ? 1.0f / l : 0.0f);
+                ml[w * KT_TILE + row] = make_float2(m, a.Z > 1 ? l : l > 0.0f || l != l ? KT_SUM_UP / l : 0.0f);
             }
         }
         __syncwarp();
@@ -740,7 +742,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) attend_kv8_rows_kernel(const __
                         o = make_float4(fmaf(g, b[k].x, o.x), fmaf(g, b[k].y, o.y), fmaf(g, b[k].z, o.z), fmaf(g, b[k].w, o.w));
                         den = fmaf(g, p[k].y, den);
                     }
-                    put(at, o, den > 0.0f || den != den ? 1.0f / den : 0.0f);
+                    put(at, o, den > 0.0f || den != den ? KT_SUM_UP / den : 0.0f);
                 }
             }
         }

@@ -44,3 +44,19 @@ def test_queries_up_to_the_largest(backend, dtype, count):
         s.scale = 1e-28
         out = s.check()
         assert float((out[:, 0] - out[:, 1]).abs().max()) > 0.05
+
+
+@pytest.mark.parametrize("dtype,counts,lengths", [("f32", [1, 3], [90, 200]), ("f32", [40, 70], [90, 200]), ("f32", [1], [40000]), ("bf16", [1, 2], [90, 200]), ("bf16", [9, 20], [90, 200]),
+                                                  ("bf16", [64, 190], [90, 200]), ("bf16", [64], [9000])])
+def test_values_up_to_the_largest(backend, dtype, counts, lengths):
+    """Finite values give finite results: sums of probabilities times values stay below the largest f32 on the way."""
+    for hd in (64, 128):
+        s = Setting(backend, lengths, counts, 4, 2, hd, dtype, seed=33)
+        n = sum(lengths)
+        g = torch.Generator(device=DEV)
+        g.manual_seed(34)
+        v = torch.randn((n, 2, hd), device=DEV, generator=g).clamp(-1.0, 1.0) * 3e38
+        every = Kv8Seqs(start=i32([0] * len(lengths)), rows=i32(s.first_of), n_rows=n, max_rows=max(lengths), max_blocks=s.max_blocks, table=s.table)
+        k = s.k.clone()
+        assert s.cache.append(every, k, v) and s.cache.read(every, s.k, s.v)
+        assert torch.isfinite(s.check()).all() and torch.isfinite(s.check(cap=3.0, window=50)).all()
