@@ -272,8 +272,8 @@ int b2_kv8_read_dev(b2_ctx* ctx, b2_kv8 kv, const b2_kv8_seqs* seqs, float* k_de
  *   score = cap * tanh(scale * q.k / cap) + slopes[h] * (j - p)
  * (cap 0: scale * q.k; slopes NULL: no bias; prefix NULL: 0 each; window 0: none). q_dev and out_dev of `dtype`, rows of nh * hd values, a row q_stride /
  * out_stride elements behind the one ahead; out_dev may be q_dev. |scale| is at most 2^60, a cap 2^-60 to 2^60. f32 results, and those of up to eight rows a KV head, have
- * f32-like accuracy (22 bits of queries and probabilities); more f16 / bf16 rows are multiplied as f16 with f32 sums, from 64 rows a KV head on with the values of
- * blocks whose scale is below 2^-29 of the sequence's largest as zeros. A row that sees nothing gives zeros; rows that no sequence has stay as they were. */
+ * f32-like accuracy (22 bits of queries and probabilities; of queries whose largest magnitude is below 2^-87 fewer); more f16 / bf16 rows are multiplied as f16 with
+ * f32 sums (from 64 rows a KV head on much slower where values of one call lie more than 2^29 apart). A row that sees nothing gives zeros; rows that no sequence has stay as they were. */
 typedef struct b2_kv8_attention {
     uint32_t nh;
     float scale;

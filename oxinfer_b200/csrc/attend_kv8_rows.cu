@@ -1,6 +1,7 @@
 // Attention over the 8-bit cache for many rows of a sequence on tcgen05: S = Q K^T and O += P V with f16 operands and f32 sums in tensor memory, softmax by two
 // threads a row (attend_rows.cu has the form for f16 caches). The integers are exact as f16; a block's scale of keys multiplies its 32 columns of scores, a
-// block's scale of values, over the largest that the CTA's rows see, goes into the f16 values (a power of two, exact down to 2^-29 of the largest, zero below).
+// block's scale of values, over the largest that the CTA's rows see, goes into the f16 values (a power of two, exact down to 2^-29 of the largest). Where values lie
+// further apart, the CTA's sums of values are made anew without tensor cores (far_sums): a row may see the small ones only.
 // Queries are rounded to f16 after a power of two that brings each row's largest to 1 .. 2, probabilities to f16.
 //
 // A CTA takes 256 rows of a KV head (query heads token by token, two tiles of 128) and key tiles of 128, four blocks:
@@ -52,6 +53,11 @@ struct __align__(16) KtShared {
     uint32_t bad[4][KT_BLOCKS];             // tokens that count as NaN
     uint64_t k_full[2], v_full[2], k_empty[2], v_empty[2], q_full, s_full[2][2], s_free[2], p_full[2][2], o_full, u_full[KT_BLOCKS], u_empty[KT_BLOCKS], turn[2], pair[2][4];
     uint32_t tmem_base, v_top, item_seq, item_block;
+    volatile uint32_t far;                  // a block's values are below what f16 holds beside the largest
+    struct {
+        Seq seq;
+        uint32_t prefix, b_beg, b_end, r_block, r_end;
+    } place;                                // (far_sums: nobody else keeps them in registers for it)
     volatile uint32_t abort_flag;
 };
 
@@ -185,6 +191,86 @@ __device__ __forceinline__ float2 kt_peer_f2(const void* p, uint32_t cta) {
     return v;
 }
 
+// The sums of sixteen rows from `at0` of the CTA's on, over the CTA's share of the keys, without tensor cores: values go into f32 sums with their blocks' own scales. A warp has a row at a
+// time, a lane a key of a block for the scores, then HD / 32 dimensions of the values. m: lane i & 15's is the largest score of row i as far as it was kept. qs: [HD] of the warp's own.
+// Some 16 instructions a key and row: 2048 tokens of 32 heads behind 2048 take 9.7 ms instead of 0.11. Values 2^29 apart are hardly ever met; looking for them costs others 0.3 to 1 %.
+template <int HD, bool SPECIAL, typename T>
+__device__ __forceinline__ void far_sums(const KtArgs& a, const KtShared* sh, uint32_t at0, float m, float* qs, uint8_t* sums, float2* ml) {
+    constexpr int D = HD / 32;
+    const int lane = threadIdx.x & 31;
+    const uint32_t s = sh->item_seq, head = blockIdx.x / a.Z % a.c.nkv;
+    const Seq seq = sh->place.seq;
+    const uint32_t prefix = sh->place.prefix, b_beg = sh->place.b_beg, b_end = sh->place.b_end, r_block = sh->place.r_block, r_end = sh->place.r_end;
+#pragma unroll 1
+    for (uint32_t at = at0; at < at0 + 16 && r_block + at < r_end; at++) {
+        const uint32_t r = r_block + at, tok = kt_token(a, r), h = head * a.G + (r - tok * a.G), qp = seq.start + tok;
+        const T* const q = (const T*)a.q + (size_t)(seq.r0 + tok) * a.q_stride + (size_t)h * HD;
+        float x[D];
+        uint32_t bits = 0;
+#pragma unroll
+        for (int k = 0; k < D; k++) {
+            x[k] = to_f32<T>(q[lane + 32 * k]);
+            bits = max(bits, __float_as_uint(x[k]) & 0x7fffffffu);
+        }
+        bits = __reduce_max_sync(0xffffffffu, bits);
+        const int ex = min(max((int)(bits >> 23), 40), 254) - 127;
+        const float down = (ex == 127 ? 0x1p-127f : pow2(-ex)) * a.q_sign, qf = (bits >= 0x7f800000u ? NAN : pow2(ex)) * a.c2;
+#pragma unroll
+        for (int k = 0; k < D; k++) qs[lane + 32 * k] = x[k] * down;
+        __syncwarp();
+        const float top = __shfl_sync(0xffffffffu, m, at & 15), base = top == -INFINITY ? 0.0f : KT_P_BITS - top;
+        const float slope = SPECIAL && a.slopes ? a.slopes[h] * 1.44269504f : 0.0f;
+        const uint32_t see_to = max(qp + 1, prefix), see_from = a.window != 0 && qp + 1 > a.window ? qp + 1 - a.window : 0u;
+        const uint32_t b1 = min(b_end, (see_to + KV8_BLOCK - 1) / KV8_BLOCK);
+        float o[D] = {}, den = 0.0f;
+#pragma unroll 1
+        for (uint32_t b = max(b_beg, see_from / KV8_BLOCK); b < b1; b++) {
+            const int id = max(block_of(a.c, a.sq, s, b, a.status), 0);
+            const uint8_t* const unit = a.c.units + ((size_t)id * a.c.nkv + head) * unit_bytes(HD);
+            const Header hd = *(const Header*)unit;
+            float dot = 0.0f;
+#pragma unroll 1
+            for (int d = 0; d < HD; d += 16) {
+                const uint4 w4 = *(const uint4*)(unit + KV8_HEADER + key_at<HD>(lane, d));
+                const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+#pragma unroll
+                for (int e = 0; e < 16; e++) dot = fmaf(qs[d + e], (float)((int)((w[e >> 2] >> (8 * (e & 3))) & 0xffu) - 128), dot);
+            }
+            const uint32_t j = b * KV8_BLOCK + lane;
+            float y = dot * (qf * hd.k_scale);
+            if (SPECIAL && a.cap2 > 0.0f) y = a.cap2 * tanhf(y * a.cap_z);
+            if (SPECIAL && a.slopes) y = fmaf(slope, (float)((int)j - (int)qp), y);
+            if (((hd.k_bad | hd.v_bad) >> lane) & 1) y = NAN;
+            const float p = j >= see_from && j < see_to ? kt_exp2(y + base) : 0.0f, scale = hd.v_scale * KT_SUM_DOWN;
+            den += p;
+            float part[D] = {};
+#pragma unroll 1
+            for (int t = 0; t < 4; t++) {  // tokens 4 t .. and 16 + 4 t ..
+                uint2 w[D];
+#pragma unroll
+                for (int k = 0; k < D; k++) w[k] = *(const uint2*)(unit + KV8_HEADER + KV8_BLOCK * HD + value_at(4 * t, lane + 32 * k));
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const float pe = __shfl_sync(0xffffffffu, p, 16 * (e >> 2) + 4 * t + (e & 3));
+#pragma unroll
+                    for (int k = 0; k < D; k++) part[k] = fmaf(pe, (float)((int)(((e < 4 ? w[k].x : w[k].y) >> (8 * (e & 3))) & 0xffu) - 128), part[k]);
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < D; k++) o[k] = fmaf(part[k], scale, o[k]);
+        }
+#pragma unroll
+        for (int i = 16; i > 0; i >>= 1) den += __shfl_xor_sync(0xffffffffu, den, i);
+#pragma unroll
+        for (int k = 0; k < D; k++) {
+            const uint32_t d = lane + 32 * k;
+            ((float*)(sums + (size_t)at * HD * 4))[4 * ((d >> 2) ^ (at & 7)) + (d & 3)] = o[k];
+        }
+        if (lane == 0) ml[at] = make_float2(top, a.Z > 1 ? den : den > 0.0f || den != den ? KT_SUM_UP / den : 0.0f);
+        __syncwarp();  // (the row's queries have been read)
+    }
+}
+
 // Grid: (block of 256 rows, KV head, share of the keys), shares first (a cluster's Z), then heads; the blocks of all sequences one after another, a sequence's last
 // first. SPECIAL: a cap or a bias.
 template <int HD, bool SPECIAL, typename T>
@@ -224,6 +310,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) attend_kv8_rows_kernel(const __
             sh->item_seq = found;
             sh->item_block = blk;
             sh->v_top = 0;
+            sh->far = 0;
             sh->abort_flag = 0;
         }
     }
@@ -243,6 +330,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) attend_kv8_rows_kernel(const __
     const uint32_t b_0 = (all_0 + z * share) * KT_BLOCKS, b_beg = max(all_beg, b_0), b_end = max(b_beg, min(all_end, b_0 + n * KT_BLOCKS));
 
     if (tid == 0) {
+        sh->place = {seq, prefix, b_beg, b_end, r_block, r_end};
         for (int i = 0; i < 2; i++) {
             mbar_init(&sh->k_full[i], 4);
             mbar_init(&sh->v_full[i], 4);
@@ -280,6 +368,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) attend_kv8_rows_kernel(const __
         // ---------------- bytes to f16: a warp for each block of a tile ----------------
         const uint32_t bq = warp - 20, t = lane & 3, n0 = (lane >> 2) & 1, u2 = lane >> 3;
         const __half2 one = __float2half2_rn(1.0f), off = __float2half2_rn(-1152.0f);
+        float low = INFINITY;
         {  // the largest scale of values that the rows may see
             uint32_t top = 0;
 #pragma unroll 4
@@ -287,6 +376,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1) attend_kv8_rows_kernel(const __
                 const int id = block_of(a.c, a.sq, s, b, a.status);
                 const float v = ((const Header*)(a.c.units + ((size_t)max(id, 0) * a.c.nkv + head) * L::UNIT))->v_scale;
                 top = max(top, __float_as_uint(fmaxf(v, 0.0f)));
+                low = v > 0.0f ? fminf(low, v) : low;
             }
             top = __reduce_max_sync(0xffffffffu, top);
             if (lane == 0 && top) atomicMax(&sh->v_top, top);
@@ -294,6 +384,28 @@ __global__ void __launch_bounds__(KT_THREADS, 1) attend_kv8_rows_kernel(const __
         }
         const float v_top = __uint_as_float(*(volatile uint32_t*)&sh->v_top);
         const float v_inv = v_top > 0.0f ? V_ONE / v_top : 0.0f;
+        if (__any_sync(0xffffffffu, low * v_inv < 0x1p-24f)) {  // (seldom: f16 values would be zero; a block of zeros has the smallest scale, so the warp looks at its bytes)
+            bool found = false;
+#pragma unroll 1
+            for (uint32_t b0 = b_beg + (warp - 20) * 32; b0 < b_end && !found; b0 += 128) {
+                const int id = b0 + lane < b_end ? max(block_of(a.c, a.sq, s, b0 + lane, a.status), 0) : 0;
+                const unsigned long long at = (unsigned long long)(a.c.units + ((size_t)id * a.c.nkv + head) * L::UNIT);
+                const float v = b0 + lane < b_end ? ((const Header*)at)->v_scale : 0.0f;
+#pragma unroll 1
+                for (uint32_t left = __ballot_sync(0xffffffffu, v > 0.0f && v * v_inv < 0x1p-24f); left && !found; left &= left - 1) {
+                    const uint4* const bytes = (const uint4*)(__shfl_sync(0xffffffffu, at, __ffs(left) - 1) + KV8_HEADER + KV8_BLOCK * HD);
+                    uint32_t any = 0;
+#pragma unroll
+                    for (uint32_t k = 0; k < KV8_BLOCK * HD / 512; k++) {
+                        const uint4 w = bytes[32 * k + lane];
+                        any |= (w.x ^ 0x80808080u) | (w.y ^ 0x80808080u) | (w.z ^ 0x80808080u) | (w.w ^ 0x80808080u);
+                    }
+                    found = __any_sync(0xffffffffu, any != 0);
+                }
+            }
+            if (found && lane == 0) sh->far = 1;
+            __syncwarp();
+        }
         const uint8_t* const unit = smem + L::RING + bq * L::UNIT;
         const int skipped = b_0 + bq < b_beg ? 1 : 0;
         for (int i = 0; i < n; i++) {
@@ -668,21 +780,25 @@ __global__ void __launch_bounds__(KT_THREADS, 1) attend_kv8_rows_kernel(const __
         ok = __all_sync(0xffffffffu, kt_wait(&sh->o_full, 0, sh, a.status) && !sh->abort_flag);
         if (ok && live) {
             tc_fence_after();
-            float4* const dst = (float4*)(smem + (size_t)(w * KT_TILE + row) * HD * 4);
-            const float one = __uint_as_float(*(volatile uint32_t*)&sh->v_top) * (KT_SUM_DOWN / V_ONE);
+            if (sh->far) {
+                far_sums<HD, SPECIAL, T>(a, sh, w * KT_TILE + (warp & 3) * 32 + hc * 16, __shfl_sync(0xffffffffu, m, (lane & 15) + hc * 16), (float*)(smem + L::RING) + warp * HD, smem, ml);
+            } else {
+                float4* const dst = (float4*)(smem + (size_t)(w * KT_TILE + row) * HD * 4);
+                const float one = __uint_as_float(*(volatile uint32_t*)&sh->v_top) * (KT_SUM_DOWN / V_ONE);
 #pragma unroll
-            for (int h = hc * (HD / 64); h < (hc + 1) * (HD / 64); h++) {
-                uint32_t o[32];
-                kt_ld32(o_at + 32 * h, o);
-                kt_ld_wait();
-                auto f = [&](int e) { return n > 0 ? __uint_as_float(o[e]) * one : 0.0f; };
+                for (int h = hc * (HD / 64); h < (hc + 1) * (HD / 64); h++) {
+                    uint32_t o[32];
+                    kt_ld32(o_at + 32 * h, o);
+                    kt_ld_wait();
+                    auto f = [&](int e) { return n > 0 ? __uint_as_float(o[e]) * one : 0.0f; };
 #pragma unroll
-                for (int e = 0; e < 8; e++) dst[(8 * h + e) ^ (row & 7)] = make_float4(f(4 * e), f(4 * e + 1), f(4 * e + 2), f(4 * e + 3));
-            }
-            sh->told[hc][w * KT_TILE + row] = l;
-            if (meet(n + 1) && hc == 0) {
-                l += sh->told[1][w * KT_TILE + row];
-                ml[w * KT_TILE + row] = make_float2(m, a.Z > 1 ? l : l > 0.0f || l != l ? KT_SUM_UP / l : 0.0f);
+                    for (int e = 0; e < 8; e++) dst[(8 * h + e) ^ (row & 7)] = make_float4(f(4 * e), f(4 * e + 1), f(4 * e + 2), f(4 * e + 3));
+                }
+                sh->told[hc][w * KT_TILE + row] = l;
+                if (meet(n + 1) && hc == 0) {
+                    l += sh->told[1][w * KT_TILE + row];
+                    ml[w * KT_TILE + row] = make_float2(m, a.Z > 1 ? l : l > 0.0f || l != l ? KT_SUM_UP / l : 0.0f);
+                }
             }
         }
         __syncwarp();

@@ -60,3 +60,74 @@ def test_values_up_to_the_largest(backend, dtype, counts, lengths):
         k = s.k.clone()
         assert s.cache.append(every, k, v) and s.cache.read(every, s.k, s.v)
         assert torch.isfinite(s.check()).all() and torch.isfinite(s.check(cap=3.0, window=50)).all()
+
+
+class Apart:
+    """One sequence whose values are `size` [n] large, and the formula's results with a bound that goes by the largest value in a row's own sight."""
+
+    def __init__(self, backend, size, t, nh, nkv, hd, seed, poison=()):
+        n = size.numel()
+        self.s = s = Setting(backend, [n], [t], nh, nkv, hd, "bf16", seed=seed)
+        g = torch.Generator(device=DEV)
+        g.manual_seed(seed)
+        v = torch.randn((n, nkv, hd), device=DEV, generator=g) * size[:, None, None].float()
+        for pos, head in poison:
+            v[pos, head, 3] = math.nan
+        every = Kv8Seqs(start=i32([0]), max_rows=n, max_blocks=s.max_blocks, table=s.table)
+        k = s.k.clone()
+        assert s.cache.append(every, k, v) and s.cache.read(every, s.k, s.v)
+        self.n, self.t = n, t
+
+    def check(self, **kw):
+        s, n, t = self.s, self.n, self.t
+        y, _ = s.want(**kw)
+        out = torch.full_like(s.q, 9.0)
+        pre = i32(kw["prefix"]) if kw.get("prefix") is not None else None
+        assert s.cache.attend(s.seqs, s.q, out, scale=s.scale, cap=kw.get("cap", 0.0), window=kw.get("window", 0), slopes=kw.get("slopes"), prefix=pre)
+        torch.cuda.synchronize()
+        s.be.check_status()
+        j, p = torch.arange(n, device=DEV), torch.arange(n - t, n, device=DEV)
+        see = j[None] <= p[:, None]
+        if pre is not None:
+            see |= j[None] < pre[0]
+        if kw.get("window"):
+            see &= p[:, None] - j[None] < kw["window"]
+        top = (see[:, :, None] * s.v.nan_to_num(0.0).abs().amax(-1).double()[None]).amax(1)  # [t][nkv]: the largest value that a row sees
+        top = top.repeat_interleave(s.nh // s.nkv, 1)[:, :, None]
+        # 2^-11 of a probability, 2^-13 for the scores' rounding (2^-18.5 of magnitudes of up to 45), half a step of the result
+        tol = top * (2.0 ** -11 + 2.0 ** -13) + torch.finfo(torch.bfloat16).eps / 2 * y.abs().nan_to_num(0.0)
+        got = out.double()
+        assert torch.equal(torch.isnan(got), torch.isnan(y))
+        err = ((got - y).abs() - tol).nan_to_num(0.0)
+        assert (err <= 0).all(), ((got - y).abs() / top.clamp(min=1e-300)).nan_to_num(0.0).max()
+        return out
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("nh,nkv", [(2, 2), (8, 2), (6, 2)])
+def test_large_values_reach_no_row_that_does_not_see_them(backend, nh, nkv, hd):
+    """Values 2^31 to 2^45 apart: behind the rows that see the small ones, within one tile of keys, and in front of the window."""
+    n = 400
+    at = torch.arange(n, device=DEV)
+    for size in (2.0 ** torch.where(at < 200, -45.0, 0.0), 2.0 ** torch.where(at < 200, 0.0, -45.0), 2.0 ** torch.where(at // 32 % 3 == 2, 1.0, torch.where(at // 32 % 3 == 1, -30.0, -31.0))):
+        a = Apart(backend, size, 350, nh, nkv, hd, seed=35)
+        a.check()
+        a.check(window=20)
+        a.check(cap=4.0, window=70, prefix=[90])
+        a.check(slopes=torch.tensor([-0.05 * (i + 1) for i in range(nh)], device=DEV), prefix=[150])
+
+
+def test_large_values_with_shares_and_what_is_not_finite(backend):
+    at = torch.arange(5000, device=DEV)
+    for size in (2.0 ** torch.where(at < 4960, -50.0, 3.0), 2.0 ** torch.where(at < 100, 3.0, -50.0), 2.0 ** torch.where(at % 1000 < 500, -40.0, 0.0)):
+        a = Apart(backend, size, 80, 4, 2, 128, seed=36)
+        a.check()
+        a.check(window=30)
+        a.check(window=600, cap=5.0)
+        a = Apart(backend, size, 80, 4, 2, 64, seed=37, poison=[(4955, 1), (4500, 0)])
+        out = a.check(window=50)
+        assert torch.isnan(out[35:, 2:]).all() and not torch.isnan(out[:35]).any() and not torch.isnan(out[:, :2]).any()
+    # the smallest scale there is, with values and without
+    size = torch.where(at < 4960, 0.0, 1.0).double()
+    size[4800:4900] = 2.0 ** -96
+    Apart(backend, size, 300, 2, 1, 64, seed=38).check(window=130)
