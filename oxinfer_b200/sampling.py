@@ -37,7 +37,8 @@ class GenerateRules:
 class LogitRules:
     """What changes rows of logits, in this order: ``l / repeat`` (``l * repeat`` where ``l <= 0``) and ``- (frequency * count + presence)`` for tokens of the
     history; ``+ bias``; ``-inf`` where ``mask`` has no bit. ``history`` and ``bias_ids`` are int32 lists on the device, ``bias`` f32; row ``r`` has the part
-    ``ptr[r] .. ptr[r + 1] - 1`` of a list, or all of it where the ``ptr`` is None. ``mask``: int32 words, one row for all or a row each."""
+    ``ptr[r] .. ptr[r + 1] - 1`` of a list, or all of it where the ``ptr`` is None. ``mask``: int32 words, ``[words]`` or ``[1, words]`` for all rows, or
+    ``[t, words]``, with ``words`` at least ``(n + 31) // 32`` (exactly that many in the first form)."""
     repeat: float = 1.0
     frequency: float = 0.0
     presence: float = 0.0
@@ -68,7 +69,9 @@ class LogitRules:
                 assert ok(self.bias_ptr, int32) and self.bias_ptr.numel() == t + 1
                 r.bias_ptr = self.bias_ptr.data_ptr()
         if m is not None:
-            width = m.shape[-1]
-            assert ok(m, int32) and width >= (n + 31) // 32 and m.numel() in (width, t * width)
+            assert m.dim() > 0 and ok(m, int32)
+            width, words = m.shape[-1], (n + 31) // 32
+            # (a list of words is one row: the rows of several would all get the first one's bits)
+            assert width >= words and m.numel() in (width, t * width) and (m.dim() > 1 or t == 1 or width == words)
             r.mask, r.mask_stride = m.data_ptr(), width if m.numel() == t * width else 0
         return r
