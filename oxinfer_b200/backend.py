@@ -333,8 +333,8 @@ class Backend:
         (int32 [t]; -1 where nothing is left)."""
         t, n = logits.shape
         dev, (xs, one) = logits.device, logits.stride()
-        assert dev.index == self.ordinal and one == 1
-        assert out is None or (out.shape == logits.shape and out.dtype == logits.dtype and out.device == dev and out.stride(1) == 1)
+        assert dev.index == self.ordinal and (one == 1 or n == 1)
+        assert out is None or (out.shape == logits.shape and out.dtype == logits.dtype and out.device == dev and (out.stride(1) == 1 or n == 1))
         assert pick is None or (pick.element_size() == 4 and not pick.is_floating_point() and pick.numel() == t and pick.is_contiguous() and pick.device == dev)
         r = rules.c(t, n, dev) if rules is not None else None
         return self._check(self._L.b2_logits_dev(self._ctx, logits.data_ptr(), None if out is None else out.data_ptr(), _dtype_code(logits), t, n, xs,

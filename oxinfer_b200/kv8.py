@@ -81,11 +81,23 @@ class Kv8Cache:
         with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=self.device) if stream else torch.cuda.default_stream(self.device)):
             return torch.empty(self._work_bytes, dtype=torch.uint8, device=self.device)
 
+    @staticmethod
+    def _strides(x):
+        """Of ``[rows][heads][hd]``; a dimension of one has whatever stride torch gave it, and counts as if it lay side by side."""
+        rows, heads, hd = x.shape
+        a, b, c = x.stride()
+        if heads == 1:
+            b = hd
+        return (heads * hd if rows == 1 else a), b, c
+
     def append(self, seqs: Kv8Seqs, k, v) -> bool:
         """Keys and values ``[n_rows][nkv][hd]`` (f32, bf16 or f16; any strides of rows and heads, the same for both)."""
         shape, stride = (seqs.n_rows, self.nkv, self.hd), k.stride()
         assert k.shape == shape and v.shape == shape and k.dtype == v.dtype and k.device == self.device == v.device == seqs.device
-        assert v.stride() == stride and stride[2] == 1
+        if v.stride() != stride:
+            stride = self._strides(k)
+            assert self._strides(v) == stride
+        assert stride[2] == 1
         be = self.backend
         return be._check(be._L.b2_kv8_append_dev(be._ctx, self.handle, seqs._ref, k.data_ptr(), v.data_ptr(), self._codes[k.dtype], stride[0], stride[1]))
 
@@ -103,6 +115,8 @@ class Kv8Cache:
         position or below ``prefix`` (int32 [n]), and with a ``window`` only if it is less than that far behind."""
         n, nh, hd = q.shape
         dtype, qs, os = q.dtype, q.stride(), out.stride()
+        if nh == 1:
+            qs, os = self._strides(q), self._strides(out)
         assert out.shape == q.shape and n == seqs.n_rows and hd == self.hd and out.dtype == dtype and q.device == self.device == out.device == seqs.device
         assert qs[2] == os[2] == 1 and qs[1] == os[1] == hd
         assert slopes is None or (slopes.dtype == self._f32 and slopes.numel() == nh and slopes.is_contiguous() and slopes.device == self.device)
