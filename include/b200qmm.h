@@ -271,7 +271,7 @@ int b2_kv8_read_dev(b2_ctx* ctx, b2_kv8 kv, const b2_kv8_seqs* seqs, float* k_de
  * then): key j is seen where j <= p or j < prefix[s], and, with a window, p - j < window. Query head h reads KV head h / (nh / nkv).
  *   score = cap * tanh(scale * q.k / cap) + slopes[h] * (j - p)
  * (cap 0: scale * q.k; slopes NULL: no bias; prefix NULL: 0 each; window 0: none). q_dev and out_dev of `dtype`, rows of nh * hd values, a row q_stride /
- * out_stride elements behind the one ahead; out_dev may be q_dev. |scale| is at most 2^60, a cap 2^-60 to 2^60. f32 results, and those of up to eight rows a KV head, have
+ * out_stride elements behind the one ahead; out_dev may be q_dev with its stride, or share no value with it (else refused). |scale| is at most 2^60, a cap 2^-60 to 2^60. f32 results, and those of up to eight rows a KV head, have
  * f32-like accuracy (22 bits of queries and probabilities; of queries whose largest magnitude is below 2^-87 fewer); more f16 / bf16 rows are multiplied as f16 with
  * f32 sums (from 64 rows a KV head on much slower where values of one call lie more than 2^29 apart). A row that sees nothing gives zeros; rows that no sequence has stay as they were. */
 typedef struct b2_kv8_attention {
@@ -293,7 +293,7 @@ int b2_attend_kv8_dev(b2_ctx* ctx, b2_kv8 kv, const b2_kv8_seqs* seqs, const b2_
  *   1. a token that the row's history holds c > 0 times: l = l > 0 ? l / repeat : l * repeat, then l = l - (frequency * c + presence);
  *   2. a token of the row's bias list: l = l + bias (of a token given twice, the last entry);
  *   3. a token that the mask does not allow: -inf.
- * out_dev (may be logits_dev, or NULL) receives the rows, rounded to `dtype`; pick_dev[r] (may be NULL) the first of the largest as they are stored, -1 where none is
+ * out_dev (may be logits_dev with its stride, or NULL; other overlaps are refused) receives the rows, rounded to `dtype`; pick_dev[r] (may be NULL) the first of the largest as they are stored, -1 where none is
  * above -inf (NaN is never chosen). Row r's history is history[history_ptr[r]] .. history[history_ptr[r + 1] - 1], of n_history in all (history_ptr NULL: all
  * of it for every row); the same for the biases. Ids outside 0 .. n - 1 are left out. Bit i % 32 of word i / 32 of a row's mask allows token i; a row's
  * mask lies mask_stride words behind the one ahead (0: one mask for all rows). Lists and mask are on the device. A row whose part of a list lies outside it has

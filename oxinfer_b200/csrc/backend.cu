@@ -1558,6 +1558,15 @@ class Backend {
         return B2_OK;
     }
     static bool dtype_ok(int d) { return d == B2_F32 || d == B2_BF16 || d == B2_F16; }
+    // Whether results [rows][width] may be written while other rows of the input are still to be read from there: not where they are the input's own rows, or lie beside them.
+    static bool over_other_rows(const void* in, size_t is, const void* out, size_t os, size_t rows, size_t width, int dtype) {
+        const uintptr_t e = dtype == B2_F32 ? 4 : 2, a = (uintptr_t)in, b = (uintptr_t)out;
+        if (rows == 1) is = os = width;
+        if ((a == b && is == os) || a + ((rows - 1) * is + width) * e <= b || b + ((rows - 1) * os + width) * e <= a) return false;
+        if (is != os) return true;
+        const uintptr_t at = a < b ? (b - a) % (os * e) : (os * e - (a - b) % (os * e)) % (os * e);
+        return at < width * e || os * e - at < width * e;
+    }
     int kv8_seqs(const Kv8Pool* p, const b2_kv8_seqs* s, const char* who, Kv8Seqs* out) {
         if (!p) return fail(B2_ERR_ARG, "[b200qmm: %s: unknown cache]", who);
         if (!s) return fail(B2_ERR_ARG, "[b200qmm: %s: null argument]", who);
@@ -1608,6 +1617,7 @@ class Backend {
         if (!q || !out) return fail(B2_ERR_ARG, "[b200qmm: attend_kv8: null argument]");
         if ((uintptr_t)a->work & 15) return fail(B2_ERR_ARG, "[b200qmm: attend_kv8: the work memory is not aligned to 16 bytes]");
         if (s.n_rows > 1 && out_stride < (size_t)a->nh * p->dev.hd) return fail(B2_ERR_ARG, "[b200qmm: attend_kv8: rows of the result overlap]");
+        if (over_other_rows(q, q_stride, out, out_stride, s.n_rows, (size_t)a->nh * p->dev.hd, dtype)) return fail(B2_ERR_ARG, "[b200qmm: attend_kv8: the results lie over queries of other rows]");
         if ((uint64_t)s.n_rows * (a->nh / p->dev.nkv) > 0x7fffffffu) return fail(B2_DECLINED, "[b200qmm: attend_kv8: too many rows for one call]");
         cudaError_t e = launch_attend_kv8(p->dev, s, Kv8Attn{a->nh, a->scale, a->cap, a->window, a->slopes, a->prefix, 0, a->work}, q, q_stride, out, out_stride, dtype, list_status(), launches, stream);
         return e == cudaSuccess ? B2_OK : cuda_fail(e, "attend_kv8");
@@ -1631,6 +1641,7 @@ class Backend {
         if (!x || (!out && !pick)) return fail(B2_ERR_ARG, "[b200qmm: logits: null argument]");
         if (n > 0x7fffff00u || t > 0x7ffffffu) return fail(B2_DECLINED, "[b200qmm: logits: %zu rows of %zu are too many for one call]", t, n);
         if (t > 1 && ((out && os < n) || xs < n)) return fail(B2_ERR_ARG, "[b200qmm: logits: rows overlap]");
+        if (out && over_other_rows(x, xs, out, os, t, n, dtype)) return fail(B2_ERR_ARG, "[b200qmm: logits: the results lie over logits of other rows]");
         cudaError_t e = launch_logits(x, out, dtype, xs, os, (uint32_t)t, (uint32_t)n, r, pick, list_status(), stream);
         launches++;
         return e == cudaSuccess ? B2_OK : cuda_fail(e, "logits");

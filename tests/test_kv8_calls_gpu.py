@@ -34,3 +34,39 @@ def test_rows_of_one_logit(backend):
     for view in (x, x.as_strided((3, 1), (2, 17))):
         assert backend.logits_dev(view, out.as_strided((3, 1), (5, 3)), pick) and pick.tolist() == [0, 0, -1]
         assert torch.equal(out[:2, 0], x[:2, 0]) and torch.isnan(out[2, 0]) and (out[:, 1:] == 7.0).all()
+
+
+def test_results_over_other_rows_are_refused(backend):
+    """The input's own rows, rows beside them and rows behind them are fine."""
+    s = Setting(backend, [40, 77], [3, 5], 4, 2, 64, "f16", seed=41)
+    want, w = s.check(), 4 * 64
+    for q_at, qs, o_at, os, fine in ((0, w, 0, w, True), (0, 2 * w, w, 2 * w, True), (w, 2 * w, 0, 2 * w, True), (0, 2 * w + 8, w + 8, 2 * w + 8, True), (0, w, 8 * w, w, True),
+                                     (8 * 2 * w, w, 0, 2 * w, True), (0, 2 * w, 3 * w, 2 * w, True),
+                                     (0, 2 * w, 0, w, False), (0, w, 0, 2 * w, False), (0, w, w, w, False), (w, w, 0, w, False), (0, 2 * w, w - 1, 2 * w, False), (0, 2 * w, w + 1, 2 * w, False),
+                                     (0, 2 * w, 2 * w, 2 * w, False), (0, w, 7 * w, w, False)):
+        room = torch.full((30 * w,), 5.0, dtype=s.dtype, device=DEV)
+        q, out = (room.as_strided((8, 4, 64), (stride, 64, 1), at) for at, stride in ((q_at, qs), (o_at, os)))
+        q.copy_(s.q)
+        before = room.clone()
+        if fine:
+            assert s.cache.attend(s.seqs, q, out, scale=s.scale) and torch.equal(out, want), (q_at, qs, o_at, os)
+            continue
+        with pytest.raises(ob.BackendError) as e:
+            s.cache.attend(s.seqs, q, out, scale=s.scale)
+        assert e.value.code == -2 and torch.equal(room, before), (q_at, qs, o_at, os)
+    t, n = 6, 1000
+    x = torch.randn((t, n), device=DEV)
+    for x_at, xs, o_at, os, fine in ((0, n, 0, n, True), (0, 2 * n, n, 2 * n, True), (n, n, n + t * n, n, True), (0, 2 * n, 0, n, False), (0, n, 0, 2 * n, False), (0, n, n, n, False),
+                                     (0, 2 * n, 2 * n - 1, 2 * n, False), (5, n, 0, n, False)):
+        room = torch.full((3 * t * n,), 5.0, device=DEV)
+        a, out = (room.as_strided((t, n), (stride, 1), at) for at, stride in ((x_at, xs), (o_at, os)))
+        a.copy_(x)
+        before = room.clone()
+        if fine:
+            assert backend.logits_dev(a, out) and torch.equal(out, x)
+            continue
+        with pytest.raises(ob.BackendError) as e:
+            backend.logits_dev(a, out)
+        assert e.value.code == -2 and torch.equal(room, before)
+    one = torch.randn((1, n), device=DEV)  # (a row's stride means nothing)
+    assert backend.logits_dev(one, one.as_strided((1, n), (3, 1)))
