@@ -1637,7 +1637,12 @@ class Backend {
         LogitRulesDev r;
         if (int rc = logit_rules(rules, n, "logits", &r)) return rc;
         if (!dtype_ok(dtype)) return fail(B2_ERR_ARG, "[b200qmm: logits: unknown element type %d]", dtype);
-        if (t == 0 || n == 0) return B2_OK;
+        if (t == 0) return B2_OK;
+        if (n == 0) {  // rows of nothing: there is nothing to choose
+            if (pick && t > 0x7ffffffu) return fail(B2_DECLINED, "[b200qmm: logits: %zu rows are too many for one call]", t);
+            cudaError_t e = pick ? cudaMemsetAsync(pick, 0xff, t * sizeof *pick, stream) : cudaSuccess;
+            return e == cudaSuccess ? B2_OK : cuda_fail(e, "logits");
+        }
         if (!x || (!out && !pick)) return fail(B2_ERR_ARG, "[b200qmm: logits: null argument]");
         if (n > 0x7fffff00u || t > 0x7ffffffu) return fail(B2_DECLINED, "[b200qmm: logits: %zu rows of %zu are too many for one call]", t, n);
         if (t > 1 && ((out && os < n) || xs < n)) return fail(B2_ERR_ARG, "[b200qmm: logits: rows overlap]");

@@ -70,3 +70,9 @@ def test_results_over_other_rows_are_refused(backend):
         assert e.value.code == -2 and torch.equal(room, before)
     one = torch.randn((1, n), device=DEV)  # (a row's stride means nothing)
     assert backend.logits_dev(one, one.as_strided((1, n), (3, 1)))
+
+
+def test_rows_of_no_logits(backend):
+    x, pick = torch.empty((3, 0), device=DEV), torch.full((3,), 7, dtype=torch.int32, device=DEV)
+    assert backend.logits_dev(x, x, pick) and pick.tolist() == [-1, -1, -1]
+    assert backend.logits_dev(x, x) and backend.logits_dev(x[:0], None, pick[:0])
