@@ -1645,7 +1645,7 @@ class Backend {
         }
         if (!x || (!out && !pick)) return fail(B2_ERR_ARG, "[b200qmm: logits: null argument]");
         if (n > 0x7fffff00u || t > 0x7ffffffu) return fail(B2_DECLINED, "[b200qmm: logits: %zu rows of %zu are too many for one call]", t, n);
-        if (t > 1 && ((out && os < n) || xs < n)) return fail(B2_ERR_ARG, "[b200qmm: logits: rows overlap]");
+        if (t > 1 && out && os < n) return fail(B2_ERR_ARG, "[b200qmm: logits: rows of the result overlap]");
         if (out && over_other_rows(x, xs, out, os, t, n, dtype)) return fail(B2_ERR_ARG, "[b200qmm: logits: the results lie over logits of other rows]");
         cudaError_t e = launch_logits(x, out, dtype, xs, os, (uint32_t)t, (uint32_t)n, r, pick, list_status(), stream);
         launches++;

@@ -76,3 +76,20 @@ def test_rows_of_no_logits(backend):
     x, pick = torch.empty((3, 0), device=DEV), torch.full((3,), 7, dtype=torch.int32, device=DEV)
     assert backend.logits_dev(x, x, pick) and pick.tolist() == [-1, -1, -1]
     assert backend.logits_dev(x, x) and backend.logits_dev(x[:0], None, pick[:0])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_one_row_of_logits_under_the_rules_of_several(backend, dtype):
+    """A row that is read for all (stride zero), and rows that share a part of theirs; not over themselves."""
+    t, n = 5, 20000
+    room = torch.randn(n + 4 * 8, device=DEV).to(dtype)
+    rules = ob.LogitRules(bias_ids=i32([11, 12, 13, 14, 15]), bias=torch.full((5,), 50.0, device=DEV), bias_ptr=i32([0, 1, 2, 3, 4, 5]))
+    for stride in (0, 8):
+        x, out, pick = room.as_strided((t, n), (stride, 1)), torch.empty((t, n), dtype=dtype, device=DEV), torch.empty(t, dtype=torch.int32, device=DEV)
+        assert backend.logits_dev(x, out, pick, rules) and pick.tolist() == [11, 12, 13, 14, 15]
+        want = x.float().clone()
+        for i in range(t):
+            want[i, 11 + i] += 50.0
+        assert torch.equal(out, want.to(dtype))
+        with pytest.raises(ob.BackendError):
+            backend.logits_dev(x, x, pick, rules)
