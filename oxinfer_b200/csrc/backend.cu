@@ -8,6 +8,7 @@
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
+#include <initializer_list>
 #include <mutex>
 #include <string>
 #include <unordered_map>
@@ -1558,6 +1559,13 @@ class Backend {
         return B2_OK;
     }
     static bool dtype_ok(int d) { return d == B2_F32 || d == B2_BF16 || d == B2_F16; }
+    // Device pointers that lie between two elements would fault the GPU.
+    static bool between(int dtype, const void* a, const void* b) { return (((uintptr_t)a | (uintptr_t)b) & (dtype == B2_F32 ? 3 : 1)) != 0; }
+    static bool words_ok(std::initializer_list<const void*> all) {
+        for (const void* p : all)
+            if ((uintptr_t)p & 3) return false;
+        return true;
+    }
     // Whether results [rows][width] may be written while other rows of the input are still to be read from there: not where they are the input's own rows, or lie beside them.
     static bool over_other_rows(const void* in, size_t is, const void* out, size_t os, size_t rows, size_t width, int dtype) {
         const uintptr_t e = dtype == B2_F32 ? 4 : 2, a = (uintptr_t)in, b = (uintptr_t)out;
@@ -1572,6 +1580,7 @@ class Backend {
         if (!s) return fail(B2_ERR_ARG, "[b200qmm: %s: null argument]", who);
         *out = Kv8Seqs{s->n_seqs, s->n_rows, s->max_rows, s->max_blocks, s->table, s->start, s->rows};
         if (s->n_seqs == 0 || s->n_rows == 0) return B2_OK;
+        if (!words_ok({s->table, s->start, s->rows})) return fail(B2_ERR_ARG, "[b200qmm: %s: an array of the sequences is not aligned to 4 bytes]", who);
         if (!s->start) return fail(B2_ERR_ARG, "[b200qmm: %s: the sequences' first positions are missing]", who);
         if (s->max_rows == 0 || s->max_rows > s->n_rows || (!s->rows && (uint64_t)s->n_seqs * s->max_rows != s->n_rows))
             return fail(B2_ERR_ARG, "[b200qmm: %s: %u rows in %u sequences of up to %u]", who, s->n_rows, s->n_seqs, s->max_rows);
@@ -1589,6 +1598,7 @@ class Backend {
         if (!dtype_ok(dtype)) return fail(B2_ERR_ARG, "[b200qmm: kv8_append: unknown element type %d]", dtype);
         if (s.n_seqs == 0 || s.n_rows == 0) return B2_OK;
         if (!k || !v) return fail(B2_ERR_ARG, "[b200qmm: kv8_append: null argument]");
+        if (between(dtype, k, v)) return fail(B2_ERR_ARG, "[b200qmm: kv8_append: keys or values are not aligned to their type]");
         cudaError_t e = launch_kv8_append(p->dev, s, Kv8Rows{k, v, dtype, rs, hs}, false, list_status(), stream);
         launches++;
         return e == cudaSuccess ? B2_OK : cuda_fail(e, "kv8_append");
@@ -1615,6 +1625,7 @@ class Backend {
             return fail(B2_ERR_ARG, "[b200qmm: attend_kv8: a scale of at most 2^60 and a cap of 2^-60 to 2^60, or none]");
         if (s.n_seqs == 0 || s.n_rows == 0) return B2_OK;
         if (!q || !out) return fail(B2_ERR_ARG, "[b200qmm: attend_kv8: null argument]");
+        if (between(dtype, q, out) || !words_ok({a->slopes, a->prefix})) return fail(B2_ERR_ARG, "[b200qmm: attend_kv8: an argument is not aligned to its type]");
         if ((uintptr_t)a->work & 15) return fail(B2_ERR_ARG, "[b200qmm: attend_kv8: the work memory is not aligned to 16 bytes]");
         if (s.n_rows > 1 && out_stride < (size_t)a->nh * p->dev.hd) return fail(B2_ERR_ARG, "[b200qmm: attend_kv8: rows of the result overlap]");
         if (over_other_rows(q, q_stride, out, out_stride, s.n_rows, (size_t)a->nh * p->dev.hd, dtype)) return fail(B2_ERR_ARG, "[b200qmm: attend_kv8: the results lie over queries of other rows]");
@@ -1644,6 +1655,8 @@ class Backend {
             return e == cudaSuccess ? B2_OK : cuda_fail(e, "logits");
         }
         if (!x || (!out && !pick)) return fail(B2_ERR_ARG, "[b200qmm: logits: null argument]");
+        if (between(dtype, x, out) || !words_ok({r.history, r.history_ptr, r.bias_ids, r.bias, r.bias_ptr, r.mask, pick}))
+            return fail(B2_ERR_ARG, "[b200qmm: logits: an argument is not aligned to its type]");
         if (n > 0x7fffff00u || t > 0x7ffffffu) return fail(B2_DECLINED, "[b200qmm: logits: %zu rows of %zu are too many for one call]", t, n);
         if (t > 1 && out && os < n) return fail(B2_ERR_ARG, "[b200qmm: logits: rows of the result overlap]");
         if (out && over_other_rows(x, xs, out, os, t, n, dtype)) return fail(B2_ERR_ARG, "[b200qmm: logits: the results lie over logits of other rows]");

@@ -1,4 +1,6 @@
 """Calls of the 8-bit cache and of rules on logits that their documentation allows: strides, alignments, results over inputs, sizes of one and of none."""
+import ctypes as C
+
 import pytest
 import torch
 
@@ -93,3 +95,33 @@ def test_one_row_of_logits_under_the_rules_of_several(backend, dtype):
         assert torch.equal(out, want.to(dtype))
         with pytest.raises(ob.BackendError):
             backend.logits_dev(x, x, pick, rules)
+
+
+def test_addresses_between_elements_are_refused(backend):
+    """Ahead of any launch."""
+    s = Setting(backend, [40], [1], 4, 2, 64, "f32", seed=42)
+    L, F32, F16 = ob.lib(), ob._lib.F32, ob._lib.F16
+    room = torch.zeros(4096, device=DEV)
+    at = room.data_ptr()
+    words = i32([0, 1, 2, 3])
+    w = words.data_ptr()
+    seqs = lambda **k: C.byref(ob._lib.Kv8Seqs(**{**dict(n_seqs=1, n_rows=1, max_rows=1, max_blocks=1, table=None, start=w, rows=None), **k}))
+    attn = lambda **k: C.byref(ob._lib.Kv8Attention(**{**dict(nh=4, scale=1.0, cap=0.0, window=0, slopes=None, prefix=None, work=None), **k}))
+    rules = lambda **k: C.byref(ob._lib.LogitRules(**{**dict(repeat=1.5, frequency=0.0, presence=0.0), **k}))
+    append = lambda q, k, v, t: L.b2_kv8_append_dev(backend._ctx, s.cache.handle, q, k, v, t, 128, 64)
+    attend = lambda q, a, x, y, t: L.b2_attend_kv8_dev(backend._ctx, s.cache.handle, q, a, x, 256, y, 256, t)
+    logits = lambda x, y, t, r, p: L.b2_logits_dev(backend._ctx, x, y, t, 1, 100, 100, 100, r, p)
+    before = backend.launch_count()
+    for rc in (append(seqs(), at + 2, at + 2048, F32), append(seqs(), at, at + 2049, F32), append(seqs(), at + 1, at, F16), append(seqs(start=w + 2), at, at, F32),
+               append(seqs(table=w + 1), at, at, F32), append(seqs(rows=w + 2), at, at, F32), L.b2_kv8_read_dev(backend._ctx, s.cache.handle, seqs(start=w + 1), at, at + 2048),
+               attend(seqs(), attn(), at + 2, at + 4096, F32), attend(seqs(), attn(), at, at + 4097, F16), attend(seqs(), attn(slopes=at + 2), at, at + 4096, F32),
+               attend(seqs(), attn(prefix=w + 3), at, at + 4096, F32), attend(seqs(start=w + 2), attn(), at, at + 4096, F32),
+               logits(at + 2, None, F32, None, w), logits(at, at + 4097, F16, None, w), logits(at, None, F32, None, w + 2), logits(at, None, F32, rules(n_history=1, history=w + 2), w),
+               logits(at, None, F32, rules(n_history=1, history=w, history_ptr=w + 1), w), logits(at, None, F32, rules(n_bias=1, bias_ids=w + 2, bias=at), w),
+               logits(at, None, F32, rules(n_bias=1, bias_ids=w, bias=at + 2), w), logits(at, None, F32, rules(n_bias=1, bias_ids=w, bias=at, bias_ptr=w + 2), w),
+               logits(at, None, F32, rules(mask=w + 2), w)):
+        assert rc == -2
+    assert backend.launch_count() == before
+    assert append(seqs(), at + 2, at + 514, F16) == 0 and attend(seqs(), attn(), at + 2, at + 4098, F16) == 0 and logits(at + 2, None, F16, None, w) == 0
+    torch.cuda.synchronize()
+    backend.check_status()
