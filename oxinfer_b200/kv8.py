@@ -121,9 +121,10 @@ class Kv8Cache:
         assert qs[2] == os[2] == 1 and qs[1] == os[1] == hd
         assert slopes is None or (slopes.dtype == self._f32 and slopes.numel() == nh and slopes.is_contiguous() and slopes.device == self.device)
         assert prefix is None or (prefix.dtype == self._torch.int32 and prefix.numel() == seqs.n_seqs and prefix.is_contiguous() and prefix.device == self.device)
+        assert window is None or window >= 0
         few = dtype == self._f32 or seqs.max_rows * nh <= 8 * self.nkv
         work = self._work() if few and seqs.max_blocks * BLOCK >= DEALT_FROM else None
-        a = _lib.Kv8Attention(nh, scale, cap, window or 0, None if slopes is None else slopes.data_ptr(), None if prefix is None else prefix.data_ptr(),
+        a = _lib.Kv8Attention(nh, scale, cap, min(window or 0, 0xFFFFFFFF), None if slopes is None else slopes.data_ptr(), None if prefix is None else prefix.data_ptr(),
                               None if work is None else work.data_ptr())
         be = self.backend
         return be._check(be._L.b2_attend_kv8_dev(be._ctx, self.handle, seqs._ref, C.byref(a), q.data_ptr(), qs[0], out.data_ptr(), os[0], self._codes[dtype]))

@@ -125,3 +125,13 @@ def test_addresses_between_elements_are_refused(backend):
     assert append(seqs(), at + 2, at + 514, F16) == 0 and attend(seqs(), attn(), at + 2, at + 4098, F16) == 0 and logits(at + 2, None, F16, None, w) == 0
     torch.cuda.synchronize()
     backend.check_status()
+
+
+def test_windows_that_32_bits_do_not_hold(backend):
+    for count in (1, 70):
+        s = Setting(backend, [200], [count], 2, 1, 64, "f16", seed=43)
+        want, out = s.check(), torch.empty_like(s.q)
+        for window in (None, 0, 2 ** 32 - 1, 2 ** 32, 2 ** 32 + 7, 2 ** 40 + 1):
+            assert s.cache.attend(s.seqs, s.q, out, scale=s.scale, window=window) and torch.equal(out, want), window
+        with pytest.raises(AssertionError):
+            s.cache.attend(s.seqs, s.q, out, scale=s.scale, window=-1)
