@@ -1367,10 +1367,8 @@ int DecodePlanImpl::generate(cudaStream_t st, uint64_t embed_handle, const Weigh
             PLAN_CUDA(cudaMemsetAsync(w, 0, 8 * 4, cap_stream_), "cudaMemset(rules)");
             PLAN_CUDA(launch_set_step(sp_, 0, 0, 0, token_, first_token, cap_stream_), "set_step");
             PLAN_CUDA(launch_dequantize(embed, 0, 1, input_, cap_stream_, token_), "embedding lookup");
-            LogitRulesDev none = gen_rules_.dev;
-            none.n_history = none.n_bias = 0;
-            none.mask = nullptr;
-            PLAN_CUDA(launch_logits(logits_, nullptr, B2_F32, n_logits_, n_logits_, 1, n_logits_, none, w + 4, status_, cap_stream_), "logits");
+            // (with the rules as they will be captured: another choice of lists is another kernel; the words say that the lists are empty)
+            PLAN_CUDA(launch_logits(logits_, nullptr, B2_F32, n_logits_, n_logits_, 1, n_logits_, gen_rules_.dev, w + 4, status_, cap_stream_), "logits");
             PLAN_CUDA(launch_advance(w + 4, token_, out_tokens_, w + 5, w, sp_, cap_stream_), "advance");
             PLAN_CUDA(cudaStreamSynchronize(cap_stream_), "generate warm-up");
             int rc = capture(cap_stream_, true, &gen_rules_exec_, err);
