@@ -11,9 +11,9 @@
 // tile the instruction's other eight carry the second f16 term of the queries (each row first multiplied by a power of two) and of the probabilities, 22 bits of
 // both: results of f32 accuracy at no further cost. Tiles of sixteen rows (f16 and bf16 results of many rows) have one term.
 //
-// What bounds it: long contexts HBM, at 4.5 to 4.9 TB/s of a measured 6.5 (750 instructions a block of 128 dimensions keep half of the issue slots busy, with three warps a scheduler to
+// What bounds it (times of replays; with cold caches one token over 2048 keys takes 10.3, over 131071 59, the 64 sequences with a cap 73): long contexts HBM, at 4.3 to 4.9 TB/s of a measured 6.5 (750 instructions a block of 128 dimensions keep half of the issue slots busy, with three warps a scheduler to
 // cover the softmax's chain); short ones latency: a launch, the first block, two to four blocks a warp one behind the other, the cluster's sums. 32 heads of 8 KV heads of 128, us: one
-// token over 2048 keys 7.9, over 131071 55.5; 64 sequences of up to 4096 67, with a cap 68.5. Steps: two CTAs an SM 110, three 84 (131071: 121), blocks dealt out over all of the GPU 76 and
+// token over 2048 keys 7.9, over 131071 54.9; 64 sequences of up to 4096 with a cap 67.1. f32 rows of a prompt take eight-row tiles, too: 2048 tokens behind 2048 820, 16-bit rows (attend_kv8_rows.cu) 112. Steps: two CTAs an SM 110, three 84 (131071: 121), blocks dealt out over all of the GPU 76 and
 // 68 (55), caps and sums two values an instruction 68.5 instead of 78.7 with a cap.
 #include <algorithm>
 #include <cfloat>
@@ -771,7 +771,8 @@ cudaError_t launch_attend_kv8(const Kv8Cache& c, const Kv8Seqs& s, const Kv8Attn
     if (s.n_seqs == 0 || s.n_rows == 0 || s.max_rows == 0) return cudaSuccess;
     // Many rows go to the form on tcgen05, from 64 of a KV head and sequence on.
     // mma.sync / tcgen05, us, 4 heads a KV head, 8 KV heads of 128, one sequence behind 4096 keys, eight behind 1024, 32 behind 512: 32 rows 14.2 / 17.7, 13.7 / 15.4, 22.9 / 28.6; 64 rows
-    // 14.9 / 18.3, 17.3 / 15.7, 29.0 / 25.8; 128 rows 19.8 / 19.5, 21.7 / 19.0, 50.7 / 29.9; 512 rows 50.5 / 30.5, 64.8 / 26.7, 167 / 52.
+    // 14.9 / 18.3, 17.3 / 15.7, 29.0 / 25.8; 128 rows 19.8 / 19.5, 21.7 / 19.0, 50.7 / 29.9; 512 rows 50.5 / 30.5, 64.8 / 26.7, 167 / 52. (One threshold for all numbers of sequences: the
+    // hint of a call's longest sequence changes its bits at one place only.)
     launched++;
     if ((dtype != B2_F32 || p.halves) && (size_t)s.max_rows * (p.nh / c.nkv) >= 64 && attend_kv8_rows_supports(c, s, p.nh))
         return launch_attend_kv8_rows(c, s, p, q, q_stride, out, out_stride, dtype, status, st, pdl);

@@ -17,7 +17,7 @@
 // What bounds it: a softmax warp's chain for a tile of keys, 3700 cycles without a cap (scores out of tensor memory and their largest 830, the row's two warps' meeting and the turn 870,
 // exponentials 1330 of which the exponential unit needs 1024, the rest waits for products), 5600 with one. The row tiles take turns at the exponentials: left to themselves they
 // meet there, and the tensor cores, 2048 cycles of 3700, idle while both wait for products (136 us instead of 110, turns handed on at half of them 119). 2048 tokens of 32 heads over 8 KV heads
-// of 128 behind 2048 more (103 GFLOP): 110 us, 940 TFLOP/s; with a cap 170 us. On mma.sync (attend_kv8.cu) 741 and 940. Steps, without / with a cap: bytes expanded by four
+// of 128 behind 2048 more (103 GFLOP): 112 us, 920 TFLOP/s; with a cap 170 us (replays). On mma.sync (attend_kv8.cu) 741 and 940. Steps, without / with a cap: bytes expanded by four
 // warps a block and everyone in step 164 us, a warp a block 142, descriptors in the warp's registers and places by turned bits 132, turns 115, a shorter start 106 / 187, two
 // warps a row 120 / 181, each with a block of both halves of the keys 110 / 170. Short prompts (five of 185 to 542 tokens with 12 heads 25.3 us, half of it in the
 // tiles) pay for the CTA's start: the largest scale of values is looked for by the warps that expand, while the others take in the queries, eight values a lane (33 us before; one warp
@@ -941,7 +941,7 @@ cudaError_t launch_attend_kv8_rows(const Kv8Cache& c, const Kv8Seqs& s, const Kv
     a.blocks = (uint32_t)blocks;
     a.Z = 1;
     // Shares of the keys while two fit the chip beside each other (of clusters of eight no more than fourteen do) and have two tiles each. 32 heads of 8 KV heads of 128
-    // behind 4096 keys, us without and with: 64 tokens 110 / 26, 512 tokens (64 CTAs) 81 / 52.
+    // behind 4096 keys, us without and with: 64 tokens 110 / 24, 512 tokens (64 CTAs) 81 / 49.
     while (a.Z < 8 && 2 * a.Z * blocks * c.nkv <= (a.Z == 4 ? 112 : 148) && 4 * a.Z * KT_BLOCKS <= s.max_blocks) a.Z *= 2;
     a.window = p.window <= 0x7fffffffu ? p.window : 0;
     a.q_sign = p.scale < 0.0f ? -1.0f : 1.0f;

@@ -3,7 +3,7 @@
 //
 // append: scale = 2^e, e the smallest with largest magnitude <= 127 * 2^e over the block's new rows (not below 2^-100), and not below the scale of the
 // rows of the block that stay; q = round half to even (x / scale), exact but for that rounding (at the scale 2^122 at most 63, so that the value is finite). Rows that stay are brought to a larger scale the same way.
-// What bounds it: a prompt of 8192 rows of 8 KV heads of 128 the issue slots beside HBM, f32 rows appended in 15.1 us (84 MB, 5.6 TB/s), bf16 in 12.7 (50 MB, 4 TB/s), read back in 14.2
+// What bounds it (times of replays with warm caches): a prompt of 8192 rows of 8 KV heads of 128 the issue slots beside HBM, f32 rows appended in 15.1 us (84 MB, 5.6 TB/s), bf16 in 12.7 (50 MB, 4 TB/s), read back in 14.2
 // (84 MB, 5.9 TB/s); a step of 64 sequences a launch and three dependent reads, 2.8 and 2.3 us.
 // A row with a value that is not finite is marked, and counts as NaN: it does not enter the scale, and the block's other rows are as they would be without it.
 #include "kv8.cuh"
@@ -72,7 +72,7 @@ __device__ __forceinline__ uint32_t top_bits(uint32_t top) {
 // Grid: (sequence, block of the rows', KV head), a CTA each: the unit's image in shared memory, then out of it 16 bytes a thread at a time. A thread has eight
 // dimensions (and eight of the other half of 128) of a token's keys and values. 8192 rows of 8 KV heads of 128, us, f32 and bf16: keys and values
 // a CTA each, four dimensions at a time and a barrier more a block 19.2 and 19.3, eight dimensions and six CTAs an SM 17.9 and 16.1, both kinds by one CTA 15.1 and 12.7 (that
-// halves what is done once a block; issue slots bound it, 78 % of them).
+// halves what is done once a block; issue slots bound it, 69 % of them).
 template <int HD, typename T>
 __global__ void __launch_bounds__(KV_THREADS, KV_CTAS) append_kernel(Kv8Cache c, Kv8Seqs sq, Kv8Rows x, uint32_t tiles, int keep_behind, int wide, uint32_t* status) {
     constexpr int J = HD / 64, UNIT = (int)unit_bytes(HD), WARPS = KV_THREADS / 32, IMAGE = (int)KV8_BLOCK * HD, WORDS = IMAGE / 16, V = 16 / (int)sizeof(T), PARTS = 8 / V;

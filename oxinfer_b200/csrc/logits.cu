@@ -8,7 +8,7 @@
 // atomics does not matter), every list read once by each CTA; the tokens that are on one are listed by whoever counts them first and changed, and the pass over the
 // logits, which were asked for before all that, takes those values where there are any. The CTAs' largest values go to the first one's shared memory.
 // What bounds it: a CTA's chain for a part (a list's bounds, its tokens, the counts, the changes, the pass), some 6 us for two to four CTAs an SM at a time, and
-// whole waves of them. One row of 128256 with 1500 tokens of history 6.9 us, 64 rows with 700 15.5 us (4.3 TB/s of 66.8 MB, half of it from L2), 256 bf16 rows of 32064
+// whole waves of them. Replays (cold caches 9.0, 24.6 and 28.3 us): one row of 128256 with 1500 tokens of history 6.9 us, 64 rows with 700 15.5 us (4.3 TB/s of 66.8 MB, half of it from L2), 256 bf16 rows of 32064
 // under all rules 22.6 us. Steps: changes made in the pass itself, where every warp met one, 8.3 / 32.7 / 39.1; tokens listed one warp's vote at a time 7.3 / 21.5 / 34
 // (gathered ahead of their counting, too, 8.1 / 25 / 39.5: the barriers cost more); not a CTA for every part of a row but whole waves of them 6.8 / 15.7 / 28.4; a warp's
 // votes for all of a thread's tokens at once 6.9 / 15.4 / 23.3; 16-bit logits two at a time 7.0 / 15.5 / 22.6.
